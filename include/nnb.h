@@ -30,7 +30,7 @@
 extern "C" {
 #endif
 
-#define NNB_ABI_VERSION 13
+#define NNB_ABI_VERSION 14
 
 enum nnb_status {
   NNB_OK = 0,
@@ -625,6 +625,79 @@ int32_t nnb_spline_resize(const nnb_spline_resize_args* args, void* stream);
  * 0, S - 1) (float64, one rounding per operation); the value is rounded once. */
 int32_t nnb_nearest_axis_resize(const double* source, int32_t channels, const int32_t source_dims[3],
                                 const int32_t target_dims[3], float* target, void* stream);
+
+/*
+ * Norms of channels-last rows (voxels or tokens) before and after a block, and
+ * the block's gated residual join.  No reference counterpart: they stand beside
+ * nnb_instance_norm_finalize and nnb_residual_join for blocks whose norm is
+ * taken over the channels of each row.  Values are read as float32, bfloat16 or
+ * float16 and computed in float32; weight, bias and scale are float32.
+ */
+enum nnb_type { NNB_F32 = 0, NNB_BF16 = 1, NNB_F16 = 2 };
+
+enum nnb_norm_kind { NNB_CHANNEL_NORM_NONE = 0, NNB_CHANNEL_NORM_RMS = 1, NNB_CHANNEL_NORM_LAYER = 2 };
+
+#define NNB_NORM_MAX_CHANNELS 16384 /* a row is held in registers */
+
+typedef struct nnb_channel_norm {
+  int32_t kind;        /* enum nnb_norm_kind */
+  float eps;           /* added to the mean square (rms) or the variance (layer); positive */
+  const float* weight; /* (channels) or NULL for 1 */
+  const float* bias;   /* (channels) or NULL for 0 */
+} nnb_channel_norm;
+
+typedef struct nnb_norm_args {
+  const void* x;   /* rows of `channels` values, x_stride elements apart (0: one row for all) */
+  void* out;       /* rows out_stride elements apart */
+  int64_t rows;
+  int64_t x_stride;
+  int64_t out_stride;
+  int32_t channels; /* 1 to NNB_NORM_MAX_CHANNELS */
+  int32_t x_type;   /* enum nnb_type */
+  int32_t out_type;
+  int32_t reserved; /* 0 */
+  nnb_channel_norm norm;
+} nnb_norm_args;
+
+/* out = norm(x), row by row. */
+int32_t nnb_channel_norm_rows(const nnb_norm_args* args, void* stream);
+
+/* What the gate of a join multiplies: nothing, each element, each row, or each channel of a sample. */
+enum nnb_gate_mode { NNB_GATE_NONE = 0, NNB_GATE_FULL = 1, NNB_GATE_ROW = 2, NNB_GATE_SAMPLE = 3 };
+enum nnb_gate_act { NNB_GATE_LINEAR = 0, NNB_GATE_SIGMOID = 1, NNB_GATE_SILU = 2, NNB_GATE_TANH = 3 };
+
+typedef struct nnb_join_args {
+  const void* branch; /* the block's output; rows branch_stride elements apart */
+  const void* skip;   /* the residual stream it joins */
+  const void* gate;   /* gate_mode FULL: (rows, channels); ROW: (rows); SAMPLE: (samples, channels);
+                         of the branch's type, rows gate_stride elements apart */
+  void* stream;       /* joined stream, of skip's type; may be skip itself with the same stride */
+  void* normed;       /* next(stream), or NULL without a next norm */
+  int64_t rows;
+  int64_t branch_stride;
+  int64_t skip_stride;
+  int64_t gate_stride;
+  int64_t stream_stride;
+  int64_t normed_stride;
+  int64_t rows_per_sample; /* gate_mode SAMPLE */
+  int32_t channels;        /* 1 to NNB_NORM_MAX_CHANNELS */
+  int32_t branch_type;     /* enum nnb_type: skip's type, or any when skip is float32 */
+  int32_t skip_type;
+  int32_t normed_type;
+  int32_t gate_mode;
+  int32_t gate_act;
+  float residual_scale;
+  int32_t reserved;   /* 0 */
+  const float* scale; /* (channels) or NULL for 1 */
+  nnb_channel_norm post;
+  nnb_channel_norm next;
+} nnb_join_args;
+
+/*
+ * stream = skip + residual_scale * scale * act(gate) * post(branch), and
+ * normed = next(stream) of the float32 stream (before its rounding to skip's type).
+ */
+int32_t nnb_gated_join(const nnb_join_args* args, void* stream);
 
 #ifdef __cplusplus
 }

@@ -16,7 +16,7 @@ from pathlib import Path
 from nnunet_mlx_b200.errors import ContractError
 
 LIB_PATH = Path(__file__).resolve().parent / "_nnb.so"
-ABI_VERSION = 13
+ABI_VERSION = 14
 
 PREC_FP32 = 0        # split fp16 pairs on the tensor cores, float32-level accuracy (|activation| < 65504)
 PREC_TF32 = 1        # single-pass TF32 tensor cores
@@ -90,6 +90,33 @@ class TorchResizeArgs(ctypes.Structure):
                 ("source_dims", I32x3), ("channel_stride", ctypes.c_int64), ("source_strides", I64x3),
                 ("target_dims", I32x3), ("mode", ctypes.c_int32), ("tiebreak", ctypes.c_int32),
                 ("target", ctypes.c_void_p)]
+
+
+# value types of the row operators (enum nnb_type)
+F32, BF16, F16 = 0, 1, 2
+
+
+class ChannelNorm(ctypes.Structure):
+    _fields_ = [("kind", ctypes.c_int32), ("eps", ctypes.c_float), ("weight", ctypes.c_void_p),
+                ("bias", ctypes.c_void_p)]
+
+
+class NormArgs(ctypes.Structure):
+    _fields_ = [("x", ctypes.c_void_p), ("out", ctypes.c_void_p), ("rows", ctypes.c_int64),
+                ("x_stride", ctypes.c_int64), ("out_stride", ctypes.c_int64), ("channels", ctypes.c_int32),
+                ("x_type", ctypes.c_int32), ("out_type", ctypes.c_int32), ("reserved", ctypes.c_int32),
+                ("norm", ChannelNorm)]
+
+
+class JoinArgs(ctypes.Structure):
+    _fields_ = [("branch", ctypes.c_void_p), ("skip", ctypes.c_void_p), ("gate", ctypes.c_void_p),
+                ("stream", ctypes.c_void_p), ("normed", ctypes.c_void_p), ("rows", ctypes.c_int64),
+                ("branch_stride", ctypes.c_int64), ("skip_stride", ctypes.c_int64), ("gate_stride", ctypes.c_int64),
+                ("stream_stride", ctypes.c_int64), ("normed_stride", ctypes.c_int64),
+                ("rows_per_sample", ctypes.c_int64), ("channels", ctypes.c_int32), ("branch_type", ctypes.c_int32),
+                ("skip_type", ctypes.c_int32), ("normed_type", ctypes.c_int32), ("gate_mode", ctypes.c_int32),
+                ("gate_act", ctypes.c_int32), ("residual_scale", ctypes.c_float), ("reserved", ctypes.c_int32),
+                ("scale", ctypes.c_void_p), ("post", ChannelNorm), ("next", ChannelNorm)]
 
 
 SYMBOLS = {
@@ -170,6 +197,8 @@ SYMBOLS = {
     "nnb_spline_resize": (ctypes.c_int32, [ctypes.POINTER(SplineResizeArgs), ctypes.c_void_p]),
     "nnb_nearest_axis_resize": (ctypes.c_int32, [ctypes.c_void_p, ctypes.c_int32, I32x3, I32x3, ctypes.c_void_p,
                                                  ctypes.c_void_p]),
+    "nnb_channel_norm_rows": (ctypes.c_int32, [ctypes.POINTER(NormArgs), ctypes.c_void_p]),
+    "nnb_gated_join": (ctypes.c_int32, [ctypes.POINTER(JoinArgs), ctypes.c_void_p]),
 }
 
 _lib: ctypes.CDLL | None = None

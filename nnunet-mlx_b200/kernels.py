@@ -952,3 +952,226 @@ def nearest_axis_resize(source: torch.Tensor, target) -> torch.Tensor:
                                                          _native.dims3(source.shape[1:]), _native.dims3(target),
                                                          out.data_ptr(), _stream()), "nearest_axis_resize")
     return out
+
+
+# ---------------------------------------------------------------------------
+# Channel norms and gated joins of channels-last rows (voxels or tokens)
+# ---------------------------------------------------------------------------
+_ROW_TYPES = {torch.float32: _native.F32, torch.bfloat16: _native.BF16, torch.float16: _native.F16}
+_CHANNEL_NORMS = {"rms": 1, "layer": 2}
+_GATE_ACTS = {"none": 0, "sigmoid": 1, "silu": 2, "tanh": 3}
+_NO_NORM = _native.ChannelNorm()
+
+
+@dataclass(frozen=True)
+class ChannelNorm:
+    """A norm over the channels of each row, in float32.
+
+    ``"rms"``: ``x / sqrt(mean(x^2) + eps) * weight + bias``; ``"layer"``
+    subtracts the row's mean first and divides by its standard deviation.
+    ``weight`` and ``bias`` are contiguous float32 ``(C,)`` CUDA tensors, or
+    ``None`` for one and zero.  A row whose square sum leaves float32's range
+    gives what float32 arithmetic gives.
+    """
+
+    kind: str = "rms"
+    weight: torch.Tensor | None = None
+    bias: torch.Tensor | None = None
+    eps: float = 1e-6
+
+    def __post_init__(self) -> None:
+        if self.kind not in _CHANNEL_NORMS:
+            raise ContractError(f"unknown channel norm {self.kind!r}: one of {', '.join(_CHANNEL_NORMS)}")
+        if not 0.0 < float(self.eps) < math.inf:
+            raise ContractError(f"a channel norm's eps must be positive, got {self.eps}")
+
+    def arguments(self, channels: int, device: torch.device) -> _native.ChannelNorm:
+        for name, p in (("weight", self.weight), ("bias", self.bias)):
+            _check_channels(p, f"norm {name}", channels, device)
+        return _native.ChannelNorm(_CHANNEL_NORMS[self.kind], self.eps, _ptr(self.weight), _ptr(self.bias))
+
+
+def _check_channels(p: torch.Tensor | None, name: str, channels: int, device: torch.device) -> None:
+    """A per-channel float32 parameter, or none."""
+    if p is None:
+        return
+    _check_tensor(p, name)
+    if p.shape != (channels,) or p.device != device:
+        raise ContractError(f"{name} must hold {channels} values on {device}, "
+                            f"got {tuple(p.shape)} on {p.device}")
+
+
+def _check_rows(t: torch.Tensor, name: str) -> None:
+    if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype not in _ROW_TYPES:
+        raise ContractError(f"{name} must be a float32, bfloat16 or float16 CUDA tensor")
+    if t.dim() < 1 or t.shape[-1] < 1:
+        raise ContractError(f"{name} must have channels in its last axis, got shape {tuple(t.shape)}")
+    if t.requires_grad and torch.is_grad_enabled():
+        raise ContractError(f"{name} requires a gradient: this operator has no backward pass "
+                            "(call it under torch.no_grad())")
+
+
+def _row_stride(t: torch.Tensor, name: str) -> int:
+    """Elements between the rows (all leading axes, flattened) of a tensor whose channels are contiguous."""
+    channels = t.shape[-1]
+    if t.is_contiguous():
+        return channels
+    if channels == 1 or t.stride(-1) == 1:
+        axes = [(n, st) for n, st in zip(t.shape[:-1], t.stride()[:-1]) if n != 1]
+        if all(outer == n * inner for (_, outer), (n, inner) in zip(axes, axes[1:])):
+            return axes[-1][1] if axes else channels
+    raise ContractError(f"the rows of {name} must be evenly spaced with contiguous channels, "
+                        f"got shape {tuple(t.shape)} with strides {t.stride()}")
+
+
+def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether the address ranges of two tensors meet."""
+    def span(t):
+        start = t.data_ptr()
+        return start, start + t.element_size() * (1 + sum((n - 1) * st for n, st in zip(t.shape, t.stride())))
+
+    if a.numel() == 0 or b.numel() == 0:
+        return False
+    (a0, a1), (b0, b1) = span(a), span(b)
+    return a0 < b1 and b0 < a1
+
+
+def _check_out(out: torch.Tensor, name: str, shape, dtype: torch.dtype, device: torch.device) -> int:
+    """A caller's output tensor; returns its row stride."""
+    _check_rows(out, name)
+    if out.shape != shape or out.dtype != dtype or out.device != device:
+        raise ContractError(f"{name} must be a {dtype} tensor of shape {tuple(shape)} on {device}")
+    stride = _row_stride(out, name)
+    if stride < out.shape[-1] and math.prod(shape[:-1]) > 1:
+        raise ContractError(f"the rows of {name} overlap one another")
+    return stride
+
+
+def _call_rows(function, args, device: torch.device, what: str) -> None:
+    """A row operator's launch, on ``device``'s current stream."""
+    if device.index == torch.cuda.current_device():
+        _native.check(function(ctypes.byref(args), _stream()), what)
+    else:
+        with torch.cuda.device(device):
+            _native.check(function(ctypes.byref(args), _stream()), what)
+
+
+def channel_norm(x: torch.Tensor, norm: ChannelNorm, *, out_dtype: torch.dtype | None = None,
+                 out: torch.Tensor | None = None) -> torch.Tensor:
+    """``norm`` of each row of ``x`` (``(..., C)``, contiguous channels, evenly spaced rows).
+
+    ``x`` is float32, bfloat16 or float16 and the result ``out_dtype`` of the
+    three (``x``'s by default), computed in float32 and rounded once; up to
+    16384 channels.  ``out`` receives the result: it may be ``x`` itself, and
+    shares no memory with the other inputs or with part of ``x``.
+    """
+    _check_rows(x, "x")
+    shape, device = x.shape, x.device
+    channels = shape[-1]
+    dtype = out_dtype or (x.dtype if out is None else out.dtype)
+    if dtype not in _ROW_TYPES:
+        raise ContractError(f"out_dtype must be float32, bfloat16 or float16, got {dtype}")
+    x_stride = _row_stride(x, "x")
+    n = norm.arguments(channels, device)
+    if out is None:
+        out, out_stride = torch.empty(shape, dtype=dtype, device=device), channels
+    else:
+        out_stride = _check_out(out, "out", shape, dtype, device)
+        same = out.data_ptr() == x.data_ptr() and out_stride == x_stride and dtype == x.dtype
+        for name, t in (("x", None if same else x), ("weight", norm.weight), ("bias", norm.bias)):
+            if t is not None and _overlap(out, t):
+                raise ContractError(f"out overlaps {name}")
+    rows = out.numel() // channels
+    if rows == 0:
+        return out
+    args = _native.NormArgs(x.data_ptr(), out.data_ptr(), rows, x_stride, out_stride, channels,
+                            _ROW_TYPES[x.dtype], _ROW_TYPES[dtype], 0, n)
+    token = PROFILE.start("channel_norm", 0.0, float(rows * channels * (x.element_size() + out.element_size())))
+    _call_rows(_native.load().nnb_channel_norm_rows, args, device, "channel_norm")
+    PROFILE.stop(token)
+    return out
+
+
+def gated_residual_join(branch: torch.Tensor, skip: torch.Tensor, *, post: ChannelNorm | None = None,
+                        gate: torch.Tensor | None = None, gate_act: str = "none",
+                        scale: torch.Tensor | None = None, residual_scale: float = 1.0,
+                        next_norm: ChannelNorm | None = None, next_dtype: torch.dtype | None = None,
+                        out: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor | None]:
+    """A block's join with its residual stream, and the next block's norm, in one pass over the rows.
+
+    ``stream = skip + residual_scale * scale * act(gate) * post(branch)`` and
+    ``normed = next_norm(stream)``; returns ``(stream, normed)``, ``normed``
+    being ``None`` without ``next_norm``.
+
+    ``branch`` and ``skip`` are ``(..., C)`` rows of one shape; ``branch`` has
+    ``skip``'s type, or ``skip`` is float32.  ``gate``, of ``branch``'s type,
+    multiplies each element (``branch``'s shape), each row (``(..., 1)``) or
+    each channel of a sample (``(B, C)`` beside a ``(B, ..., C)`` branch, or
+    ``(1, C)``), through ``gate_act`` (``"none"``, ``"sigmoid"``, ``"silu"``,
+    ``"tanh"``).  ``scale`` is a float32 ``(C,)`` factor.  Everything is
+    computed in float32; the stream is rounded to ``skip``'s type where it is
+    stored, the normed rows (``next_dtype``, by default ``branch``'s type) are
+    taken from the unrounded stream.  ``out`` receives the stream: it may be
+    ``skip`` itself, and shares no memory with the other inputs.
+    """
+    _check_rows(branch, "branch")
+    _check_rows(skip, "skip")
+    shape, device = branch.shape, branch.device
+    if skip.shape != shape or skip.device != device:
+        raise ContractError(f"residual shapes differ: {tuple(shape)} on {device} vs {tuple(skip.shape)} "
+                            f"on {skip.device}")
+    if branch.dtype != skip.dtype and skip.dtype != torch.float32:
+        raise ContractError(f"a {branch.dtype} branch joins a stream of its own type or a float32 one, "
+                            f"got {skip.dtype}")
+    if gate_act not in _GATE_ACTS:
+        raise ContractError(f"unknown gate activation {gate_act!r}: one of {', '.join(_GATE_ACTS)}")
+    channels = shape[-1]
+    _check_channels(scale, "scale", channels, device)
+    rows = math.prod(shape[:-1])
+    mode, gate_stride, per_sample = 0, 0, 0
+    if gate is not None:
+        _check_rows(gate, "gate")
+        if gate.dtype != branch.dtype or gate.device != device:
+            raise ContractError(f"the gate must have the branch's type and device, got {gate.dtype} on {gate.device}")
+        if gate.shape == shape:
+            mode = 1
+        elif gate.shape == (*shape[:-1], 1):
+            mode = 2
+        elif gate.shape == (1, channels) or (len(shape) > 2 and gate.shape == (shape[0], channels)):
+            mode, per_sample = 3, max(1, rows // max(1, gate.shape[0]))
+        else:
+            raise ContractError(f"a gate of shape {tuple(gate.shape)} fits no element, row or sample of "
+                                f"{tuple(shape)}")
+        gate_stride = _row_stride(gate, "gate")
+    branch_stride, skip_stride = _row_stride(branch, "branch"), _row_stride(skip, "skip")
+    post_args = _NO_NORM if post is None else post.arguments(channels, device)
+    next_args = _NO_NORM if next_norm is None else next_norm.arguments(channels, device)
+    if out is None:
+        out, out_stride = torch.empty(shape, dtype=skip.dtype, device=device), channels
+    else:
+        out_stride = _check_out(out, "out", shape, skip.dtype, device)
+        same = out.data_ptr() == skip.data_ptr() and out_stride == skip_stride
+        others = [("branch", branch), ("gate", gate), ("scale", scale), ("skip", None if same else skip)]
+        others += [(f"a norm's {part}", getattr(n, part)) for n in (post, next_norm) if n is not None
+                   for part in ("weight", "bias")]
+        for name, t in others:
+            if t is not None and _overlap(out, t):
+                raise ContractError(f"out overlaps {name}")
+    normed, normed_type = None, 0
+    if next_norm is not None:
+        dtype = next_dtype or branch.dtype
+        if dtype not in _ROW_TYPES:
+            raise ContractError(f"next_dtype must be float32, bfloat16 or float16, got {dtype}")
+        normed, normed_type = torch.empty(shape, dtype=dtype, device=device), _ROW_TYPES[dtype]
+    if rows == 0:
+        return out, normed
+    args = _native.JoinArgs(branch.data_ptr(), skip.data_ptr(), _ptr(gate), out.data_ptr(), _ptr(normed), rows,
+                            branch_stride, skip_stride, gate_stride, out_stride, channels, per_sample, channels,
+                            _ROW_TYPES[branch.dtype], _ROW_TYPES[skip.dtype], normed_type, mode,
+                            _GATE_ACTS[gate_act], residual_scale, 0, _ptr(scale), post_args, next_args)
+    nbytes = (branch.element_size() + 2 * skip.element_size() + (0 if normed is None else normed.element_size())
+              + (gate.element_size() if mode == 1 else 0))
+    token = PROFILE.start("gated_residual_join", 0.0, float(nbytes) * rows * channels)
+    _call_rows(_native.load().nnb_gated_join, args, device, "gated_residual_join")
+    PROFILE.stop(token)
+    return out, normed

@@ -30,7 +30,7 @@
 extern "C" {
 #endif
 
-#define NNB_ABI_VERSION 14
+#define NNB_ABI_VERSION 15
 
 enum nnb_status {
   NNB_OK = 0,
@@ -698,6 +698,46 @@ typedef struct nnb_join_args {
  * normed = next(stream) of the float32 stream (before its rounding to skip's type).
  */
 int32_t nnb_gated_join(const nnb_join_args* args, void* stream);
+
+/*
+ * Projection of rows shared by many requests, with each request's low-rank
+ * adapter beside it.  No reference counterpart: it stands beside nnb_conv3d's
+ * 1x1x1 convolutions for rows of bfloat16 or float16 whose requests (samples,
+ * tokens) each bring a fine-tuned variant of the same projection.
+ *
+ *   out_t = W x_t + bias + scale_a up_a (down_a x_t),  a = index[t / rows_per_index], -1 for none
+ *
+ * An index outside [-1, adapters) gives its rows the shared projection alone
+ * and records NNB_E_DEVICE for nnb_device_status.
+ */
+#define NNB_PROJECT_MAX_RANK 256
+
+typedef struct nnb_project_args {
+  const void* x;        /* rows of k values, x_stride elements apart (0: one row for all) */
+  const void* weight;   /* (n, weight_stride), x's type; columns from k on are zero */
+  const void* down;     /* (adapters, rank, weight_stride), x's type; zero from each adapter's rank and from k on */
+  const void* up;       /* (adapters, n, rank) bfloat16 for bfloat16 rows; (adapters, n, 2, rank) bfloat16 for
+                           float16 rows: the values rounded to bfloat16, then what the rounding left */
+  const float* scales;  /* (adapters) */
+  const float* bias;    /* (n) or NULL */
+  const int32_t* index; /* an adapter, or -1, for each rows_per_index rows */
+  void* out;            /* rows out_stride elements apart, x's type */
+  float* low;           /* workspace of nnb_project_workspace_bytes(args) bytes, 16-byte aligned */
+  int64_t rows;         /* below 2^31 */
+  int64_t x_stride;
+  int64_t out_stride;
+  int64_t rows_per_index;
+  int64_t weight_stride; /* a multiple of 8 */
+  int32_t k;
+  int32_t n;
+  int32_t adapters;
+  int32_t rank; /* the adapters' largest rank rounded up to a multiple of 16 */
+  int32_t type; /* NNB_BF16 or NNB_F16 */
+  int32_t reserved; /* 0 */
+} nnb_project_args;
+
+int64_t nnb_project_workspace_bytes(const nnb_project_args* args);
+int32_t nnb_project(const nnb_project_args* args, void* stream);
 
 #ifdef __cplusplus
 }

@@ -16,7 +16,7 @@ from pathlib import Path
 from nnunet_mlx_b200.errors import ContractError
 
 LIB_PATH = Path(__file__).resolve().parent / "_nnb.so"
-ABI_VERSION = 14
+ABI_VERSION = 15
 
 PREC_FP32 = 0        # split fp16 pairs on the tensor cores, float32-level accuracy (|activation| < 65504)
 PREC_TF32 = 1        # single-pass TF32 tensor cores
@@ -94,6 +94,7 @@ class TorchResizeArgs(ctypes.Structure):
 
 # value types of the row operators (enum nnb_type)
 F32, BF16, F16 = 0, 1, 2
+PROJECT_MAX_RANK = 256
 
 
 class ChannelNorm(ctypes.Structure):
@@ -117,6 +118,16 @@ class JoinArgs(ctypes.Structure):
                 ("skip_type", ctypes.c_int32), ("normed_type", ctypes.c_int32), ("gate_mode", ctypes.c_int32),
                 ("gate_act", ctypes.c_int32), ("residual_scale", ctypes.c_float), ("reserved", ctypes.c_int32),
                 ("scale", ctypes.c_void_p), ("post", ChannelNorm), ("next", ChannelNorm)]
+
+
+class ProjectArgs(ctypes.Structure):
+    _fields_ = [("x", ctypes.c_void_p), ("weight", ctypes.c_void_p), ("down", ctypes.c_void_p),
+                ("up", ctypes.c_void_p), ("scales", ctypes.c_void_p), ("bias", ctypes.c_void_p),
+                ("index", ctypes.c_void_p), ("out", ctypes.c_void_p), ("low", ctypes.c_void_p),
+                ("rows", ctypes.c_int64), ("x_stride", ctypes.c_int64), ("out_stride", ctypes.c_int64),
+                ("rows_per_index", ctypes.c_int64), ("weight_stride", ctypes.c_int64), ("k", ctypes.c_int32),
+                ("n", ctypes.c_int32), ("adapters", ctypes.c_int32), ("rank", ctypes.c_int32),
+                ("type", ctypes.c_int32), ("reserved", ctypes.c_int32)]
 
 
 SYMBOLS = {
@@ -199,6 +210,8 @@ SYMBOLS = {
                                                  ctypes.c_void_p]),
     "nnb_channel_norm_rows": (ctypes.c_int32, [ctypes.POINTER(NormArgs), ctypes.c_void_p]),
     "nnb_gated_join": (ctypes.c_int32, [ctypes.POINTER(JoinArgs), ctypes.c_void_p]),
+    "nnb_project_workspace_bytes": (ctypes.c_int64, [ctypes.POINTER(ProjectArgs)]),
+    "nnb_project": (ctypes.c_int32, [ctypes.POINTER(ProjectArgs), ctypes.c_void_p]),
 }
 
 _lib: ctypes.CDLL | None = None

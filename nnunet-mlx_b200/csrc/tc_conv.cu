@@ -1979,16 +1979,26 @@ int launch_conv_transpose_tc(const nnb_segment& in, int batch, const int32_t in_
 
 }  // namespace nnb
 
+namespace nnb {
+int project_device_status(int32_t* where, bool reset);  // project.cu
+}
+
 extern "C" int32_t nnb_device_status(int32_t* where, int32_t reset) {
   int status = 0, loc = 0;
   if (cudaDeviceSynchronize() != cudaSuccess) return NNB_E_CUDA;
   if (cudaMemcpyFromSymbol(&status, nnb::g_device_status, sizeof(int)) != cudaSuccess) return NNB_E_CUDA;
   cudaMemcpyFromSymbol(&loc, nnb::g_device_status_where, sizeof(int));
-  if (where) *where = loc;
   if (reset) {
     const int zero = 0;
     cudaMemcpyToSymbol(nnb::g_device_status, &zero, sizeof(int));
     cudaMemcpyToSymbol(nnb::g_device_status_where, &zero, sizeof(int));
   }
+  int project_loc = 0;
+  const int project_status = nnb::project_device_status(&project_loc, reset != 0);
+  if (status == 0) {
+    status = project_status;
+    loc = project_loc;
+  }
+  if (where) *where = loc;
   return status;
 }

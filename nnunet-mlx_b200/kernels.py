@@ -1175,3 +1175,148 @@ def gated_residual_join(branch: torch.Tensor, skip: torch.Tensor, *, post: Chann
     _call_rows(_native.load().nnb_gated_join, args, device, "gated_residual_join")
     PROFILE.stop(token)
     return out, normed
+
+
+# ---------------------------------------------------------------------------
+# Projection shared by many requests, with each request's low-rank adapter
+# ---------------------------------------------------------------------------
+@dataclass(frozen=True)
+class Adapter:
+    """A low-rank change of a projection: ``scale * up @ down`` added to its ``(N, K)`` weight.
+
+    ``down`` is ``(r, K)`` and ``up`` ``(N, r)``, of the weight's type.
+    """
+
+    down: torch.Tensor
+    up: torch.Tensor
+    scale: float = 1.0
+
+
+@dataclass(frozen=True)
+class AdaptedProjection:
+    """A projection and its adapters, laid out for ``adapted_projection`` by ``pack_projection``."""
+
+    weight: torch.Tensor       # (N, K rounded up to 8)
+    down: torch.Tensor         # (adapters, R, K rounded up to 8), R the largest rank rounded up to 16
+    up: torch.Tensor           # (adapters, N, planes, R) bfloat16
+    scales: torch.Tensor       # (adapters,) float32
+    bias: torch.Tensor | None  # (N,) float32
+    in_channels: int
+
+    @property
+    def out_channels(self) -> int:
+        return int(self.weight.shape[0])
+
+    @property
+    def adapters(self) -> int:
+        return int(self.down.shape[0])
+
+
+def pack_projection(weight: torch.Tensor, adapters: list[Adapter],
+                    bias: torch.Tensor | None = None) -> AdaptedProjection:
+    """Lay out a shared ``(N, K)`` projection and its adapters once, for ``adapted_projection``.
+
+    ``weight`` is bfloat16 or float16, ``bias`` float32 ``(N,)``.  The packed
+    tensors are copies: later changes of the originals do not reach them.
+    Adapters may differ in rank (1 to 256) and must be finite, since a tile of
+    rows of several requests multiplies each adapter by the others' zeros
+    (read once here, which synchronises).
+    """
+    for name, t in (("weight", weight), *((f"adapter {part}", getattr(a, part)) for a in adapters
+                                          for part in ("down", "up"))):
+        if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype not in (torch.bfloat16, torch.float16):
+            raise ContractError(f"{name} must be a bfloat16 or float16 CUDA tensor")
+        if t.dim() != 2 or min(t.shape) < 1 or t.dtype != weight.dtype or t.device != weight.device:
+            raise ContractError(f"{name} must be a matrix of the weight's type and device, got "
+                                f"{tuple(t.shape)} {t.dtype} on {t.device}")
+    if not adapters:
+        raise ContractError("an adapted projection needs at least one adapter")
+    n, k = (int(v) for v in weight.shape)
+    device, dtype = weight.device, weight.dtype
+    _check_channels(bias, "projection bias", n, device)
+    for i, a in enumerate(adapters):
+        if a.down.shape[1] != k or a.up.shape != (n, a.down.shape[0]):
+            raise ContractError(f"adapter {i}: down {tuple(a.down.shape)} and up {tuple(a.up.shape)} do not fit a "
+                                f"{n} x {k} projection")
+        if a.down.shape[0] > _native.PROJECT_MAX_RANK:
+            raise ContractError(f"adapter {i}: rank {a.down.shape[0]} above {_native.PROJECT_MAX_RANK}")
+        if not math.isfinite(a.scale):
+            raise ContractError(f"adapter {i}: scale must be finite, got {a.scale}")
+    with torch.no_grad():
+        rank = max(-(-int(a.down.shape[0]) // 16) * 16 for a in adapters)
+        stride = -(-k // 8) * 8
+        packed = torch.zeros((n, stride), dtype=dtype, device=device)
+        packed[:, :k] = weight
+        down = torch.zeros((len(adapters), rank, stride), dtype=dtype, device=device)
+        # bfloat16 planes on the up side: float16 values are a bfloat16 and an exact remainder
+        up = torch.zeros((len(adapters), n, 1 if dtype == torch.bfloat16 else 2, rank), dtype=torch.bfloat16,
+                         device=device)
+        for i, a in enumerate(adapters):
+            r = int(a.down.shape[0])
+            down[i, :r, :k] = a.down
+            up[i, :, 0, :r] = a.up
+            if dtype == torch.float16:
+                up[i, :, 1, :r] = a.up.float() - up[i, :, 0, :r].float()
+        if not bool(torch.isfinite(down).all() & torch.isfinite(up).all()):
+            raise ContractError("adapters must be finite")
+        scales = torch.tensor([float(a.scale) for a in adapters], dtype=torch.float32, device=device)
+        return AdaptedProjection(packed, down, up, scales, None if bias is None else bias.detach().clone(), k)
+
+
+def adapted_projection(x: torch.Tensor, projection: AdaptedProjection, index: torch.Tensor, *,
+                       out: torch.Tensor | None = None) -> torch.Tensor:
+    """``x W^T + bias`` of every row, plus ``scale x down^T up^T`` of the adapter its request names.
+
+    ``x`` is ``(..., K)`` rows of the projection's type (contiguous channels,
+    evenly spaced rows).  ``index`` is a contiguous int32 tensor over leading
+    axes of ``x``: one adapter, or -1 for none, per row (``x.shape[:-1]``) or
+    per sample (``x.shape[:1]`` and so on).  An index out of range gives its
+    rows the shared projection alone and is reported by
+    ``_native.device_status``.  Products are accumulated in float32, the
+    low-rank rows are kept to 16 bits of mantissa or more, and the result is
+    rounded once to the projection's type.  ``out`` receives the result and
+    shares no memory with the inputs.
+
+    Rows of one request that follow one another share the reading of its
+    adapter; any order gives the same values.
+    """
+    _check_rows(x, "x")
+    if not isinstance(projection, AdaptedProjection):
+        raise ContractError("adapted_projection takes a projection packed by pack_projection")
+    weight, device, shape = projection.weight, x.device, x.shape
+    if x.dtype != weight.dtype or device != weight.device or shape[-1] != projection.in_channels:
+        raise ContractError(f"x must hold {projection.in_channels} {weight.dtype} channels on {weight.device}, got "
+                            f"{tuple(shape)} {x.dtype} on {device}")
+    axes = index.dim()
+    if index.dtype != torch.int32 or not index.is_contiguous() or index.device != device \
+            or not 1 <= axes < len(shape) or index.shape != shape[:axes]:
+        raise ContractError(f"index must be a contiguous int32 tensor over leading axes of {tuple(shape)} on {device}, "
+                            f"got {tuple(index.shape)} {index.dtype} on {index.device}")
+    n, rank = int(weight.shape[0]), int(projection.down.shape[1])
+    x_stride = _row_stride(x, "x")
+    if out is None:
+        out, out_stride = torch.empty((*shape[:-1], n), dtype=x.dtype, device=device), n
+    else:
+        out_stride = _check_out(out, "out", (*shape[:-1], n), x.dtype, device)
+        for name, t in (("x", x), ("index", index), ("the projection", weight), ("the projection", projection.down),
+                        ("the projection", projection.up), ("the projection", projection.bias)):
+            if t is not None and _overlap(out, t):
+                raise ContractError(f"out overlaps {name}")
+    rows = out.numel() // n
+    if rows == 0:
+        return out
+    args = _native.ProjectArgs(x.data_ptr(), weight.data_ptr(), projection.down.data_ptr(),
+                               projection.up.data_ptr(), projection.scales.data_ptr(), _ptr(projection.bias),
+                               index.data_ptr(), out.data_ptr(), 0, rows, x_stride, out_stride,
+                               math.prod(shape[axes:-1]), weight.shape[1], shape[-1], n, projection.down.shape[0],
+                               rank, _ROW_TYPES[x.dtype], 0)
+    nbytes = int(_native.load().nnb_project_workspace_bytes(ctypes.byref(args)))
+    if nbytes < 0:
+        _native.check(nbytes, "adapted_projection")
+    workspace = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    args.low = workspace.data_ptr()
+    token = PROFILE.start("adapted_projection", 2.0 * rows * (n * shape[-1] + rank * (n + shape[-1])),
+                          2.0 * (rows * (n + shape[-1]) + n * shape[-1]), launches=2)
+    _call_rows(_native.load().nnb_project, args, device, "adapted_projection")
+    PROFILE.stop(token)
+    return out

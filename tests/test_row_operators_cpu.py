@@ -94,9 +94,36 @@ def test_c_entry_refuses_types_of_a_join():
     assert _native.load().nnb_channel_norm_rows(None, None) == -1
 
 
+def _project_args(**over):
+    values = dict(x=16, weight=16, down=16, up=16, scales=16, bias=0, index=16, out=16, low=16, rows=2, x_stride=8,
+                  out_stride=8, rows_per_index=1, weight_stride=8, k=8, n=8, adapters=1, rank=16, type=_native.BF16)
+    values.update(over)
+    return _native.ProjectArgs(**values)
+
+
+@pytest.mark.parametrize("over", [
+    *(dict([(name, 0)]) for name in ("x", "weight", "down", "up", "scales", "index", "out", "low", "rows", "k", "n",
+                                     "adapters", "rank", "rows_per_index")),
+    dict(rows=2 ** 31), dict(rank=8), dict(rank=272), dict(rank=24), dict(type=_native.F32), dict(x_stride=-1),
+    dict(out_stride=7), dict(weight_stride=0), dict(weight_stride=12), dict(weight=18), dict(down=8), dict(up=4),
+    dict(low=20)])
+def test_c_entry_refuses_projection(over):
+    args = _project_args(**over)
+    assert _native.load().nnb_project(ctypes.byref(args), None) == -1
+    assert b"project" in _native.load().nnb_last_error()
+
+
+def test_projection_workspace():
+    load = _native.load()
+    assert load.nnb_project_workspace_bytes(ctypes.byref(_project_args(rows=10, rank=32))) >= 10 * 32 * 4
+    assert load.nnb_project_workspace_bytes(ctypes.byref(_project_args(rows=0))) == -1
+    assert load.nnb_project_workspace_bytes(None) == -1
+    assert load.nnb_project(None, None) == -1
+
+
 def test_structures_match_the_header(tmp_path):
     names = {"nnb_channel_norm": _native.ChannelNorm, "nnb_norm_args": _native.NormArgs,
-             "nnb_join_args": _native.JoinArgs}
+             "nnb_join_args": _native.JoinArgs, "nnb_project_args": _native.ProjectArgs}
     lines = []
     for c_name, struct in names.items():
         lines.append(f'printf("{c_name} %zu\\n", sizeof({c_name}));')

@@ -4,25 +4,102 @@
 //   out_t = W x_t + bias + up_a (scale_a down_a x_t),   a = the adapter of row t's request, or none
 //
 // down_a has the adapter's rank of rows, up_a that many columns; both are
-// padded with zeros to a common multiple of 16.  The low-rank rows
-// scale_a down_a x_t are float32 in a workspace.
+// padded with zeros to a common multiple of 16.
+//
+// project_low_kernel computes the low-rank rows scale_a down_a x_t in float32.
+// project_kernel is a tcgen05 GEMM over tiles of 128 rows x BN columns whose K
+// axis goes on past W's channels: for every adapter among a tile's rows it
+// appends the adapter's ranks, with the rows of other requests set to zero.
+// So adapters cost a tile a few more K-steps into the same accumulator, and
+// need neither sorting of the rows nor a pass over the output; requests whose
+// rows follow one another keep the number of adapters of a tile small.
+//
+// Roles of project_kernel's warps:
+//   0      TMA producer of x and W chunks (64 channels a stage, 128-byte swizzle)
+//   1      MMA issuer (one thread) and TMEM owner
+//   2-5    adapter producers, a thread per row: list the tile's adapters, and
+//          for each write the rows' low-rank values into a stage, as two
+//          bfloat16 parts hi + lo (2^-17 of the value at most is lost; a single
+//          bfloat16 would cost the output as much as its own rounding)
+//   6-9    epilogue: TMEM -> bias -> 16-bit rows, one of two accumulators each
+// W's chunks and the adapters' have rings of their own, so each producer runs
+// ahead as far as its ring allows; warps 2-5 announce the number of adapters of
+// a tile, which only the MMA issuer needs.
+#include <cuda.h>
+#include <cudaTypedefs.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <climits>
+#include <mutex>
+#include <type_traits>
 
 #include "common.cuh"
 
 namespace nnb {
 namespace {
-
 __device__ int g_device_status = 0;
 __device__ int g_device_status_where = 0;
+}  // namespace
+}  // namespace nnb
 
-constexpr int kBadIndex = 41;  // wait-site number of an adapter index out of range
+#include "tc_common.cuh"
+
+namespace nnb {
+namespace {
+
+using namespace tc;
+
+constexpr int kBadIndex = 41;  // site number of an adapter index out of range; 42-52 are waits
+
+constexpr int kThreads = 320;
+constexpr int kStageA = BM * 128;
+constexpr int kRankBlock = 32;  // ranks of an adapter stage: a 128-byte row of 32 hi and 32 lo parts
+
+template <int BN>
+struct Tile {
+  // Stages as shared memory allows beside the staging rows; the narrowest tile leaves room for a second CTA.
+  static constexpr int kStages = BN == 256 ? 3 : BN == 128 ? 4 : BN == 64 ? 6 : 3;
+  static constexpr int kLowStages = BN == 256 ? 1 : 2;
+  static constexpr int kCtas = BN == 32 ? 2 : 1;
+  static constexpr int kStageB = BN * 128;
+  static constexpr int kStage = kStageA + kStageB;
+  static constexpr int kColumns = BN < 64 ? BN : 64;  // columns an epilogue warp stages at a time
+  static constexpr int kStaging = 32 * kColumns * 2;
+  static constexpr int kTmem = 2 * BN;
+  static constexpr int kSmem = 1024 + (kStages + kLowStages) * kStage + 4 * (kStaging + BN * 4) + 1024;
+};
+
+constexpr int kCounts = 4;  // tiles whose number of adapters may be announced ahead
+
+// Position in a ring of stages: a consumer waits for the full barrier's `phase`, a producer for the empty
+// barrier's opposite one (which a fresh barrier has passed).  Every position is waited for in turn: a parity
+// says nothing about a barrier more than one phase away.
+template <int STAGES>
+struct Ring {
+  int s = 0;
+  uint32_t phase = 0;
+  __device__ __forceinline__ void next() {
+    if (++s == STAGES) s = 0, phase ^= 1u;
+  }
+};
+
+struct Maps {
+  CUtensorMap x, weight, up;
+};
 
 __device__ __forceinline__ float value(__nv_bfloat16 v) { return __bfloat162float(v); }
 __device__ __forceinline__ float value(__half v) { return __half2float(v); }
+
+__device__ __forceinline__ uint32_t pack2(float a, float b, __nv_bfloat16) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ uint32_t pack2(float a, float b, __half) {
+  const __half2 v = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
 
 // The adapter of a row, -1 for none.  An index out of range counts as none and is recorded.
 __device__ __forceinline__ int row_adapter(const nnb_project_args& a, int64_t row) {
@@ -34,7 +111,29 @@ __device__ __forceinline__ int row_adapter(const nnb_project_args& a, int64_t ro
   return v;
 }
 
+// ---------------------------------------------------------------------------
+// Rows that TMA cannot read (a start or a stride off 16 bytes), copied once.
+// ---------------------------------------------------------------------------
+__global__ void __launch_bounds__(256) align_rows_kernel(const uint16_t* x, int64_t stride, int64_t rows, int k,
+                                                         uint16_t* out, int out_stride) {
+  const int64_t values = rows * out_stride;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < values; i += (int64_t)gridDim.x * 256) {
+    const int64_t row = i / out_stride;
+    const int c = (int)(i - row * out_stride);
+    out[i] = c < k ? x[row * stride + c] : (uint16_t)0;
+  }
+}
+
+// ---------------------------------------------------------------------------
 // low[t][j] = scale_a sum_k down_a[j][k] x[t][k]: a warp takes four ranks of one row.
+// ---------------------------------------------------------------------------
+template <typename T>
+__device__ __forceinline__ void widen(float (&v)[8], const uint4& raw) {
+  const T* t = reinterpret_cast<const T*>(&raw);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = value(t[i]);
+}
+
 template <typename T>
 __global__ void __launch_bounds__(128) project_low_kernel(const nnb_project_args a) {
   const int64_t row = blockIdx.x;
@@ -44,10 +143,21 @@ __global__ void __launch_bounds__(128) project_low_kernel(const nnb_project_args
   const T* x = reinterpret_cast<const T*>(a.x) + row * a.x_stride;
   const T* down = reinterpret_cast<const T*>(a.down) + ((int64_t)adapter * a.rank + j0) * a.weight_stride;
   float sum[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int k = lane; k < a.k; k += 32) {
-    const float v = value(x[k]);
+  const int whole = a.k & ~7;
+  for (int k = lane * 8; k < whole; k += 256) {
+    float v[8], d[8];
+    widen<T>(v, *reinterpret_cast<const uint4*>(x + k));
 #pragma unroll
-    for (int j = 0; j < 4; ++j) sum[j] = fmaf(v, value(down[j * a.weight_stride + k]), sum[j]);
+    for (int j = 0; j < 4; ++j) {
+      widen<T>(d, __ldg(reinterpret_cast<const uint4*>(down + j * a.weight_stride + k)));
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sum[j] = fmaf(v[i], d[i], sum[j]);
+    }
+  }
+  if (whole + lane < a.k) {
+    const float v = value(x[whole + lane]);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) sum[j] = fmaf(v, value(down[j * a.weight_stride + whole + lane]), sum[j]);
   }
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
@@ -57,62 +167,486 @@ __global__ void __launch_bounds__(128) project_low_kernel(const nnb_project_args
   }
 }
 
-// 64 x 64 outputs per block, 4 x 4 per thread, 16 channels at a time.
-template <typename T>
-__global__ void __launch_bounds__(256) project_kernel(const nnb_project_args a) {
-  __shared__ float xs[16][65], ws[16][65];
-  const int64_t row0 = (int64_t)blockIdx.x * 64;
-  const int col0 = blockIdx.y * 64;
-  const int ty = threadIdx.x / 16, tx = threadIdx.x % 16;
-  float acc[4][4] = {};
-  for (int k0 = 0; k0 < a.k; k0 += 16) {
-    for (int i = threadIdx.x; i < 64 * 16; i += 256) {
-      const int r = i / 16, k = i % 16;
-      const bool in = k0 + k < a.k;
-      xs[k][r] = in && row0 + r < a.rows
-                     ? value(reinterpret_cast<const T*>(a.x)[(row0 + r) * a.x_stride + k0 + k]) : 0.f;
-      ws[k][r] = in && col0 + r < a.n
-                     ? value(reinterpret_cast<const T*>(a.weight)[(col0 + r) * a.weight_stride + k0 + k]) : 0.f;
+// ---------------------------------------------------------------------------
+// The GEMM.
+// ---------------------------------------------------------------------------
+__device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, int c0, int c1, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
+          dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(bar)
+      : "memory");
+}
+
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2,
+                                            uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], "
+      "[%5];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(bar)
+      : "memory");
+}
+
+__device__ __forceinline__ void mbar_expect_tx(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+
+__device__ __forceinline__ void mma_f16(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                        uint32_t accumulate) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// Barrier of the four adapter warps; true when every one of their threads passed `ok`.
+__device__ __forceinline__ bool adapter_barrier(bool ok) {
+  uint32_t all;
+  asm volatile(
+      "{\n .reg .pred p, q;\n setp.ne.u32 p, %1, 0;\n barrier.cta.red.and.pred q, 1, 128, p;\n"
+      " selp.u32 %0, 1, 0, q;\n}\n"
+      : "=r"(all)
+      : "r"((uint32_t)ok)
+      : "memory");
+  return all != 0;
+}
+
+struct TileAt {
+  int64_t row0;
+  int col0;
+};
+
+// Tiles in groups of 16 row tiles, rows first: the tiles in flight at a time share few rows and few columns.
+__device__ __forceinline__ TileAt tile_at(int64_t tile, int64_t row_tiles, int col_tiles, int bn) {
+  const int64_t group = tile / (16 * (int64_t)col_tiles);
+  const int64_t rest = tile - group * 16 * col_tiles;
+  const int64_t rows = min((int64_t)16, row_tiles - group * 16);
+  return {(group * 16 + rest % rows) * BM, (int)(rest / rows) * bn};
+}
+
+template <typename T, int BN>
+__global__ void __launch_bounds__(kThreads, Tile<BN>::kCtas)
+    project_kernel(const nnb_project_args a, const __grid_constant__ Maps maps) {
+  using C = Tile<BN>;
+  constexpr int S = C::kStages, SL = C::kLowStages;
+  constexpr bool kF16 = !std::is_same<T, __nv_bfloat16>::value;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* stages = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* low_stages = stages + S * C::kStage;
+  uint8_t* staging = low_stages + SL * C::kStage;
+  float* bias_rows = reinterpret_cast<float*>(staging + 4 * C::kStaging);
+  uint64_t* full = reinterpret_cast<uint64_t*>(bias_rows + 4 * BN);
+  uint64_t* empty = full + S;
+  uint64_t* low_full = empty + S;
+  uint64_t* low_empty = low_full + SL;
+  uint64_t* acc_full = low_empty + SL;
+  uint64_t* acc_empty = acc_full + 2;
+  uint64_t* count_full = acc_empty + 2;
+  uint64_t* count_empty = count_full + kCounts;
+  uint64_t* drain = count_empty + kCounts;
+  volatile int* counts = reinterpret_cast<volatile int*>(drain + 1);  // adapters of the tiles announced
+  volatile int* smallest = counts + kCounts;                          // 2 x 4 warps
+  volatile int* listed = smallest + 8;                                // the tile's adapters, ascending
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(const_cast<int*>(listed + BM));
+  int* abort_flag = reinterpret_cast<int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t row_tiles = (a.rows + BM - 1) / BM;
+  const int col_tiles = (a.n + BN - 1) / BN;
+  const int64_t tiles = row_tiles * col_tiles;
+  const int my_tiles = (int)((tiles - blockIdx.x + gridDim.x - 1) / gridDim.x);
+  const int chunks = (a.k + 63) / 64;
+  const int blocks = (a.rank + kRankBlock - 1) / kRankBlock;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < S; ++s) {
+      mbar_init(smem_u32(&full[s]), 1);
+      mbar_init(smem_u32(&empty[s]), 1);
     }
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < 16; ++k)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(xs[k][ty * 4 + i], ws[k][tx * 4 + j], acc[i][j]);
-    __syncthreads();
+    for (int s = 0; s < SL; ++s) {
+      mbar_init(smem_u32(&low_full[s]), 1);
+      mbar_init(smem_u32(&low_empty[s]), 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(smem_u32(&acc_full[i]), 1);
+      mbar_init(smem_u32(&acc_empty[i]), 4);  // the epilogue's warps
+    }
+    for (int i = 0; i < kCounts; ++i) {
+      mbar_init(smem_u32(&count_full[i]), 1);
+      mbar_init(smem_u32(&count_empty[i]), 1);
+    }
+    mbar_init(smem_u32(drain), 1);
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  const int planes = sizeof(T) == 2 && a.type == NNB_F16 ? 2 : 1;
-  for (int i = 0; i < 4; ++i) {
-    const int64_t row = row0 + ty * 4 + i;
-    if (row >= a.rows) continue;
-    const int adapter = row_adapter(a, row);
-    for (int j = 0; j < 4; ++j) {
-      const int col = col0 + tx * 4 + j;
-      if (col >= a.n) continue;
-      float v = acc[i][j] + (a.bias ? __ldg(a.bias + col) : 0.f);
-      if (adapter >= 0) {
-        const __nv_bfloat16* up = reinterpret_cast<const __nv_bfloat16*>(a.up) +
-                                  ((int64_t)adapter * a.n + col) * planes * a.rank;
-        for (int r = 0; r < a.rank; ++r) {
-          float u = value(up[r]);
-          if (planes == 2) u += value(up[a.rank + r]);
-          v = fmaf(a.low[row * a.rank + r], u, v);
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                 "r"(C::kTmem)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  fence_before();
+  __syncthreads();
+  fence_after();
+  const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(tmem_slot);
+
+  if (warp == 0) {
+    // ------------------------------ TMA producer -----------------------------
+    if (lane == 0) {
+      Ring<S> ring;
+      int issued = 0;
+      bool alive = true;
+      for (int it = 0; it < my_tiles && alive; ++it) {
+        const TileAt t = tile_at(blockIdx.x + (int64_t)it * gridDim.x, row_tiles, col_tiles, BN);
+        for (int c = 0; c < chunks; ++c) {
+          if (!mbar_wait(smem_u32(&empty[ring.s]), ring.phase ^ 1, abort_flag, 42)) {
+            alive = false;
+            break;
+          }
+          const uint32_t bar = smem_u32(&full[ring.s]), at = smem_u32(stages + ring.s * C::kStage);
+          mbar_arrive_expect_tx(bar, C::kStage);
+          tma_load_2d(at, &maps.x, c * 64, (int)t.row0, bar);
+          tma_load_2d(at + kStageA, &maps.weight, c * 64, t.col0, bar);
+          ring.next();
+          ++issued;
         }
       }
-      reinterpret_cast<T*>(a.out)[row * a.out_stride + col] = T(v);
+      if (*reinterpret_cast<volatile int*>(abort_flag))  // wait (bounded) for the copies still in flight
+        for (int g = max(0, issued - S); g < issued; ++g)
+          mbar_wait(smem_u32(&full[g % S]), (uint32_t)(g / S) & 1, abort_flag, 43, false);
     }
+    __syncwarp();
+  } else if (warp == 1) {
+    // ------------------------------ MMA issuer -------------------------------
+    if (lane == 0) {
+      const uint32_t main_idesc = kF16 ? idesc_f16(BM, BN) : idesc_bf16(BM, BN);
+      const uint32_t low_idesc = idesc_bf16(BM, BN);
+      Ring<S> ring;
+      Ring<SL> low_ring;
+      Ring<kCounts> counted;
+      bool alive = true;
+      for (int it = 0; it < my_tiles && alive; ++it) {
+        const int acc = it & 1;
+        if (!mbar_wait(smem_u32(&acc_empty[acc]), (uint32_t)((it >> 1) & 1) ^ 1, abort_flag, 44)) break;
+        fence_after();
+        const uint32_t d = tmem + acc * BN;
+        uint32_t accumulate = 0;
+        for (int c = 0; c < chunks; ++c) {
+          if (!mbar_wait(smem_u32(&full[ring.s]), ring.phase, abort_flag, 45)) {
+            alive = false;
+            break;
+          }
+          fence_after();
+          const uint32_t at = smem_u32(stages + ring.s * C::kStage);
+          const uint64_t ad = sw128_desc(at), bd = sw128_desc(at + kStageA);
+          const int steps = min(4, (a.k - c * 64 + 15) / 16);
+          for (int k = 0; k < steps; ++k) {  // 16 channels: 32 bytes of every row
+            mma_f16(d, ad + k * 2, bd + k * 2, main_idesc, accumulate);
+            accumulate = 1;
+          }
+          mma_commit(smem_u32(&empty[ring.s]));
+          ring.next();
+        }
+        if (!alive || !mbar_wait(smem_u32(&count_full[counted.s]), counted.phase, abort_flag, 46)) break;
+        const int low_stages_due = counts[counted.s] * blocks;
+        mbar_arrive(smem_u32(&count_empty[counted.s]));
+        counted.next();
+        for (int i = 0; i < low_stages_due; ++i) {
+          if (!mbar_wait(smem_u32(&low_full[low_ring.s]), low_ring.phase, abort_flag, 47)) {
+            alive = false;
+            break;
+          }
+          fence_after();
+          const uint32_t at = smem_u32(low_stages + low_ring.s * C::kStage);
+          const uint64_t hi = sw128_desc(at), lo = hi + 4, up = sw64_desc(at + kStageA);
+          const int steps = min(2, (a.rank - (i % blocks) * kRankBlock) / 16);
+          for (int k = 0; k < steps; ++k) {
+            mma_f16(d, hi + k * 2, up + k * 2, low_idesc, 1);
+            mma_f16(d, lo + k * 2, up + k * 2, low_idesc, 1);
+            if constexpr (kF16) mma_f16(d, hi + k * 2, up + (BN * 64 >> 4) + k * 2, low_idesc, 1);
+          }
+          mma_commit(smem_u32(&low_empty[low_ring.s]));
+          low_ring.next();
+        }
+        if (alive) mma_commit(smem_u32(&acc_full[acc]));
+      }
+      if (*reinterpret_cast<volatile int*>(abort_flag)) {  // wait (bounded) for every MMA issued
+        mma_commit(smem_u32(drain));
+        mbar_wait(smem_u32(drain), 0, abort_flag, 48, false);
+      }
+    }
+    __syncwarp();
+  } else if (warp < 6) {
+    // ---------------------------- adapter producers --------------------------
+    const int r = threadIdx.x - 64;
+    const bool leader = r == 0;
+    Ring<SL> ring;
+    Ring<kCounts> counted;
+    int issued = 0;
+    int turn = 0;
+    bool alive = true;  // this thread; `all`: the four warps, which go on together or stop together
+    bool all = true;
+    for (int it = 0; it < my_tiles && all; ++it) {
+      const TileAt t = tile_at(blockIdx.x + (int64_t)it * gridDim.x, row_tiles, col_tiles, BN);
+      const int64_t row = t.row0 + r;
+      const int mine = row < a.rows ? row_adapter(a, row) : -1;
+      // the tile's adapters in ascending order, one per turn (a second buffer of minima needs one barrier a turn)
+      int count = 0;
+      for (int low = -1;;) {
+        const int least = __reduce_min_sync(0xffffffffu, mine > low ? mine : INT_MAX);
+        if (lane == 0) smallest[turn * 4 + warp - 2] = least;
+        adapter_barrier(true);
+        low = min(min(smallest[turn * 4], smallest[turn * 4 + 1]),
+                  min(smallest[turn * 4 + 2], smallest[turn * 4 + 3]));
+        turn ^= 1;
+        if (low == INT_MAX) break;
+        if (leader) listed[count] = low;
+        ++count;
+      }
+      if (leader) {
+        alive = mbar_wait(smem_u32(&count_empty[counted.s]), counted.phase ^ 1, abort_flag, 49);
+        counts[counted.s] = count;
+        mbar_arrive(smem_u32(&count_full[counted.s]));
+      }
+      counted.next();
+      all = adapter_barrier(alive);  // also makes the list visible
+      for (int i = 0; i < count * blocks && all; ++i) {
+        const int adapter = listed[i / blocks], j0 = (i % blocks) * kRankBlock;
+        float v[kRankBlock];
+        const bool own = mine == adapter;
+#pragma unroll
+        for (int j = 0; j < kRankBlock; j += 4) {
+          float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (own && j0 + j < a.rank) f = *reinterpret_cast<const float4*>(a.low + row * a.rank + j0 + j);
+          v[j] = f.x, v[j + 1] = f.y, v[j + 2] = f.z, v[j + 3] = f.w;
+        }
+        alive = alive && mbar_wait(smem_u32(&low_empty[ring.s]), ring.phase ^ 1, abort_flag, 50);
+        uint8_t* at = low_stages + ring.s * C::kStage;
+        const uint32_t bar = smem_u32(&low_full[ring.s]);
+        if (leader && alive) {
+          const uint32_t dst = smem_u32(at) + kStageA;
+          mbar_expect_tx(bar, BN * 64 * (kF16 ? 2 : 1));
+          tma_load_3d(dst, &maps.up, j0, t.col0, adapter, bar);
+          if constexpr (kF16) tma_load_3d(dst + BN * 64, &maps.up, a.rank + j0, t.col0, adapter, bar);
+          ++issued;
+        }
+        if (alive) {
+          uint32_t hi[kRankBlock / 2], lo[kRankBlock / 2];
+#pragma unroll
+          for (int j = 0; j < kRankBlock / 2; ++j) {
+            const float h0 = __bfloat162float(__float2bfloat16_rn(v[2 * j]));
+            const float h1 = __bfloat162float(__float2bfloat16_rn(v[2 * j + 1]));
+            hi[j] = pack2(h0, h1, __nv_bfloat16());
+            // what an infinity leaves would be no number
+            lo[j] = pack2(isfinite(h0) ? v[2 * j] - h0 : 0.f, isfinite(h1) ? v[2 * j + 1] - h1 : 0.f,
+                          __nv_bfloat16());
+          }
+          uint4* line = reinterpret_cast<uint4*>(at + r * 128);
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            line[c ^ (r & 7)] = make_uint4(hi[4 * c], hi[4 * c + 1], hi[4 * c + 2], hi[4 * c + 3]);
+            line[(c + 4) ^ (r & 7)] = make_uint4(lo[4 * c], lo[4 * c + 1], lo[4 * c + 2], lo[4 * c + 3]);
+          }
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        }
+        all = adapter_barrier(alive);
+        if (leader && alive) mbar_arrive(bar);  // also on the way out, so that the copy's phase completes
+        ring.next();
+      }
+    }
+    if (leader && *reinterpret_cast<volatile int*>(abort_flag))
+      for (int g = max(0, issued - SL); g < issued; ++g)
+        mbar_wait(smem_u32(&low_full[g % SL]), (uint32_t)(g / SL) & 1, abort_flag, 51, false);
+    __syncwarp();
+  } else {
+    // -------------------------------- epilogue -------------------------------
+    const int quarter = warp & 3;  // the TMEM lanes a warp may read
+    uint8_t* stage_rows = staging + (warp - 6) * C::kStaging;
+    float* bias = bias_rows + (warp - 6) * BN;
+    const bool vector = (reinterpret_cast<uintptr_t>(a.out) % 16 == 0) && (a.rows == 1 || a.out_stride % 8 == 0);
+    for (int it = 0; it < my_tiles; ++it) {
+      const TileAt t = tile_at(blockIdx.x + (int64_t)it * gridDim.x, row_tiles, col_tiles, BN);
+      const int acc = it & 1;
+      __syncwarp();
+      for (int c = lane; c < BN; c += 32) bias[c] = a.bias != nullptr && t.col0 + c < a.n ? a.bias[t.col0 + c] : 0.f;
+      __syncwarp();
+      const bool ok = mbar_wait(smem_u32(&acc_full[acc]), (uint32_t)(it >> 1) & 1, abort_flag, 52);
+      if (!__all_sync(0xffffffffu, ok)) break;
+      fence_after();
+      const uint32_t src = tmem + acc * BN + ((uint32_t)quarter << 21);
+      const int64_t row0 = t.row0 + quarter * 32;
+#pragma unroll 1
+      for (int c0 = 0; c0 < BN; c0 += C::kColumns) {
+        if (t.col0 + c0 >= a.n) break;
+        constexpr int kChunks = C::kColumns / 8;  // 16-byte chunks of a staged row
+#pragma unroll
+        for (int h = 0; h < C::kColumns; h += 32) {
+          float v[32];
+          tmem_ld32(src + c0 + h, v);
+          uint4* line = reinterpret_cast<uint4*>(stage_rows + lane * C::kColumns * 2);
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            uint32_t p[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const float2 b = *reinterpret_cast<const float2*>(bias + c0 + h + c * 8 + j * 2);
+              p[j] = pack2(v[c * 8 + j * 2] + b.x, v[c * 8 + j * 2 + 1] + b.y, T());
+            }
+            // chunks permuted by row so that neither side meets in a bank
+            const int swap = kChunks == 8 ? lane & 7 : (lane >> 1) & 3;
+            line[(h / 8 + c) ^ swap] = make_uint4(p[0], p[1], p[2], p[3]);
+          }
+        }
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < kChunks; ++i) {
+          const int r = (i * 32 + lane) / kChunks, c = (i * 32 + lane) % kChunks;
+          const int swap = kChunks == 8 ? r & 7 : (r >> 1) & 3;
+          const uint4 packed = reinterpret_cast<const uint4*>(stage_rows + r * C::kColumns * 2)[c ^ swap];
+          const int col = t.col0 + c0 + c * 8;
+          if (row0 + r < a.rows && col < a.n) {
+            T* out = reinterpret_cast<T*>(a.out) + (row0 + r) * a.out_stride + col;
+            if (vector && col + 8 <= a.n) {
+              *reinterpret_cast<uint4*>(out) = packed;
+            } else {
+              const T* values = reinterpret_cast<const T*>(&packed);
+#pragma unroll
+              for (int j = 0; j < 8; ++j)
+                if (col + j < a.n) out[j] = values[j];
+            }
+          }
+        }
+        __syncwarp();
+      }
+      fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&acc_empty[acc]));
+    }
+  }
+  __syncthreads();
+  if (warp == 1) {
+    fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(C::kTmem) : "memory");
   }
 }
 
-template <typename T>
-int launch_project(const nnb_project_args& a, cudaStream_t stream) {
-  project_low_kernel<T><<<dim3((unsigned)a.rows, a.rank / 16), 128, 0, stream>>>(a);
-  NNB_LAUNCH_CHECK();
-  project_kernel<T><<<dim3((unsigned)((a.rows + 63) / 64), (a.n + 63) / 64), 256, 0, stream>>>(a);
+// ---------------------------------------------------------------------------
+// Host side.
+// ---------------------------------------------------------------------------
+using EncodeTiledFn = PFN_cuTensorMapEncodeTiled_v12000;
+
+EncodeTiledFn encode_tiled() {
+  static EncodeTiledFn fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q = cudaDriverEntryPointSymbolNotFound;
+    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<EncodeTiledFn>(p);
+  });
+  return fn;
+}
+
+// A map of `rank` axes (innermost first, strides of the outer ones in bytes) over 16-bit values.
+int encode(CUtensorMap* map, bool f16, int axes, const void* base, const cuuint64_t* dims, const cuuint64_t* strides,
+           const cuuint32_t* box, CUtensorMapSwizzle swizzle) {
+  const EncodeTiledFn fn = encode_tiled();
+  NNB_REQUIRE(fn != nullptr, "project: cuTensorMapEncodeTiled is not available from the driver");
+  const cuuint32_t ones[3] = {1, 1, 1};
+  const CUresult r = fn(map, f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, axes,
+                        const_cast<void*>(base), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  NNB_REQUIRE(r == CUDA_SUCCESS, "project: cuTensorMapEncodeTiled failed (%d)", (int)r);
+  return NNB_OK;
+}
+
+// Whether TMA can read the rows where they are.
+bool rows_in_place(const nnb_project_args& a) {
+  return reinterpret_cast<uintptr_t>(a.x) % 16 == 0 &&
+         (a.rows == 1 || (a.x_stride % 8 == 0 && a.x_stride >= a.k));
+}
+
+int64_t low_bytes(const nnb_project_args& a) { return a.rows * a.rank * (int64_t)sizeof(float); }
+
+template <typename T, int BN>
+int launch_tiles(const nnb_project_args& a, int sms, int dev, cudaStream_t stream) {
+  using C = Tile<BN>;
+  constexpr bool kF16 = !std::is_same<T, __nv_bfloat16>::value;
+  static bool configured[64] = {false};
+  if (dev >= 64 || !configured[dev]) {
+    NNB_CUDA_CHECK(
+        cudaFuncSetAttribute(project_kernel<T, BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
+    if (dev < 64) configured[dev] = true;
+  }
+  static_assert(C::kSmem * C::kCtas <= kMaxSmem + 1024 * (C::kCtas - 1), "the tile's stages exceed shared memory");
+  Maps maps;
+  {
+    const cuuint64_t dims[2] = {(cuuint64_t)a.k, (cuuint64_t)a.rows};
+    const cuuint64_t strides[1] = {(cuuint64_t)(a.rows == 1 ? (a.k + 7) / 8 * 8 : a.x_stride) * 2};
+    const cuuint32_t box[2] = {64, BM};
+    if (const int rc = encode(&maps.x, kF16, 2, a.x, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B)) return rc;
+  }
+  {
+    const cuuint64_t dims[2] = {(cuuint64_t)a.k, (cuuint64_t)a.n};
+    const cuuint64_t strides[1] = {(cuuint64_t)a.weight_stride * 2};
+    const cuuint32_t box[2] = {64, BN};
+    if (const int rc = encode(&maps.weight, kF16, 2, a.weight, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B))
+      return rc;
+  }
+  {
+    const cuuint64_t width = (cuuint64_t)a.rank * (kF16 ? 2 : 1);
+    const cuuint64_t dims[3] = {width, (cuuint64_t)a.n, (cuuint64_t)a.adapters};
+    const cuuint64_t strides[2] = {width * 2, width * 2 * (cuuint64_t)a.n};
+    const cuuint32_t box[3] = {kRankBlock, BN, 1};
+    if (const int rc = encode(&maps.up, false, 3, a.up, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_64B)) return rc;
+  }
+  const int64_t tiles = (a.rows + BM - 1) / BM * ((a.n + BN - 1) / BN);
+  const int grid = (int)std::min<int64_t>(tiles, (int64_t)sms * C::kCtas);
+  project_kernel<T, BN><<<grid, kThreads, C::kSmem, stream>>>(a, maps);
   NNB_LAUNCH_CHECK();
   return NNB_OK;
+}
+
+// Tile width: the one whose waves of tiles take least, a tile's time being the larger of its MMAs' and its
+// loads' (cycles per 64 channels), plus a fixed start and epilogue.
+int tile_columns(const nnb_project_args& a, int sms) {
+  const int widths[4] = {32, 64, 128, 256};
+  const int chunk_cycles[4] = {320, 384, 512, 768};
+  int best = 32;
+  int64_t least = INT64_MAX;
+  for (int i = 0; i < 4; ++i) {
+    const int64_t tiles = (a.rows + BM - 1) / BM * ((a.n + widths[i] - 1) / widths[i]);
+    const int64_t waves = (tiles + sms - 1) / sms;
+    const int64_t cost = waves * (chunk_cycles[i] * (int64_t)((a.k + 63) / 64) + 2 * widths[i]) + 2000;
+    if (cost < least) least = cost, best = widths[i];
+  }
+  return best;
+}
+
+template <typename T>
+int launch_project(nnb_project_args a, cudaStream_t stream) {
+  int dev = 0, sms = 0;
+  NNB_CUDA_CHECK(cudaGetDevice(&dev));
+  NNB_CUDA_CHECK(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
+  if (!rows_in_place(a)) {
+    uint16_t* rows = reinterpret_cast<uint16_t*>(reinterpret_cast<uint8_t*>(a.low) + low_bytes(a));
+    const int64_t blocks = (a.rows * a.weight_stride + 255) / 256;
+    align_rows_kernel<<<(unsigned)std::min<int64_t>(blocks, sms * 8), 256, 0, stream>>>(
+        reinterpret_cast<const uint16_t*>(a.x), a.x_stride, a.rows, a.k, rows, (int)a.weight_stride);
+    NNB_LAUNCH_CHECK();
+    a.x = rows;
+    a.x_stride = a.weight_stride;
+  }
+  project_low_kernel<T><<<dim3((unsigned)a.rows, a.rank / 16), 128, 0, stream>>>(a);
+  NNB_LAUNCH_CHECK();
+  switch (tile_columns(a, sms)) {
+    case 32: return launch_tiles<T, 32>(a, sms, dev, stream);
+    case 64: return launch_tiles<T, 64>(a, sms, dev, stream);
+    case 128: return launch_tiles<T, 128>(a, sms, dev, stream);
+    default: return launch_tiles<T, 256>(a, sms, dev, stream);
+  }
 }
 
 }  // namespace
@@ -135,8 +669,9 @@ int project_device_status(int32_t* where, bool reset) {
 using namespace nnb;
 
 extern "C" int64_t nnb_project_workspace_bytes(const nnb_project_args* args) {
-  NNB_REQUIRE(args != nullptr && args->rows >= 1 && args->rank >= 16, "project_workspace_bytes: bad shape");
-  return args->rows * args->rank * (int64_t)sizeof(float);
+  NNB_REQUIRE(args != nullptr && args->rows >= 1 && args->rank >= 16 && args->weight_stride >= 1,
+              "project_workspace_bytes: bad shape");
+  return low_bytes(*args) + (rows_in_place(*args) ? 0 : args->rows * args->weight_stride * 2);
 }
 
 extern "C" int32_t nnb_project(const nnb_project_args* args, void* stream) {

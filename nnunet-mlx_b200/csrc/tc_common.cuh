@@ -1,7 +1,8 @@
 // Shared sm_100a helpers of the tensor-core kernels: mbarriers with bounded
 // waits, bulk copies, TMEM loads/stores, UMMA descriptors and MMA issue.
-// Included by tc_conv.cu (one translation unit for all tensor-core kernels),
-// which defines nnb::g_device_status / g_device_status_where first.
+// Included by the translation units with tensor-core kernels (tc_conv.cu,
+// project.cu), each of which defines its g_device_status / g_device_status_where
+// in namespace nnb first; nnb_device_status reads them all.
 #pragma once
 
 #include <cuda_runtime.h>
@@ -54,7 +55,7 @@ __device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity) {
 }
 
 // Bounded wait, slow path: returns false if the CTA is aborting or the time limit expired.
-__device__ __noinline__ bool mbar_wait_slow(uint32_t bar, uint32_t parity, volatile int* abort_flag, int where,
+static __device__ __noinline__ bool mbar_wait_slow(uint32_t bar, uint32_t parity, volatile int* abort_flag, int where,
                                             bool honor_abort) {
   const uint64_t start = global_ns();
   for (;;) {

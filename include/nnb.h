@@ -722,7 +722,7 @@ typedef struct nnb_project_args {
   const float* bias;    /* (n) or NULL */
   const int32_t* index; /* an adapter, or -1, for each rows_per_index rows */
   void* out;            /* rows out_stride elements apart, x's type */
-  float* low;           /* workspace of nnb_project_workspace_bytes(args) bytes, 16-byte aligned */
+  float* low;           /* workspace of nnb_project_workspace_bytes(args) bytes, 16-byte aligned; NULL if none */
   int64_t rows;         /* below 2^31 */
   int64_t x_stride;
   int64_t out_stride;

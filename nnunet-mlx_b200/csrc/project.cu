@@ -103,7 +103,7 @@ __device__ __forceinline__ uint32_t pack2(float a, float b, __half) {
 
 // The adapter of a row, -1 for none.  An index out of range counts as none and is recorded.
 __device__ __forceinline__ int row_adapter(const nnb_project_args& a, int64_t row) {
-  const int v = __ldg(a.index + (a.rows_per_index == 1 ? row : row / a.rows_per_index));
+  const int v = __ldg(a.index + (a.rows_per_index == 1 ? row : (uint32_t)row / (uint32_t)a.rows_per_index));
   if (v >= a.adapters || v < -1) {
     if (atomicCAS(&g_device_status, 0, NNB_E_DEVICE) == 0) g_device_status_where = kBadIndex;
     return -1;
@@ -568,7 +568,9 @@ bool rows_in_place(const nnb_project_args& a) {
          (a.rows == 1 || (a.x_stride % 8 == 0 && a.x_stride >= a.k));
 }
 
-int64_t low_bytes(const nnb_project_args& a) { return a.rows * a.rank * (int64_t)sizeof(float); }
+bool narrow(const nnb_project_args& a) { return a.k <= 128 && a.n <= 128; }
+
+int64_t low_bytes(const nnb_project_args& a) { return narrow(a) ? 0 : a.rows * a.rank * (int64_t)sizeof(float); }
 
 template <typename T, int BN>
 int launch_tiles(const nnb_project_args& a, int sms, int dev, cudaStream_t stream) {
@@ -625,8 +627,222 @@ int tile_columns(const nnb_project_args& a, int sms) {
   return best;
 }
 
+// ---------------------------------------------------------------------------
+// Narrow projections (up to 128 channels on either side), bound by HBM: a warp
+// carries 16 M rows from x to out in registers, low-rank values included.
+//
+// mma.sync fragments, with the axes permuted so that every thread's share is
+// contiguous: of 32 channels thread q of a row's four holds 8q..8q+7 (one
+// 16-byte load feeds two K-steps; W's rows are read in the same order), of 32
+// columns 8q..8q+7 (one 16-byte store), of 16 ranks 4q..4q+3.  The low-rank
+// accumulators are the A fragments of the product with up_a, as two bfloat16
+// parts; rows of other requests are zeroed there, once per adapter among the
+// warp's rows.  The tensor rate is no bound here (some 20 operations per byte),
+// so the plain warp MMAs serve, and no stage or barrier stands between x and out.
+// ---------------------------------------------------------------------------
+__device__ __forceinline__ void warp_mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1,
+                                         __nv_bfloat16) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void warp_mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, __half) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// Eight channels of a row from column k on; zero from column `width` on.
+template <typename T>
+__device__ __forceinline__ uint4 row_chunk(const T* row, int k, int width) {
+  if (k + 8 <= width) return *reinterpret_cast<const uint4*>(row + k);
+  uint4 v = make_uint4(0, 0, 0, 0);
+  uint16_t* e = reinterpret_cast<uint16_t*>(&v);
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    if (k + i < width) e[i] = reinterpret_cast<const uint16_t*>(row)[k + i];
+  return v;
+}
+
+constexpr int kNarrowThreads = 256;
+
+// NK, NN: groups of 32 channels and columns; M: 16-row fragments per warp.
+template <typename T, int NK, int NN, int M>
+__global__ void __launch_bounds__(kNarrowThreads, 2) project_narrow_kernel(const nnb_project_args a) {
+  constexpr bool kF16 = !std::is_same<T, __nv_bfloat16>::value;
+  constexpr int kPitch = 4 * (NK | 1);  // 16-byte chunks of a W row in shared memory: neighbouring rows 64 bytes
+                                        // apart modulo the banks' 128
+  __shared__ uint4 weight[NN * 32 * kPitch];
+  __shared__ float bias[NN * 32];
+  for (int i = threadIdx.x; i < NN * 32 * NK * 4; i += kNarrowThreads) {
+    const int n = i / (NK * 4), c = i % (NK * 4);
+    weight[n * kPitch + c] =
+        n < a.n ? row_chunk(reinterpret_cast<const T*>(a.weight) + n * a.weight_stride, c * 8, (int)a.weight_stride)
+                : make_uint4(0, 0, 0, 0);
+  }
+  for (int i = threadIdx.x; i < NN * 32; i += kNarrowThreads) bias[i] = a.bias != nullptr && i < a.n ? a.bias[i] : 0.f;
+  __syncthreads();
+
+  const int lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
+  const int spread = (g >> 1) * 8 + (g & 1);  // of 32 columns, the one of B fragment row g of tile 0; tile j: + 2 j
+  const bool vector = reinterpret_cast<uintptr_t>(a.out) % 16 == 0 && (a.rows == 1 || a.out_stride % 8 == 0);
+  const int64_t step = (int64_t)gridDim.x * (kNarrowThreads / 32) * 16 * M;
+  for (int64_t row0 = ((int64_t)blockIdx.x * (kNarrowThreads / 32) + (threadIdx.x >> 5)) * 16 * M; row0 < a.rows;
+       row0 += step) {
+    // A fragments of x: of each 32 channels, words 0-1 are the first K-step's and 2-3 the second's
+    uint4 x[M][2][NK];
+    int mine[M][2];
+#pragma unroll
+    for (int m = 0; m < M; ++m)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int64_t row = row0 + m * 16 + h * 8 + g;
+        const bool live = row < a.rows;
+#pragma unroll
+        for (int c = 0; c < NK; ++c)
+          x[m][h][c] = live ? row_chunk(reinterpret_cast<const T*>(a.x) + row * a.x_stride, c * 32 + q * 8, a.k)
+                            : make_uint4(0, 0, 0, 0);
+        mine[m][h] = live ? row_adapter(a, row) : -1;
+      }
+    float acc[M][NN * 4][4] = {};
+#pragma unroll
+    for (int c = 0; c < NK; ++c)
+#pragma unroll
+      for (int t = 0; t < NN * 4; ++t) {
+        const uint4 w = weight[((t >> 2) * 32 + spread + (t & 3) * 2) * kPitch + c * 4 + q];
+#pragma unroll
+        for (int m = 0; m < M; ++m) {
+          const uint4 &u = x[m][0][c], &v = x[m][1][c];
+          const uint32_t first[4] = {u.x, v.x, u.y, v.y}, second[4] = {u.z, v.z, u.w, v.w};
+          warp_mma(acc[m][t], first, w.x, w.y, T());
+          warp_mma(acc[m][t], second, w.z, w.w, T());
+        }
+      }
+    int listed = -1;
+    for (;;) {
+      int least = INT_MAX;
+#pragma unroll
+      for (int m = 0; m < M; ++m)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          if (mine[m][h] > listed) least = min(least, mine[m][h]);
+      listed = __reduce_min_sync(0xffffffffu, least);
+      if (listed == INT_MAX) break;
+      const float scale = __ldg(a.scales + listed);
+      const T* down = reinterpret_cast<const T*>(a.down) + (int64_t)listed * a.rank * a.weight_stride;
+      const __nv_bfloat16* up =
+          reinterpret_cast<const __nv_bfloat16*>(a.up) + (int64_t)listed * a.n * a.rank * (kF16 ? 2 : 1);
+      for (int j0 = 0; j0 < a.rank; j0 += 16) {
+        float low[M][2][4] = {};
+#pragma unroll
+        for (int c = 0; c < NK; ++c)
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            const int k = c * 32 + q * 8;
+            const T* src = down + (j0 + (g >> 1) * 4 + t * 2 + (g & 1)) * a.weight_stride + k;
+            const uint4 w = k < a.weight_stride ? __ldg(reinterpret_cast<const uint4*>(src)) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+            for (int m = 0; m < M; ++m) {
+              const uint4 &u = x[m][0][c], &v = x[m][1][c];
+              const uint32_t first[4] = {u.x, v.x, u.y, v.y}, second[4] = {u.z, v.z, u.w, v.w};
+              warp_mma(low[m][t], first, w.x, w.y, T());
+              warp_mma(low[m][t], second, w.z, w.w, T());
+            }
+          }
+        uint32_t hi[M][4], lo[M][4];
+#pragma unroll
+        for (int m = 0; m < M; ++m)
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const bool own = mine[m][h] == listed;
+              const float v0 = own ? low[m][t][h * 2] * scale : 0.f, v1 = own ? low[m][t][h * 2 + 1] * scale : 0.f;
+              const float h0 = __bfloat162float(__float2bfloat16_rn(v0));
+              const float h1 = __bfloat162float(__float2bfloat16_rn(v1));
+              hi[m][t * 2 + h] = pack2(h0, h1, __nv_bfloat16());
+              lo[m][t * 2 + h] = pack2(isfinite(h0) ? v0 - h0 : 0.f, isfinite(h1) ? v1 - h1 : 0.f, __nv_bfloat16());
+            }
+#pragma unroll
+        for (int t = 0; t < NN * 4; ++t) {
+          const int col = min((t >> 2) * 32 + spread + (t & 3) * 2, a.n - 1);  // columns past n are not stored
+          const __nv_bfloat16* src = up + (int64_t)col * a.rank * (kF16 ? 2 : 1) + j0 + q * 4;
+          const uint2 w = __ldg(reinterpret_cast<const uint2*>(src));
+#pragma unroll
+          for (int m = 0; m < M; ++m) {
+            warp_mma(acc[m][t], hi[m], w.x, w.y, __nv_bfloat16());
+            warp_mma(acc[m][t], lo[m], w.x, w.y, __nv_bfloat16());
+          }
+          if constexpr (kF16) {
+            const uint2 rest = __ldg(reinterpret_cast<const uint2*>(src + a.rank));
+#pragma unroll
+            for (int m = 0; m < M; ++m) warp_mma(acc[m][t], hi[m], rest.x, rest.y, __nv_bfloat16());
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int m = 0; m < M; ++m)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int64_t row = row0 + m * 16 + h * 8 + g;
+        if (row >= a.rows) continue;
+#pragma unroll
+        for (int p = 0; p < NN; ++p) {
+          const int col = p * 32 + q * 8;
+          uint4 packed;
+          uint32_t* words = reinterpret_cast<uint32_t*>(&packed);
+#pragma unroll
+          for (int t = 0; t < 4; ++t)
+            words[t] = pack2(acc[m][p * 4 + t][h * 2] + bias[col + t * 2],
+                             acc[m][p * 4 + t][h * 2 + 1] + bias[col + t * 2 + 1], T());
+          T* out = reinterpret_cast<T*>(a.out) + row * a.out_stride + col;
+          if (vector && col + 8 <= a.n) {
+            *reinterpret_cast<uint4*>(out) = packed;
+          } else {
+            const T* values = reinterpret_cast<const T*>(&packed);
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              if (col + j < a.n) out[j] = values[j];
+          }
+        }
+      }
+  }
+}
+
+template <typename T, int NK, int NN>
+int launch_narrow(const nnb_project_args& a, int sms, int dev, cudaStream_t stream) {
+  constexpr int M = NK <= 2 && NN <= 2 ? 2 : 1;  // a second fragment shares W's reads, as registers allow
+  static int resident[64] = {0};
+  int blocks = dev < 64 ? resident[dev] : 0;
+  if (blocks == 0) {
+    NNB_CUDA_CHECK(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&blocks, project_narrow_kernel<T, NK, NN, M>,
+                                                                 kNarrowThreads, 0));
+    blocks = std::max(1, blocks);
+    if (dev < 64) resident[dev] = blocks;
+  }
+  const int64_t groups = (a.rows + kNarrowThreads / 2 * M - 1) / (kNarrowThreads / 2 * M);
+  project_narrow_kernel<T, NK, NN, M>
+      <<<(unsigned)std::min<int64_t>(groups, (int64_t)blocks * sms), kNarrowThreads, 0, stream>>>(a);
+  NNB_LAUNCH_CHECK();
+  return NNB_OK;
+}
+
+template <typename T, int NK>
+int launch_narrow_columns(const nnb_project_args& a, int sms, int dev, cudaStream_t stream) {
+  if (a.n <= 32) return launch_narrow<T, NK, 1>(a, sms, dev, stream);
+  if (a.n <= 64) return launch_narrow<T, NK, 2>(a, sms, dev, stream);
+  if (a.n <= 96) return launch_narrow<T, NK, 3>(a, sms, dev, stream);
+  return launch_narrow<T, NK, 4>(a, sms, dev, stream);
+}
+
 template <typename T>
 int launch_project(nnb_project_args a, cudaStream_t stream) {
+  a.rows_per_index = std::min(a.rows_per_index, a.rows);
   int dev = 0, sms = 0;
   NNB_CUDA_CHECK(cudaGetDevice(&dev));
   NNB_CUDA_CHECK(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
@@ -638,6 +854,12 @@ int launch_project(nnb_project_args a, cudaStream_t stream) {
     NNB_LAUNCH_CHECK();
     a.x = rows;
     a.x_stride = a.weight_stride;
+  }
+  if (narrow(a)) {
+    if (a.k <= 32) return launch_narrow_columns<T, 1>(a, sms, dev, stream);
+    if (a.k <= 64) return launch_narrow_columns<T, 2>(a, sms, dev, stream);
+    if (a.k <= 96) return launch_narrow_columns<T, 3>(a, sms, dev, stream);
+    return launch_narrow_columns<T, 4>(a, sms, dev, stream);
   }
   project_low_kernel<T><<<dim3((unsigned)a.rows, a.rank / 16), 128, 0, stream>>>(a);
   NNB_LAUNCH_CHECK();
@@ -677,7 +899,7 @@ extern "C" int64_t nnb_project_workspace_bytes(const nnb_project_args* args) {
 extern "C" int32_t nnb_project(const nnb_project_args* args, void* stream) {
   NNB_REQUIRE(args != nullptr, "project: null args");
   const nnb_project_args& a = *args;
-  NNB_REQUIRE(a.x && a.weight && a.down && a.up && a.scales && a.index && a.out && a.low, "project: null pointer");
+  NNB_REQUIRE(a.x && a.weight && a.down && a.up && a.scales && a.index && a.out, "project: null pointer");
   NNB_REQUIRE(a.type == NNB_BF16 || a.type == NNB_F16, "project: rows must be bfloat16 or float16");
   NNB_REQUIRE(a.rows >= 1 && a.rows < (int64_t)1 << 31 && a.k >= 1 && a.n >= 1, "project: bad shape (%lld x %d -> %d)",
               (long long)a.rows, a.k, a.n);
@@ -690,6 +912,7 @@ extern "C" int32_t nnb_project(const nnb_project_args* args, void* stream) {
                   (reinterpret_cast<uintptr_t>(a.weight) | reinterpret_cast<uintptr_t>(a.down) |
                    reinterpret_cast<uintptr_t>(a.up) | reinterpret_cast<uintptr_t>(a.low)) % 16 == 0,
               "project: packed weights and workspace must be 16-byte aligned");
+  NNB_REQUIRE(a.low != nullptr || nnb_project_workspace_bytes(args) == 0, "project: missing workspace");
   return a.type == NNB_BF16 ? launch_project<__nv_bfloat16>(a, (cudaStream_t)stream)
                             : launch_project<__half>(a, (cudaStream_t)stream);
 }

@@ -1313,8 +1313,9 @@ def adapted_projection(x: torch.Tensor, projection: AdaptedProjection, index: to
     nbytes = int(_native.load().nnb_project_workspace_bytes(ctypes.byref(args)))
     if nbytes < 0:
         _native.check(nbytes, "adapted_projection")
-    workspace = torch.empty(nbytes, dtype=torch.uint8, device=device)
-    args.low = workspace.data_ptr()
+    if nbytes > 0:
+        workspace = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        args.low = workspace.data_ptr()
     token = PROFILE.start("adapted_projection", 2.0 * rows * (n * shape[-1] + rank * (n + shape[-1])),
                           2.0 * (rows * (n + shape[-1]) + n * shape[-1]), launches=2)
     _call_rows(_native.load().nnb_project, args, device, "adapted_projection")

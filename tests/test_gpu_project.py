@@ -109,6 +109,12 @@ SHAPES = [  # rows, k, n, ranks, index
     (3000, 40, 24, [5], "none"),
     (700, 4096, 16, [16, 16], "runs"),
     (260, 16, 2000, [16, 16, 2], "mixed"),
+    (5000, 128, 128, [32, 16, 7], "runs"),     # projections of few channels: every group count of 32
+    (333, 127, 97, [40, 16, 7], "mixed"),
+    (1, 96, 64, [200], "one"),
+    (77, 40, 96, [24] * 30, "mixed"),
+    (900, 90, 31, [2], "mixed"),
+    (4000, 31, 128, [64, 3], "runs"),
 ]
 
 

@@ -102,11 +102,11 @@ def _project_args(**over):
 
 
 @pytest.mark.parametrize("over", [
-    *(dict([(name, 0)]) for name in ("x", "weight", "down", "up", "scales", "index", "out", "low", "rows", "k", "n",
+    *(dict([(name, 0)]) for name in ("x", "weight", "down", "up", "scales", "index", "out", "rows", "k", "n",
                                      "adapters", "rank", "rows_per_index")),
     dict(rows=2 ** 31), dict(rank=8), dict(rank=272), dict(rank=24), dict(type=_native.F32), dict(x_stride=-1),
     dict(out_stride=7), dict(weight_stride=0), dict(weight_stride=12), dict(weight=18), dict(down=8), dict(up=4),
-    dict(low=20)])
+    dict(low=20), dict(low=0, k=256, weight_stride=256, x_stride=256)])
 def test_c_entry_refuses_projection(over):
     args = _project_args(**over)
     assert _native.load().nnb_project(ctypes.byref(args), None) == -1

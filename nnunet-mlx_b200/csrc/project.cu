@@ -6,25 +6,37 @@
 // down_a has the adapter's rank of rows, up_a that many columns; both are
 // padded with zeros to a common multiple of 16.
 //
-// project_low_kernel computes the low-rank rows scale_a down_a x_t in float32.
-// project_kernel is a tcgen05 GEMM over tiles of 128 rows x BN columns whose K
-// axis goes on past W's channels: for every adapter among a tile's rows it
-// appends the adapter's ranks, with the rows of other requests set to zero.
-// So adapters cost a tile a few more K-steps into the same accumulator, and
-// need neither sorting of the rows nor a pass over the output; requests whose
-// rows follow one another keep the number of adapters of a tile small.
+// Low-rank rows scale_a down_a x_t come first, in float32, as partial sums over
+// parts of the channels that their readers add up: project_low_kernel (a dot
+// product per warp) for up to 128 rows, project_low_tile_kernel (tcgen05) for
+// more.  project_kernel is a tcgen05 GEMM over tiles of 128 rows x BN columns
+// that adds the adapters in one of two ways, by the number of rows alone (so a
+// row's value does not depend on the rows beside it):
+//
+//  * more than 128 rows: the K axis goes on past W's channels.  For every
+//    adapter among a tile's rows it appends the adapter's ranks, with the rows
+//    of other requests set to zero, into the same accumulator.  It needs neither
+//    sorting of the rows nor a pass over the output; requests whose rows follow
+//    one another keep the adapters of a tile few.
+//  * FEW, up to 128 rows (serving: a row or some per request, each with another
+//    adapter): the product with up is a float32 dot product per output, summed
+//    in shared memory while W streams through the tensor cores.  Every up_a is
+//    read once either way; appended K-steps would cost a stage per adapter.
 //
 // Roles of project_kernel's warps:
 //   0      TMA producer of x and W chunks (64 channels a stage, 128-byte swizzle)
 //   1      MMA issuer (one thread) and TMEM owner
-//   2-5    adapter producers, a thread per row: list the tile's adapters, and
-//          for each write the rows' low-rank values into a stage, as two
+//   2-5    adapter producers.  They list the tile's adapters and for each write
+//          the rows' low-rank values into a stage, a thread per row, as two
 //          bfloat16 parts hi + lo (2^-17 of the value at most is lost; a single
-//          bfloat16 would cost the output as much as its own rounding)
+//          bfloat16 would cost the output as much as its own rounding); FEW: the
+//          dot products
 //   6-9    epilogue: TMEM -> bias -> 16-bit rows, one of two accumulators each
 // W's chunks and the adapters' have rings of their own, so each producer runs
 // ahead as far as its ring allows; warps 2-5 announce the number of adapters of
 // a tile, which only the MMA issuer needs.
+//
+// Up to 128 channels on either side project_narrow_kernel does it all at once.
 #include <cuda.h>
 #include <cudaTypedefs.h>
 #include <cuda_bf16.h>
@@ -51,7 +63,7 @@ namespace {
 
 using namespace tc;
 
-constexpr int kBadIndex = 41;  // site number of an adapter index out of range; 42-52 are waits
+constexpr int kBadIndex = 41;  // site number of an adapter index out of range; 42-62 are waits
 
 constexpr int kThreads = 320;
 constexpr int kStageA = BM * 128;
@@ -125,7 +137,7 @@ __global__ void __launch_bounds__(256) align_rows_kernel(const uint16_t* x, int6
 }
 
 // ---------------------------------------------------------------------------
-// low[t][j] = scale_a sum_k down_a[j][k] x[t][k]: a warp takes four ranks of one row.
+// low[p][t][j] = scale_a sum over part p of k of down_a[j][k] x[t][k]: a warp takes four ranks of one row.
 // ---------------------------------------------------------------------------
 template <typename T>
 __device__ __forceinline__ void widen(float (&v)[8], const uint4& raw) {
@@ -135,7 +147,8 @@ __device__ __forceinline__ void widen(float (&v)[8], const uint4& raw) {
 }
 
 template <typename T>
-__global__ void __launch_bounds__(128) project_low_kernel(const nnb_project_args a) {
+__global__ void __launch_bounds__(128) project_low_kernel(const nnb_project_args a, const int part) {
+  asm volatile("griddepcontrol.launch_dependents;");
   const int64_t row = blockIdx.x;
   const int adapter = row_adapter(a, row);
   if (adapter < 0) return;
@@ -143,8 +156,10 @@ __global__ void __launch_bounds__(128) project_low_kernel(const nnb_project_args
   const T* x = reinterpret_cast<const T*>(a.x) + row * a.x_stride;
   const T* down = reinterpret_cast<const T*>(a.down) + ((int64_t)adapter * a.rank + j0) * a.weight_stride;
   float sum[4] = {0.f, 0.f, 0.f, 0.f};
-  const int whole = a.k & ~7;
-  for (int k = lane * 8; k < whole; k += 256) {
+  const int begin = blockIdx.z * part, end = min(a.k, begin + part);
+  const int whole = begin + ((end - begin) & ~7);
+#pragma unroll 2
+  for (int k = begin + lane * 8; k < whole; k += 256) {
     float v[8], d[8];
     widen<T>(v, *reinterpret_cast<const uint4*>(x + k));
 #pragma unroll
@@ -154,7 +169,7 @@ __global__ void __launch_bounds__(128) project_low_kernel(const nnb_project_args
       for (int i = 0; i < 8; ++i) sum[j] = fmaf(v[i], d[i], sum[j]);
     }
   }
-  if (whole + lane < a.k) {
+  if (whole + lane < end) {
     const float v = value(x[whole + lane]);
 #pragma unroll
     for (int j = 0; j < 4; ++j) sum[j] = fmaf(v, value(down[j * a.weight_stride + whole + lane]), sum[j]);
@@ -163,13 +178,22 @@ __global__ void __launch_bounds__(128) project_low_kernel(const nnb_project_args
   for (int j = 0; j < 4; ++j) {
 #pragma unroll
     for (int h = 16; h >= 1; h >>= 1) sum[j] += __shfl_xor_sync(0xffffffffu, sum[j], h);
-    if (lane == j) a.low[row * a.rank + j0 + j] = sum[j] * __ldg(a.scales + adapter);
+    if (lane == j)
+      a.low[(blockIdx.z * a.rows + row) * a.rank + j0 + j] = sum[j] * __ldg(a.scales + adapter);
   }
 }
 
-// ---------------------------------------------------------------------------
-// The GEMM.
-// ---------------------------------------------------------------------------
+// Four low-rank values of a row from rank j on: the sum of its parts.
+__device__ __forceinline__ float4 low_values(const nnb_project_args& a, int parts, int64_t row, int j) {
+  const float* src = a.low + row * a.rank + j;
+  float4 v = *reinterpret_cast<const float4*>(src);
+  for (int p = 1; p < parts; ++p) {
+    const float4 w = *reinterpret_cast<const float4*>(src + p * a.rows * a.rank);
+    v.x += w.x, v.y += w.y, v.z += w.z, v.w += w.w;
+  }
+  return v;
+}
+
 __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, int c0, int c1, uint32_t bar) {
   asm volatile(
       "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
@@ -212,6 +236,217 @@ __device__ __forceinline__ bool adapter_barrier(bool ok) {
   return all != 0;
 }
 
+// The adapters among a tile's rows in ascending order, by the four adapter warps (thread r holds row r's in
+// `mine`, -1 for none); returns their number.  One adapter per turn; two buffers of minima need one barrier a turn.
+__device__ __forceinline__ int list_adapters(int mine, int r, volatile int* smallest, volatile int* listed,
+                                             int& turn) {
+  int count = 0;
+  for (int low = -1;;) {
+    const int least = __reduce_min_sync(0xffffffffu, mine > low ? mine : INT_MAX);
+    if ((r & 31) == 0) smallest[turn * 4 + (r >> 5)] = least;
+    adapter_barrier(true);
+    low = min(min(smallest[turn * 4], smallest[turn * 4 + 1]), min(smallest[turn * 4 + 2], smallest[turn * 4 + 3]));
+    turn ^= 1;
+    if (low == INT_MAX) return count;
+    if (r == 0) listed[count] = low;
+    ++count;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Low-rank rows of more than 128 rows.  A CTA takes 128 rows and a part of the
+// channels: x's chunk against the down rows of the tile's adapters, as many as
+// fit 128 columns of one MMA at a time.  Bound by reading x once, so two CTAs
+// share an SM to keep its loads coming while one starts or ends.
+// ---------------------------------------------------------------------------
+constexpr int kLowColumns = 128;
+constexpr int kLowStage = kStageA + kLowColumns * 128;
+constexpr int kLowStages = 3;
+constexpr int kLowThreads = 192;
+constexpr int kLowSmem = 1024 + kLowStages * kLowStage + 1024;
+
+struct LowMaps {
+  CUtensorMap x, down;
+};
+
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, float (&v)[16]) {
+  uint32_t r[16];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+      "%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kLowThreads, 2)
+    project_low_tile_kernel(const nnb_project_args a, const __grid_constant__ LowMaps maps, const int part) {
+  constexpr bool kF16 = !std::is_same<T, __nv_bfloat16>::value;
+  constexpr int S = kLowStages;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* stages = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* full = reinterpret_cast<uint64_t*>(stages + S * kLowStage);
+  uint64_t* empty = full + S;
+  uint64_t* acc_full = empty + S;
+  uint64_t* acc_empty = acc_full + 1;
+  uint64_t* drain = acc_empty + 1;
+  volatile int* smallest = reinterpret_cast<volatile int*>(drain + 1);
+  volatile int* listed = smallest + 8;
+  volatile int* list_count = listed + BM;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(const_cast<int*>(list_count + 1));
+  int* abort_flag = reinterpret_cast<int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t row0 = (int64_t)blockIdx.x * BM;
+  const int first_chunk = blockIdx.y * part, chunks = min((a.k + 63) / 64 - first_chunk, part);
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < S; ++s) {
+      mbar_init(smem_u32(&full[s]), 1);
+      mbar_init(smem_u32(&empty[s]), 1);
+    }
+    mbar_init(smem_u32(acc_full), 1);
+    mbar_init(smem_u32(acc_empty), 4);
+    mbar_init(smem_u32(drain), 1);
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                 "r"(kLowColumns)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  const int r = threadIdx.x - 64;
+  int mine = -1;
+  if (warp >= 2) {
+    if (row0 + r < a.rows) mine = row_adapter(a, row0 + r);
+    int turn = 0;
+    const int count = list_adapters(mine, r, smallest, listed, turn);
+    if (r == 0) *list_count = count;
+  }
+  fence_before();
+  __syncthreads();
+  fence_after();
+  const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(tmem_slot);
+  const int count = *list_count;
+  // The GEMM may start from here on, and not before this CTA holds its TMEM: a GEMM CTA that took all of an SM's
+  // columns first would keep them until this grid has ended.
+  asm volatile("griddepcontrol.launch_dependents;");
+  // a pass: `together` adapters of all their ranks, or 128 ranks (the last of them fewer) of one
+  const int blocks = (a.rank + kLowColumns - 1) / kLowColumns;
+  const int together = max(1, kLowColumns / a.rank);
+  const int passes = blocks > 1 ? count * blocks : (count + together - 1) / together;
+  const int box = min(a.rank, kLowColumns);
+
+  if (warp == 0) {
+    if (lane == 0) {
+      Ring<S> ring;
+      int issued = 0;
+      bool alive = true;
+      for (int p = 0; p < passes && alive; ++p) {
+        const int from = blocks > 1 ? p / blocks : p * together;
+        const int to = blocks > 1 ? from + 1 : min(count, from + together);
+        for (int c = first_chunk; c < first_chunk + chunks; ++c) {
+          if (!mbar_wait(smem_u32(&empty[ring.s]), ring.phase ^ 1, abort_flag, 53)) {
+            alive = false;
+            break;
+          }
+          const uint32_t bar = smem_u32(&full[ring.s]), at = smem_u32(stages + ring.s * kLowStage);
+          mbar_arrive_expect_tx(bar, kStageA + (to - from) * box * 128);
+          tma_load_2d(at, &maps.x, c * 64, (int)row0, bar);
+          for (int i = from; i < to; ++i)
+            tma_load_3d(at + kStageA + (i - from) * box * 128, &maps.down, c * 64, (p % blocks) * kLowColumns,
+                        listed[i], bar);
+          ring.next();
+          ++issued;
+        }
+      }
+      if (*reinterpret_cast<volatile int*>(abort_flag))
+        for (int g = max(0, issued - S); g < issued; ++g)
+          mbar_wait(smem_u32(&full[g % S]), (uint32_t)(g / S) & 1, abort_flag, 54, false);
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    if (lane == 0) {
+      Ring<S> ring;
+      bool alive = true;
+      for (int p = 0; p < passes && alive; ++p) {
+        if (!mbar_wait(smem_u32(acc_empty), (uint32_t)(p & 1) ^ 1, abort_flag, 55)) break;
+        fence_after();
+        const int columns = blocks > 1 ? min(kLowColumns, a.rank - (p % blocks) * kLowColumns)
+                                       : (min(count, (p + 1) * together) - p * together) * a.rank;
+        const uint32_t idesc = kF16 ? idesc_f16(BM, columns) : idesc_bf16(BM, columns);
+        uint32_t accumulate = 0;
+        for (int c = first_chunk; c < first_chunk + chunks; ++c) {
+          if (!mbar_wait(smem_u32(&full[ring.s]), ring.phase, abort_flag, 56)) {
+            alive = false;
+            break;
+          }
+          fence_after();
+          const uint32_t at = smem_u32(stages + ring.s * kLowStage);
+          const uint64_t ad = sw128_desc(at), bd = sw128_desc(at + kStageA);
+          const int steps = min(4, (a.k - c * 64 + 15) / 16);
+          for (int k = 0; k < steps; ++k) {
+            mma_f16(tmem, ad + k * 2, bd + k * 2, idesc, accumulate);
+            accumulate = 1;
+          }
+          mma_commit(smem_u32(&empty[ring.s]));
+          ring.next();
+        }
+        if (alive) mma_commit(smem_u32(acc_full));
+      }
+      if (*reinterpret_cast<volatile int*>(abort_flag)) {
+        mma_commit(smem_u32(drain));
+        mbar_wait(smem_u32(drain), 0, abort_flag, 57, false);
+      }
+    }
+    __syncwarp();
+  } else {
+    const int quarter = warp & 3;
+    const int64_t row = row0 + quarter * 32 + lane;
+    const int own = row < a.rows ? row_adapter(a, row) : -1;  // the lane's TMEM row, not the listed one
+    float* out = a.low + (blockIdx.y * a.rows + row) * a.rank;
+    const float scale = own < 0 ? 0.f : __ldg(a.scales + own);
+    for (int p = 0; p < passes; ++p) {
+      const int from = blocks > 1 ? p / blocks : p * together;
+      const int to = blocks > 1 ? from + 1 : min(count, from + together);
+      const int j0 = (p % blocks) * kLowColumns, width = min(kLowColumns, a.rank - j0);
+      const bool ok = mbar_wait(smem_u32(acc_full), (uint32_t)p & 1, abort_flag, 58);
+      if (!__all_sync(0xffffffffu, ok)) break;
+      fence_after();
+      for (int i = from; i < to; ++i) {
+        const int adapter = listed[i];
+        if (!__any_sync(0xffffffffu, own == adapter)) continue;
+        for (int j = 0; j < width; j += 16) {
+          float v[16];
+          tmem_ld16(tmem + ((uint32_t)quarter << 21) + (i - from) * box + j, v);
+          if (own == adapter) {
+#pragma unroll
+            for (int e = 0; e < 16; e += 4)
+              *reinterpret_cast<float4*>(out + j0 + j + e) =
+                  make_float4(v[e] * scale, v[e + 1] * scale, v[e + 2] * scale, v[e + 3] * scale);
+          }
+        }
+      }
+      fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(acc_empty));
+    }
+  }
+  __syncthreads();
+  if (warp == 1) {
+    fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kLowColumns) : "memory");
+  }
+}
+
+// ---------------------------------------------------------------------------
+// The GEMM.
+// ---------------------------------------------------------------------------
 struct TileAt {
   int64_t row0;
   int col0;
@@ -225,15 +460,17 @@ __device__ __forceinline__ TileAt tile_at(int64_t tile, int64_t row_tiles, int c
   return {(group * 16 + rest % rows) * BM, (int)(rest / rows) * bn};
 }
 
-template <typename T, int BN>
+template <typename T, int BN, bool FEW>
 __global__ void __launch_bounds__(kThreads, Tile<BN>::kCtas)
-    project_kernel(const nnb_project_args a, const __grid_constant__ Maps maps) {
+    project_kernel(const nnb_project_args a, const __grid_constant__ Maps maps, const int parts) {
   using C = Tile<BN>;
   constexpr int S = C::kStages, SL = C::kLowStages;
   constexpr bool kF16 = !std::is_same<T, __nv_bfloat16>::value;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* stages = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* low_stages = stages + S * C::kStage;
+  float* sums = reinterpret_cast<float*>(low_stages);  // FEW: the adapters' share, 128 rows of BN + 1
+  static_assert(!FEW || BM * (BN + 1) * 4 <= SL * C::kStage, "the sums exceed the adapters' stages");
   uint8_t* staging = low_stages + SL * C::kStage;
   float* bias_rows = reinterpret_cast<float*>(staging + 4 * C::kStaging);
   uint64_t* full = reinterpret_cast<uint64_t*>(bias_rows + 4 * BN);
@@ -265,8 +502,8 @@ __global__ void __launch_bounds__(kThreads, Tile<BN>::kCtas)
       mbar_init(smem_u32(&empty[s]), 1);
     }
     for (int s = 0; s < SL; ++s) {
-      mbar_init(smem_u32(&low_full[s]), 1);
-      mbar_init(smem_u32(&low_empty[s]), 1);
+      mbar_init(smem_u32(&low_full[s]), FEW ? 4 : 1);  // FEW: the adapter warps and the epilogue's
+      mbar_init(smem_u32(&low_empty[s]), FEW ? 4 : 1);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(smem_u32(&acc_full[i]), 1);
@@ -348,10 +585,14 @@ __global__ void __launch_bounds__(kThreads, Tile<BN>::kCtas)
           mma_commit(smem_u32(&empty[ring.s]));
           ring.next();
         }
-        if (!alive || !mbar_wait(smem_u32(&count_full[counted.s]), counted.phase, abort_flag, 46)) break;
-        const int low_stages_due = counts[counted.s] * blocks;
-        mbar_arrive(smem_u32(&count_empty[counted.s]));
-        counted.next();
+        if (!alive) break;
+        int low_stages_due = 0;
+        if constexpr (!FEW) {
+          if (!mbar_wait(smem_u32(&count_full[counted.s]), counted.phase, abort_flag, 46)) break;
+          low_stages_due = counts[counted.s] * blocks;
+          mbar_arrive(smem_u32(&count_empty[counted.s]));
+          counted.next();
+        }
         for (int i = 0; i < low_stages_due; ++i) {
           if (!mbar_wait(smem_u32(&low_full[low_ring.s]), low_ring.phase, abort_flag, 47)) {
             alive = false;
@@ -379,6 +620,46 @@ __global__ void __launch_bounds__(kThreads, Tile<BN>::kCtas)
     __syncwarp();
   } else if (warp < 6) {
     // ---------------------------- adapter producers --------------------------
+    // The low-rank rows are the previous kernel's, which may still run; every CTA waits for its end.
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    if constexpr (FEW) {
+      const int planes = kF16 ? 2 : 1;
+      for (int it = 0; it < my_tiles; ++it) {
+        const TileAt t = tile_at(blockIdx.x + (int64_t)it * gridDim.x, row_tiles, col_tiles, BN);
+        const bool ok = mbar_wait(smem_u32(low_empty), (uint32_t)(it & 1) ^ 1, abort_flag, 59);
+        if (!__all_sync(0xffffffffu, ok)) break;
+#pragma unroll 4
+        for (int row = warp - 2; row < (int)a.rows; row += 4) {
+          const int adapter = row_adapter(a, row);
+#pragma unroll
+          for (int h = 0; h < BN; h += 32) {
+            float sum = 0.f;
+            if (adapter >= 0) {
+              const int col = min(t.col0 + h + lane, a.n - 1);  // columns past n are not stored
+              const __nv_bfloat16* up = reinterpret_cast<const __nv_bfloat16*>(a.up) +
+                                        ((int64_t)adapter * a.n + col) * planes * a.rank;
+              for (int j = 0; j < a.rank; j += 8) {
+                const float4 l0 = low_values(a, parts, row, j), l1 = low_values(a, parts, row, j + 4);
+                const float l[8] = {l0.x, l0.y, l0.z, l0.w, l1.x, l1.y, l1.z, l1.w};
+                float u[8];
+                widen<__nv_bfloat16>(u, __ldg(reinterpret_cast<const uint4*>(up + j)));
+                if constexpr (kF16) {
+                  float rest[8];
+                  widen<__nv_bfloat16>(rest, __ldg(reinterpret_cast<const uint4*>(up + a.rank + j)));
+#pragma unroll
+                  for (int e = 0; e < 8; ++e) u[e] += rest[e];
+                }
+#pragma unroll
+                for (int e = 0; e < 8; ++e) sum = fmaf(l[e], u[e], sum);
+              }
+            }
+            sums[row * (BN + 1) + h + lane] = sum;
+          }
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(low_full));
+      }
+    } else {
     const int r = threadIdx.x - 64;
     const bool leader = r == 0;
     Ring<SL> ring;
@@ -391,19 +672,7 @@ __global__ void __launch_bounds__(kThreads, Tile<BN>::kCtas)
       const TileAt t = tile_at(blockIdx.x + (int64_t)it * gridDim.x, row_tiles, col_tiles, BN);
       const int64_t row = t.row0 + r;
       const int mine = row < a.rows ? row_adapter(a, row) : -1;
-      // the tile's adapters in ascending order, one per turn (a second buffer of minima needs one barrier a turn)
-      int count = 0;
-      for (int low = -1;;) {
-        const int least = __reduce_min_sync(0xffffffffu, mine > low ? mine : INT_MAX);
-        if (lane == 0) smallest[turn * 4 + warp - 2] = least;
-        adapter_barrier(true);
-        low = min(min(smallest[turn * 4], smallest[turn * 4 + 1]),
-                  min(smallest[turn * 4 + 2], smallest[turn * 4 + 3]));
-        turn ^= 1;
-        if (low == INT_MAX) break;
-        if (leader) listed[count] = low;
-        ++count;
-      }
+      const int count = list_adapters(mine, r, smallest, listed, turn);
       if (leader) {
         alive = mbar_wait(smem_u32(&count_empty[counted.s]), counted.phase ^ 1, abort_flag, 49);
         counts[counted.s] = count;
@@ -418,7 +687,7 @@ __global__ void __launch_bounds__(kThreads, Tile<BN>::kCtas)
 #pragma unroll
         for (int j = 0; j < kRankBlock; j += 4) {
           float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
-          if (own && j0 + j < a.rank) f = *reinterpret_cast<const float4*>(a.low + row * a.rank + j0 + j);
+          if (own && j0 + j < a.rank) f = low_values(a, parts, row, j0 + j);
           v[j] = f.x, v[j + 1] = f.y, v[j + 2] = f.z, v[j + 3] = f.w;
         }
         alive = alive && mbar_wait(smem_u32(&low_empty[ring.s]), ring.phase ^ 1, abort_flag, 50);
@@ -458,6 +727,7 @@ __global__ void __launch_bounds__(kThreads, Tile<BN>::kCtas)
     if (leader && *reinterpret_cast<volatile int*>(abort_flag))
       for (int g = max(0, issued - SL); g < issued; ++g)
         mbar_wait(smem_u32(&low_full[g % SL]), (uint32_t)(g / SL) & 1, abort_flag, 51, false);
+    }
     __syncwarp();
   } else {
     // -------------------------------- epilogue -------------------------------
@@ -473,6 +743,10 @@ __global__ void __launch_bounds__(kThreads, Tile<BN>::kCtas)
       __syncwarp();
       const bool ok = mbar_wait(smem_u32(&acc_full[acc]), (uint32_t)(it >> 1) & 1, abort_flag, 52);
       if (!__all_sync(0xffffffffu, ok)) break;
+      if constexpr (FEW) {
+        const bool summed = mbar_wait(smem_u32(low_full), (uint32_t)it & 1, abort_flag, 60);
+        if (!__all_sync(0xffffffffu, summed)) break;
+      }
       fence_after();
       const uint32_t src = tmem + acc * BN + ((uint32_t)quarter << 21);
       const int64_t row0 = t.row0 + quarter * 32;
@@ -484,6 +758,10 @@ __global__ void __launch_bounds__(kThreads, Tile<BN>::kCtas)
         for (int h = 0; h < C::kColumns; h += 32) {
           float v[32];
           tmem_ld32(src + c0 + h, v);
+          if constexpr (FEW) {
+#pragma unroll
+            for (int c = 0; c < 32; ++c) v[c] += sums[(quarter * 32 + lane) * (BN + 1) + c0 + h + c];
+          }
           uint4* line = reinterpret_cast<uint4*>(stage_rows + lane * C::kColumns * 2);
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
@@ -521,7 +799,10 @@ __global__ void __launch_bounds__(kThreads, Tile<BN>::kCtas)
       }
       fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&acc_empty[acc]));
+      if (lane == 0) {
+        mbar_arrive(smem_u32(&acc_empty[acc]));
+        if constexpr (FEW) mbar_arrive(smem_u32(low_empty));
+      }
     }
   }
   __syncthreads();
@@ -570,26 +851,78 @@ bool rows_in_place(const nnb_project_args& a) {
 
 bool narrow(const nnb_project_args& a) { return a.k <= 128 && a.n <= 128; }
 
-int64_t low_bytes(const nnb_project_args& a) { return narrow(a) ? 0 : a.rows * a.rank * (int64_t)sizeof(float); }
+// How the low-rank rows are computed: by tiles or by rows, in how many parts of the channels.
+struct LowPlan {
+  bool few;   // up to one tile of rows
+  int parts;  // partial sums
+  int part;   // channels (few) or chunks of 64 of a part
+};
 
-template <typename T, int BN>
-int launch_tiles(const nnb_project_args& a, int sms, int dev, cudaStream_t stream) {
+// Enough parts that some 300 CTAs run (two per SM), of at least 512 channels (four loads of a lane) or four
+// chunks, and no more than eight, which their readers add up.
+LowPlan low_plan(const nnb_project_args& a) {
+  LowPlan p;
+  p.few = a.rows <= BM;
+  const int64_t units = p.few ? a.rows * (a.rank / 16) : (a.rows + BM - 1) / BM;
+  const int total = p.few ? a.k : (a.k + 63) / 64, least = p.few ? 512 : 4;
+  const int wanted = (int)std::min<int64_t>(8, std::max<int64_t>(1, 300 / units));
+  const int parts = std::max(1, std::min(wanted, total / least));
+  p.part = (total + parts - 1) / parts;
+  if (p.few) p.part = (p.part + 255) / 256 * 256;  // whole loads of a warp
+  p.parts = (total + p.part - 1) / p.part;
+  return p;
+}
+
+int64_t low_bytes(const nnb_project_args& a) {
+  return narrow(a) ? 0 : low_plan(a).parts * a.rows * a.rank * (int64_t)sizeof(float);
+}
+
+int encode_rows(CUtensorMap* map, bool f16, const nnb_project_args& a) {
+  const cuuint64_t dims[2] = {(cuuint64_t)a.k, (cuuint64_t)a.rows};
+  const cuuint64_t strides[1] = {(cuuint64_t)(a.rows == 1 ? (a.k + 7) / 8 * 8 : a.x_stride) * 2};
+  const cuuint32_t box[2] = {64, BM};
+  return encode(map, f16, 2, a.x, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+template <typename T>
+int launch_low(const nnb_project_args& a, const LowPlan& plan, int dev, cudaStream_t stream) {
+  constexpr bool kF16 = !std::is_same<T, __nv_bfloat16>::value;
+  if (plan.few) {
+    project_low_kernel<T><<<dim3((unsigned)a.rows, a.rank / 16, plan.parts), 128, 0, stream>>>(a, plan.part);
+    NNB_LAUNCH_CHECK();
+    return NNB_OK;
+  }
+  static bool configured[64] = {false};
+  if (dev >= 64 || !configured[dev]) {
+    NNB_CUDA_CHECK(
+        cudaFuncSetAttribute(project_low_tile_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kLowSmem));
+    if (dev < 64) configured[dev] = true;
+  }
+  LowMaps maps;
+  if (const int rc = encode_rows(&maps.x, kF16, a)) return rc;
+  const cuuint64_t dims[3] = {(cuuint64_t)a.k, (cuuint64_t)a.rank, (cuuint64_t)a.adapters};
+  const cuuint64_t strides[2] = {(cuuint64_t)a.weight_stride * 2, (cuuint64_t)a.weight_stride * 2 * a.rank};
+  const cuuint32_t box[3] = {64, (cuuint32_t)std::min(a.rank, kLowColumns), 1};
+  if (const int rc = encode(&maps.down, kF16, 3, a.down, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B)) return rc;
+  const dim3 grid((unsigned)((a.rows + BM - 1) / BM), plan.parts);
+  project_low_tile_kernel<T><<<grid, kLowThreads, kLowSmem, stream>>>(a, maps, plan.part);
+  NNB_LAUNCH_CHECK();
+  return NNB_OK;
+}
+
+template <typename T, int BN, bool FEW>
+int launch_tiles(const nnb_project_args& a, const LowPlan& plan, int sms, int dev, cudaStream_t stream) {
   using C = Tile<BN>;
   constexpr bool kF16 = !std::is_same<T, __nv_bfloat16>::value;
   static bool configured[64] = {false};
   if (dev >= 64 || !configured[dev]) {
     NNB_CUDA_CHECK(
-        cudaFuncSetAttribute(project_kernel<T, BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
+        cudaFuncSetAttribute(project_kernel<T, BN, FEW>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
     if (dev < 64) configured[dev] = true;
   }
   static_assert(C::kSmem * C::kCtas <= kMaxSmem + 1024 * (C::kCtas - 1), "the tile's stages exceed shared memory");
   Maps maps;
-  {
-    const cuuint64_t dims[2] = {(cuuint64_t)a.k, (cuuint64_t)a.rows};
-    const cuuint64_t strides[1] = {(cuuint64_t)(a.rows == 1 ? (a.k + 7) / 8 * 8 : a.x_stride) * 2};
-    const cuuint32_t box[2] = {64, BM};
-    if (const int rc = encode(&maps.x, kF16, 2, a.x, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B)) return rc;
-  }
+  if (const int rc = encode_rows(&maps.x, kF16, a)) return rc;
   {
     const cuuint64_t dims[2] = {(cuuint64_t)a.k, (cuuint64_t)a.n};
     const cuuint64_t strides[1] = {(cuuint64_t)a.weight_stride * 2};
@@ -606,8 +939,18 @@ int launch_tiles(const nnb_project_args& a, int sms, int dev, cudaStream_t strea
   }
   const int64_t tiles = (a.rows + BM - 1) / BM * ((a.n + BN - 1) / BN);
   const int grid = (int)std::min<int64_t>(tiles, (int64_t)sms * C::kCtas);
-  project_kernel<T, BN><<<grid, kThreads, C::kSmem, stream>>>(a, maps);
-  NNB_LAUNCH_CHECK();
+  // launched while the low-rank kernel still runs: only the adapter warps wait for it (griddepcontrol)
+  cudaLaunchAttribute early[1];
+  early[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3(grid);
+  config.blockDim = dim3(kThreads);
+  config.dynamicSmemBytes = C::kSmem;
+  config.stream = stream;
+  config.attrs = early;
+  config.numAttrs = 1;
+  NNB_CUDA_CHECK(cudaLaunchKernelEx(&config, project_kernel<T, BN, FEW>, a, maps, plan.parts));
   return NNB_OK;
 }
 
@@ -861,13 +1204,16 @@ int launch_project(nnb_project_args a, cudaStream_t stream) {
     if (a.k <= 96) return launch_narrow_columns<T, 3>(a, sms, dev, stream);
     return launch_narrow_columns<T, 4>(a, sms, dev, stream);
   }
-  project_low_kernel<T><<<dim3((unsigned)a.rows, a.rank / 16), 128, 0, stream>>>(a);
-  NNB_LAUNCH_CHECK();
+  const LowPlan plan = low_plan(a);
+  if (const int rc = launch_low<T>(a, plan, dev, stream)) return rc;
+  if (plan.few)
+    return (a.n + 31) / 32 <= 2 * sms ? launch_tiles<T, 32, true>(a, plan, sms, dev, stream)
+                                      : launch_tiles<T, 64, true>(a, plan, sms, dev, stream);
   switch (tile_columns(a, sms)) {
-    case 32: return launch_tiles<T, 32>(a, sms, dev, stream);
-    case 64: return launch_tiles<T, 64>(a, sms, dev, stream);
-    case 128: return launch_tiles<T, 128>(a, sms, dev, stream);
-    default: return launch_tiles<T, 256>(a, sms, dev, stream);
+    case 32: return launch_tiles<T, 32, false>(a, plan, sms, dev, stream);
+    case 64: return launch_tiles<T, 64, false>(a, plan, sms, dev, stream);
+    case 128: return launch_tiles<T, 128, false>(a, plan, sms, dev, stream);
+    default: return launch_tiles<T, 256, false>(a, plan, sms, dev, stream);
   }
 }
 
@@ -891,7 +1237,8 @@ int project_device_status(int32_t* where, bool reset) {
 using namespace nnb;
 
 extern "C" int64_t nnb_project_workspace_bytes(const nnb_project_args* args) {
-  NNB_REQUIRE(args != nullptr && args->rows >= 1 && args->rank >= 16 && args->weight_stride >= 1,
+  NNB_REQUIRE(args != nullptr && args->rows >= 1 && args->rank >= 16 && args->k >= 1 &&
+                  args->weight_stride >= 1,
               "project_workspace_bytes: bad shape");
   return low_bytes(*args) + (rows_in_place(*args) ? 0 : args->rows * args->weight_stride * 2);
 }

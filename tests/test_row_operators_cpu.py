@@ -115,8 +115,9 @@ def test_c_entry_refuses_projection(over):
 
 def test_projection_workspace():
     load = _native.load()
-    assert load.nnb_project_workspace_bytes(ctypes.byref(_project_args(rows=10, rank=32))) >= 10 * 32 * 4
-    assert load.nnb_project_workspace_bytes(ctypes.byref(_project_args(rows=0))) == -1
+    assert load.nnb_project_workspace_bytes(ctypes.byref(_project_args(rows=10, rank=32, k=256))) >= 10 * 32 * 4
+    for bad in (dict(rows=0), dict(k=0), dict(rank=0)):
+        assert load.nnb_project_workspace_bytes(ctypes.byref(_project_args(**bad))) == -1
     assert load.nnb_project_workspace_bytes(None) == -1
     assert load.nnb_project(None, None) == -1
 

@@ -9,19 +9,19 @@
 // Low-rank rows scale_a down_a x_t come first, in float32, as partial sums over
 // parts of the channels that their readers add up: project_low_kernel (a dot
 // product per warp) for up to 128 rows, project_low_tile_kernel (tcgen05) for
-// more.  project_kernel is a tcgen05 GEMM over tiles of 128 rows x BN columns
-// that adds the adapters in one of two ways, by the number of rows alone (so a
-// row's value does not depend on the rows beside it):
+// more.  Then, by the number of rows alone (so a row's value does not depend on
+// the rows beside it):
 //
-//  * more than 128 rows: the K axis goes on past W's channels.  For every
-//    adapter among a tile's rows it appends the adapter's ranks, with the rows
-//    of other requests set to zero, into the same accumulator.  It needs neither
-//    sorting of the rows nor a pass over the output; requests whose rows follow
-//    one another keep the adapters of a tile few.
-//  * FEW, up to 128 rows (serving: a row or some per request, each with another
-//    adapter): the product with up is a float32 dot product per output, summed
-//    in shared memory while W streams through the tensor cores.  Every up_a is
-//    read once either way; appended K-steps would cost a stage per adapter.
+//  * more than 128 rows, project_kernel: a tcgen05 GEMM over tiles of 128 rows x
+//    BN columns whose K axis goes on past W's channels.  For every adapter among
+//    a tile's rows it appends the adapter's ranks, with the rows of other
+//    requests set to zero, into the same accumulator.  It needs neither sorting
+//    of the rows nor a pass over the output; requests whose rows follow one
+//    another keep the adapters of a tile few.
+//  * up to 128 rows (serving: a row or some per request, each with another
+//    adapter), project_few_kernel: W's rows are the MMA's 128 and the requests'
+//    its columns, so that nearly every byte staged is W's; clusters split K.
+//    The product with up is a float32 dot product per output while W streams.
 //
 // Roles of project_kernel's warps:
 //   0      TMA producer of x and W chunks (64 channels a stage, 128-byte swizzle)
@@ -29,8 +29,7 @@
 //   2-5    adapter producers.  They list the tile's adapters and for each write
 //          the rows' low-rank values into a stage, a thread per row, as two
 //          bfloat16 parts hi + lo (2^-17 of the value at most is lost; a single
-//          bfloat16 would cost the output as much as its own rounding); FEW: the
-//          dot products
+//          bfloat16 would cost the output as much as its own rounding)
 //   6-9    epilogue: TMEM -> bias -> 16-bit rows, one of two accumulators each
 // W's chunks and the adapters' have rings of their own, so each producer runs
 // ahead as far as its ring allows; warps 2-5 announce the number of adapters of
@@ -63,7 +62,7 @@ namespace {
 
 using namespace tc;
 
-constexpr int kBadIndex = 41;  // site number of an adapter index out of range; 42-62 are waits
+constexpr int kBadIndex = 41;  // site number of an adapter index out of range; 42-63 are waits
 
 constexpr int kThreads = 320;
 constexpr int kStageA = BM * 128;
@@ -460,7 +459,7 @@ __device__ __forceinline__ TileAt tile_at(int64_t tile, int64_t row_tiles, int c
   return {(group * 16 + rest % rows) * BM, (int)(rest / rows) * bn};
 }
 
-template <typename T, int BN, bool FEW>
+template <typename T, int BN>
 __global__ void __launch_bounds__(kThreads, Tile<BN>::kCtas)
     project_kernel(const nnb_project_args a, const __grid_constant__ Maps maps, const int parts) {
   using C = Tile<BN>;
@@ -469,8 +468,6 @@ __global__ void __launch_bounds__(kThreads, Tile<BN>::kCtas)
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* stages = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* low_stages = stages + S * C::kStage;
-  float* sums = reinterpret_cast<float*>(low_stages);  // FEW: the adapters' share, 128 rows of BN + 1
-  static_assert(!FEW || BM * (BN + 1) * 4 <= SL * C::kStage, "the sums exceed the adapters' stages");
   uint8_t* staging = low_stages + SL * C::kStage;
   float* bias_rows = reinterpret_cast<float*>(staging + 4 * C::kStaging);
   uint64_t* full = reinterpret_cast<uint64_t*>(bias_rows + 4 * BN);
@@ -502,8 +499,8 @@ __global__ void __launch_bounds__(kThreads, Tile<BN>::kCtas)
       mbar_init(smem_u32(&empty[s]), 1);
     }
     for (int s = 0; s < SL; ++s) {
-      mbar_init(smem_u32(&low_full[s]), FEW ? 4 : 1);  // FEW: the adapter warps and the epilogue's
-      mbar_init(smem_u32(&low_empty[s]), FEW ? 4 : 1);
+      mbar_init(smem_u32(&low_full[s]), 1);
+      mbar_init(smem_u32(&low_empty[s]), 1);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(smem_u32(&acc_full[i]), 1);
@@ -585,14 +582,10 @@ __global__ void __launch_bounds__(kThreads, Tile<BN>::kCtas)
           mma_commit(smem_u32(&empty[ring.s]));
           ring.next();
         }
-        if (!alive) break;
-        int low_stages_due = 0;
-        if constexpr (!FEW) {
-          if (!mbar_wait(smem_u32(&count_full[counted.s]), counted.phase, abort_flag, 46)) break;
-          low_stages_due = counts[counted.s] * blocks;
-          mbar_arrive(smem_u32(&count_empty[counted.s]));
-          counted.next();
-        }
+        if (!alive || !mbar_wait(smem_u32(&count_full[counted.s]), counted.phase, abort_flag, 46)) break;
+        const int low_stages_due = counts[counted.s] * blocks;
+        mbar_arrive(smem_u32(&count_empty[counted.s]));
+        counted.next();
         for (int i = 0; i < low_stages_due; ++i) {
           if (!mbar_wait(smem_u32(&low_full[low_ring.s]), low_ring.phase, abort_flag, 47)) {
             alive = false;
@@ -622,44 +615,6 @@ __global__ void __launch_bounds__(kThreads, Tile<BN>::kCtas)
     // ---------------------------- adapter producers --------------------------
     // The low-rank rows are the previous kernel's, which may still run; every CTA waits for its end.
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    if constexpr (FEW) {
-      const int planes = kF16 ? 2 : 1;
-      for (int it = 0; it < my_tiles; ++it) {
-        const TileAt t = tile_at(blockIdx.x + (int64_t)it * gridDim.x, row_tiles, col_tiles, BN);
-        const bool ok = mbar_wait(smem_u32(low_empty), (uint32_t)(it & 1) ^ 1, abort_flag, 59);
-        if (!__all_sync(0xffffffffu, ok)) break;
-#pragma unroll 4
-        for (int row = warp - 2; row < (int)a.rows; row += 4) {
-          const int adapter = row_adapter(a, row);
-#pragma unroll
-          for (int h = 0; h < BN; h += 32) {
-            float sum = 0.f;
-            if (adapter >= 0) {
-              const int col = min(t.col0 + h + lane, a.n - 1);  // columns past n are not stored
-              const __nv_bfloat16* up = reinterpret_cast<const __nv_bfloat16*>(a.up) +
-                                        ((int64_t)adapter * a.n + col) * planes * a.rank;
-              for (int j = 0; j < a.rank; j += 8) {
-                const float4 l0 = low_values(a, parts, row, j), l1 = low_values(a, parts, row, j + 4);
-                const float l[8] = {l0.x, l0.y, l0.z, l0.w, l1.x, l1.y, l1.z, l1.w};
-                float u[8];
-                widen<__nv_bfloat16>(u, __ldg(reinterpret_cast<const uint4*>(up + j)));
-                if constexpr (kF16) {
-                  float rest[8];
-                  widen<__nv_bfloat16>(rest, __ldg(reinterpret_cast<const uint4*>(up + a.rank + j)));
-#pragma unroll
-                  for (int e = 0; e < 8; ++e) u[e] += rest[e];
-                }
-#pragma unroll
-                for (int e = 0; e < 8; ++e) sum = fmaf(l[e], u[e], sum);
-              }
-            }
-            sums[row * (BN + 1) + h + lane] = sum;
-          }
-        }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(low_full));
-      }
-    } else {
     const int r = threadIdx.x - 64;
     const bool leader = r == 0;
     Ring<SL> ring;
@@ -727,7 +682,6 @@ __global__ void __launch_bounds__(kThreads, Tile<BN>::kCtas)
     if (leader && *reinterpret_cast<volatile int*>(abort_flag))
       for (int g = max(0, issued - SL); g < issued; ++g)
         mbar_wait(smem_u32(&low_full[g % SL]), (uint32_t)(g / SL) & 1, abort_flag, 51, false);
-    }
     __syncwarp();
   } else {
     // -------------------------------- epilogue -------------------------------
@@ -743,10 +697,6 @@ __global__ void __launch_bounds__(kThreads, Tile<BN>::kCtas)
       __syncwarp();
       const bool ok = mbar_wait(smem_u32(&acc_full[acc]), (uint32_t)(it >> 1) & 1, abort_flag, 52);
       if (!__all_sync(0xffffffffu, ok)) break;
-      if constexpr (FEW) {
-        const bool summed = mbar_wait(smem_u32(low_full), (uint32_t)it & 1, abort_flag, 60);
-        if (!__all_sync(0xffffffffu, summed)) break;
-      }
       fence_after();
       const uint32_t src = tmem + acc * BN + ((uint32_t)quarter << 21);
       const int64_t row0 = t.row0 + quarter * 32;
@@ -758,10 +708,6 @@ __global__ void __launch_bounds__(kThreads, Tile<BN>::kCtas)
         for (int h = 0; h < C::kColumns; h += 32) {
           float v[32];
           tmem_ld32(src + c0 + h, v);
-          if constexpr (FEW) {
-#pragma unroll
-            for (int c = 0; c < 32; ++c) v[c] += sums[(quarter * 32 + lane) * (BN + 1) + c0 + h + c];
-          }
           uint4* line = reinterpret_cast<uint4*>(stage_rows + lane * C::kColumns * 2);
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
@@ -799,16 +745,246 @@ __global__ void __launch_bounds__(kThreads, Tile<BN>::kCtas)
       }
       fence_before();
       __syncwarp();
-      if (lane == 0) {
-        mbar_arrive(smem_u32(&acc_empty[acc]));
-        if constexpr (FEW) mbar_arrive(smem_u32(low_empty));
-      }
+      if (lane == 0) mbar_arrive(smem_u32(&acc_empty[acc]));
     }
   }
   __syncthreads();
   if (warp == 1) {
     fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(C::kTmem) : "memory");
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Up to 128 rows: out^T tiles of 128 of W's rows, bound by streaming W.
+//
+// The MMA's A operand is a W tile, its B operand the requests' rows (16 to 128
+// columns), so a stage is 16 KB of W and 2 to 16 KB of x, and two CTAs an SM
+// keep some 150 KB of W on its way.  A cluster of up to 8 CTAs splits the
+// channels of a tile; each then sums its share of the rows over the cluster's
+// shared memories.  Before that, while W streams, warps 2-5 take the dot
+// products of the share's low-rank rows with up (a thread per W row, 16
+// requests' loads at a time).
+// ---------------------------------------------------------------------------
+constexpr int kFewThreads = 192;
+constexpr int kFewRanks = 64;  // ranks of 16 requests staged at a time
+
+struct FewMaps {
+  CUtensorMap x, weight;
+};
+
+struct FewPlan {
+  int parts;    // of the low-rank rows
+  int columns;  // rows rounded up to 16
+  int stages;
+  int split;    // CTAs of a cluster
+  int share;    // rows a CTA of the cluster writes
+};
+
+__device__ __forceinline__ void cluster_barrier() {
+  asm volatile("barrier.cluster.arrive.release;\n barrier.cluster.wait.acquire;" ::: "memory");
+}
+
+// The adapters' share of rows [t0, t0 + N) in one column, into sums[t - t0][128].
+template <bool F16, int N>
+__device__ __forceinline__ void few_dots(const nnb_project_args& a, int parts, int t0, int end, int col, int r,
+                                         float* values, volatile int* adapters, float* sums) {
+  constexpr int kPlanes = F16 ? 2 : 1;
+  float acc[N] = {};
+  for (int j0 = 0; j0 < a.rank; j0 += kFewRanks) {
+    const int fours = min(kFewRanks, a.rank - j0) / 4;
+    adapter_barrier(true);  // the values of the block before have been read
+    if (r < N) adapters[r] = t0 + r < end ? row_adapter(a, t0 + r) : -1;
+    for (int i = r; i < N * fours; i += 128) {
+      const int t = i / fours, j = (i - t * fours) * 4;
+      const bool some = t0 + t < end && row_adapter(a, t0 + t) >= 0;
+      *reinterpret_cast<float4*>(values + t * kFewRanks + j) =
+          some ? low_values(a, parts, t0 + t, j0 + j) : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    adapter_barrier(true);
+    const __nv_bfloat16* up[N];
+#pragma unroll
+    for (int t = 0; t < N; ++t)  // a row without adapter multiplies zeros
+      up[t] = reinterpret_cast<const __nv_bfloat16*>(a.up) +
+              ((int64_t)max(adapters[t], 0) * a.n + col) * kPlanes * a.rank + j0;
+    for (int j = 0; j < fours * 4; j += 8) {
+      uint4 raw[N], rest[F16 ? N : 1];
+#pragma unroll
+      for (int t = 0; t < N; ++t) {
+        raw[t] = __ldg(reinterpret_cast<const uint4*>(up[t] + j));
+        if constexpr (F16) rest[t] = __ldg(reinterpret_cast<const uint4*>(up[t] + a.rank + j));
+      }
+#pragma unroll
+      for (int t = 0; t < N; ++t) {
+        float u[8];
+        widen<__nv_bfloat16>(u, raw[t]);
+        if constexpr (F16) {
+          float more[8];
+          widen<__nv_bfloat16>(more, rest[t]);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) u[e] += more[e];
+        }
+        const float4 l0 = *reinterpret_cast<const float4*>(values + t * kFewRanks + j);
+        const float4 l1 = *reinterpret_cast<const float4*>(values + t * kFewRanks + j + 4);
+        acc[t] = fmaf(l0.x, u[0], acc[t]), acc[t] = fmaf(l0.y, u[1], acc[t]);
+        acc[t] = fmaf(l0.z, u[2], acc[t]), acc[t] = fmaf(l0.w, u[3], acc[t]);
+        acc[t] = fmaf(l1.x, u[4], acc[t]), acc[t] = fmaf(l1.y, u[5], acc[t]);
+        acc[t] = fmaf(l1.z, u[6], acc[t]), acc[t] = fmaf(l1.w, u[7], acc[t]);
+      }
+    }
+  }
+#pragma unroll
+  for (int t = 0; t < N; ++t)
+    if (t0 + t < end) sums[t * BM + r] = acc[t];
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kFewThreads, 2)
+    project_few_kernel(const nnb_project_args a, const __grid_constant__ FewMaps maps, const FewPlan plan) {
+  constexpr bool kF16 = !std::is_same<T, __nv_bfloat16>::value;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* stages = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const int S = plan.stages, stage = BM * 128 + plan.columns * 128;
+  float* partial = reinterpret_cast<float*>(stages);  // [rows][128] after the MMAs, over the stages
+  float* sums = reinterpret_cast<float*>(stages + S * stage);  // [share][128]
+  float* values = sums + plan.share * BM;                      // [16][kFewRanks]
+  uint64_t* full = reinterpret_cast<uint64_t*>(values + 16 * kFewRanks);
+  uint64_t* empty = full + S;
+  uint64_t* acc_full = empty + S;
+  uint64_t* drain = acc_full + 1;
+  volatile int* adapters = reinterpret_cast<volatile int*>(drain + 1);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(const_cast<int*>(adapters + 16));
+  int* abort_flag = reinterpret_cast<int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int part = blockIdx.x % plan.split, n0 = blockIdx.x / plan.split * BM;  // part: the rank in the cluster
+  const int chunks = (a.k + 63) / 64;
+  const int first = chunks * part / plan.split, last = chunks * (part + 1) / plan.split;
+  const uint32_t tmem_columns = plan.columns <= 32 ? 32 : plan.columns <= 64 ? 64 : 128;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < S; ++s) {
+      mbar_init(smem_u32(&full[s]), 1);
+      mbar_init(smem_u32(&empty[s]), 1);
+    }
+    mbar_init(smem_u32(acc_full), 1);
+    mbar_init(smem_u32(drain), 1);
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                 "r"(tmem_columns)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  fence_before();
+  __syncthreads();
+  fence_after();
+  const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(tmem_slot);
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int s = 0, issued = 0;
+      uint32_t phase = 0;
+      for (int c = first; c < last; ++c) {
+        if (!mbar_wait(smem_u32(&empty[s]), phase ^ 1, abort_flag, 59)) break;
+        const uint32_t bar = smem_u32(&full[s]), at = smem_u32(stages + s * stage);
+        mbar_arrive_expect_tx(bar, stage);
+        tma_load_2d(at, &maps.weight, c * 64, n0, bar);
+        tma_load_2d(at + BM * 128, &maps.x, c * 64, 0, bar);
+        if (++s == S) s = 0, phase ^= 1u;
+        ++issued;
+      }
+      if (*reinterpret_cast<volatile int*>(abort_flag))
+        for (int g = max(0, issued - S); g < issued; ++g)
+          mbar_wait(smem_u32(&full[g % S]), (uint32_t)(g / S) & 1, abort_flag, 60, false);
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    if (lane == 0) {
+      const uint32_t idesc = kF16 ? idesc_f16(BM, plan.columns) : idesc_bf16(BM, plan.columns);
+      int s = 0;
+      uint32_t phase = 0, accumulate = 0;
+      bool alive = true;
+      for (int c = first; c < last; ++c) {
+        if (!mbar_wait(smem_u32(&full[s]), phase, abort_flag, 61)) {
+          alive = false;
+          break;
+        }
+        fence_after();
+        const uint32_t at = smem_u32(stages + s * stage);
+        const uint64_t ad = sw128_desc(at), bd = sw128_desc(at + BM * 128);
+        const int steps = min(4, (a.k - c * 64 + 15) / 16);
+        for (int k = 0; k < steps; ++k) {
+          mma_f16(tmem, ad + k * 2, bd + k * 2, idesc, accumulate);
+          accumulate = 1;
+        }
+        mma_commit(smem_u32(&empty[s]));
+        if (++s == S) s = 0, phase ^= 1u;
+      }
+      if (alive) mma_commit(smem_u32(acc_full));
+      if (*reinterpret_cast<volatile int*>(abort_flag)) {
+        mma_commit(smem_u32(drain));
+        mbar_wait(smem_u32(drain), 0, abort_flag, 62, false);
+      }
+    }
+    __syncwarp();
+  }
+  const int r = threadIdx.x - 64, col = n0 + r;
+  const int begin = part * plan.share, end = min((int)a.rows, begin + plan.share);
+  if (warp >= 2) {
+    // the low-rank rows are the previous kernel's, which may still run; every CTA waits for its end
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    for (int t = begin; t < end; t += 16) {
+      float* to = sums + (t - begin) * BM;
+      if (end - t <= 4)
+        few_dots<kF16, 4>(a, plan.parts, t, end, min(col, a.n - 1), r, values, adapters, to);
+      else
+        few_dots<kF16, 16>(a, plan.parts, t, end, min(col, a.n - 1), r, values, adapters, to);
+    }
+    const bool ok = mbar_wait(smem_u32(acc_full), 0, abort_flag, 63);
+    if (__all_sync(0xffffffffu, ok)) {
+      fence_after();
+      const int quarter = warp & 3;
+      for (int t = 0; t < (int)a.rows; t += 16) {
+        float v[16];
+        tmem_ld16(tmem + ((uint32_t)quarter << 21) + t, v);
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (t + i < (int)a.rows) partial[(t + i) * BM + quarter * 32 + lane] = v[i];
+      }
+      fence_before();
+    }
+  }
+  cluster_barrier();
+  if (warp >= 2 && col < a.n && *reinterpret_cast<volatile int*>(abort_flag) == 0) {
+    const float b = a.bias != nullptr ? __ldg(a.bias + col) : 0.f;
+    uint32_t peer[8];
+#pragma unroll
+    for (int c = 0; c < 8; ++c)
+      asm("mapa.shared::cluster.u32 %0, %1, %2;"
+          : "=r"(peer[c])
+          : "r"(smem_u32(partial) + r * 4), "r"(c < plan.split ? c : 0));
+#pragma unroll 2
+    for (int t = begin; t < end; ++t) {
+      float v[8];
+#pragma unroll
+      for (int c = 0; c < 8; ++c) {
+        v[c] = 0.f;
+        if (c < plan.split)
+          asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v[c]) : "r"(peer[c] + t * BM * 4) : "memory");
+      }
+      float sum = sums[(t - begin) * BM + r] + b;
+#pragma unroll
+      for (int c = 0; c < 8; ++c) sum += v[c];
+      reinterpret_cast<T*>(a.out)[t * a.out_stride + col] = T(sum);
+    }
+  }
+  cluster_barrier();  // a CTA's shared memory stays until its peers have read it
+  __syncwarp();
+  if (warp == 1) {
+    fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(tmem_columns) : "memory");
   }
 }
 
@@ -877,10 +1053,38 @@ int64_t low_bytes(const nnb_project_args& a) {
   return narrow(a) ? 0 : low_plan(a).parts * a.rows * a.rank * (int64_t)sizeof(float);
 }
 
-int encode_rows(CUtensorMap* map, bool f16, const nnb_project_args& a) {
+// A GEMM kernel's launch while the low-rank kernel before it still runs: only the warps that read its rows wait
+// for its end (griddepcontrol).
+template <typename... P, typename... V>
+int launch_early(void (*kernel)(P...), int grid, int threads, int smem, int cluster, cudaStream_t stream, V... args) {
+  cudaLaunchAttribute attributes[2];
+  attributes[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attributes[0].val.programmaticStreamSerializationAllowed = 1;
+  attributes[1].id = cudaLaunchAttributeClusterDimension;
+  attributes[1].val.clusterDim.x = cluster;
+  attributes[1].val.clusterDim.y = attributes[1].val.clusterDim.z = 1;
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3(grid);
+  config.blockDim = dim3(threads);
+  config.dynamicSmemBytes = smem;
+  config.stream = stream;
+  config.attrs = attributes;
+  config.numAttrs = 2;
+  NNB_CUDA_CHECK(cudaLaunchKernelEx(&config, kernel, args...));
+  return NNB_OK;
+}
+
+int encode_weight(CUtensorMap* map, bool f16, const nnb_project_args& a, int box_rows) {
+  const cuuint64_t dims[2] = {(cuuint64_t)a.k, (cuuint64_t)a.n};
+  const cuuint64_t strides[1] = {(cuuint64_t)a.weight_stride * 2};
+  const cuuint32_t box[2] = {64, (cuuint32_t)box_rows};
+  return encode(map, f16, 2, a.weight, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+int encode_rows(CUtensorMap* map, bool f16, const nnb_project_args& a, int box_rows) {
   const cuuint64_t dims[2] = {(cuuint64_t)a.k, (cuuint64_t)a.rows};
   const cuuint64_t strides[1] = {(cuuint64_t)(a.rows == 1 ? (a.k + 7) / 8 * 8 : a.x_stride) * 2};
-  const cuuint32_t box[2] = {64, BM};
+  const cuuint32_t box[2] = {64, (cuuint32_t)box_rows};
   return encode(map, f16, 2, a.x, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
@@ -899,7 +1103,7 @@ int launch_low(const nnb_project_args& a, const LowPlan& plan, int dev, cudaStre
     if (dev < 64) configured[dev] = true;
   }
   LowMaps maps;
-  if (const int rc = encode_rows(&maps.x, kF16, a)) return rc;
+  if (const int rc = encode_rows(&maps.x, kF16, a, BM)) return rc;
   const cuuint64_t dims[3] = {(cuuint64_t)a.k, (cuuint64_t)a.rank, (cuuint64_t)a.adapters};
   const cuuint64_t strides[2] = {(cuuint64_t)a.weight_stride * 2, (cuuint64_t)a.weight_stride * 2 * a.rank};
   const cuuint32_t box[3] = {64, (cuuint32_t)std::min(a.rank, kLowColumns), 1};
@@ -910,26 +1114,48 @@ int launch_low(const nnb_project_args& a, const LowPlan& plan, int dev, cudaStre
   return NNB_OK;
 }
 
-template <typename T, int BN, bool FEW>
+template <typename T>
+int launch_few(const nnb_project_args& a, const LowPlan& low, int sms, int dev, cudaStream_t stream) {
+  constexpr bool kF16 = !std::is_same<T, __nv_bfloat16>::value;
+  const int tiles = (a.n + BM - 1) / BM, chunks = (a.k + 63) / 64;
+  FewPlan plan;
+  plan.parts = low.parts;
+  plan.columns = ((int)a.rows + 15) / 16 * 16;
+  plan.split = 1;  // as many parts of the channels as leave two CTAs an SM
+  while (plan.split < 8 && plan.split * 2 <= chunks && tiles * plan.split * 2 <= 2 * sms) plan.split *= 2;
+  plan.share = ((int)a.rows + plan.split - 1) / plan.split;
+  const int stage = BM * 128 + plan.columns * 128;
+  const int fixed = 1024 + plan.share * BM * 4 + 16 * kFewRanks * 4 + 512;
+  // stages for two CTAs an SM, but room for the partial sums ([rows][128] floats over the stages) and at least two
+  plan.stages = std::max(2, std::min({8, (112 * 1024 - fixed) / stage, (chunks + plan.split - 1) / plan.split}));
+  while (plan.stages * stage < (int)a.rows * BM * 4) ++plan.stages;
+  const int smem = fixed + plan.stages * stage;
+  NNB_REQUIRE(smem <= kMaxSmem, "project: internal: plan exceeds shared memory (%d bytes)", smem);
+  static bool configured[64] = {false};
+  if (dev >= 64 || !configured[dev]) {
+    NNB_CUDA_CHECK(cudaFuncSetAttribute(project_few_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem));
+    if (dev < 64) configured[dev] = true;
+  }
+  FewMaps maps;
+  if (const int rc = encode_rows(&maps.x, kF16, a, plan.columns)) return rc;
+  if (const int rc = encode_weight(&maps.weight, kF16, a, BM)) return rc;
+  return launch_early(project_few_kernel<T>, tiles * plan.split, kFewThreads, smem, plan.split, stream, a, maps, plan);
+}
+
+template <typename T, int BN>
 int launch_tiles(const nnb_project_args& a, const LowPlan& plan, int sms, int dev, cudaStream_t stream) {
   using C = Tile<BN>;
   constexpr bool kF16 = !std::is_same<T, __nv_bfloat16>::value;
   static bool configured[64] = {false};
   if (dev >= 64 || !configured[dev]) {
     NNB_CUDA_CHECK(
-        cudaFuncSetAttribute(project_kernel<T, BN, FEW>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
+        cudaFuncSetAttribute(project_kernel<T, BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
     if (dev < 64) configured[dev] = true;
   }
   static_assert(C::kSmem * C::kCtas <= kMaxSmem + 1024 * (C::kCtas - 1), "the tile's stages exceed shared memory");
   Maps maps;
-  if (const int rc = encode_rows(&maps.x, kF16, a)) return rc;
-  {
-    const cuuint64_t dims[2] = {(cuuint64_t)a.k, (cuuint64_t)a.n};
-    const cuuint64_t strides[1] = {(cuuint64_t)a.weight_stride * 2};
-    const cuuint32_t box[2] = {64, BN};
-    if (const int rc = encode(&maps.weight, kF16, 2, a.weight, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B))
-      return rc;
-  }
+  if (const int rc = encode_rows(&maps.x, kF16, a, BM)) return rc;
+  if (const int rc = encode_weight(&maps.weight, kF16, a, BN)) return rc;
   {
     const cuuint64_t width = (cuuint64_t)a.rank * (kF16 ? 2 : 1);
     const cuuint64_t dims[3] = {width, (cuuint64_t)a.n, (cuuint64_t)a.adapters};
@@ -939,19 +1165,7 @@ int launch_tiles(const nnb_project_args& a, const LowPlan& plan, int sms, int de
   }
   const int64_t tiles = (a.rows + BM - 1) / BM * ((a.n + BN - 1) / BN);
   const int grid = (int)std::min<int64_t>(tiles, (int64_t)sms * C::kCtas);
-  // launched while the low-rank kernel still runs: only the adapter warps wait for it (griddepcontrol)
-  cudaLaunchAttribute early[1];
-  early[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  early[0].val.programmaticStreamSerializationAllowed = 1;
-  cudaLaunchConfig_t config = {};
-  config.gridDim = dim3(grid);
-  config.blockDim = dim3(kThreads);
-  config.dynamicSmemBytes = C::kSmem;
-  config.stream = stream;
-  config.attrs = early;
-  config.numAttrs = 1;
-  NNB_CUDA_CHECK(cudaLaunchKernelEx(&config, project_kernel<T, BN, FEW>, a, maps, plan.parts));
-  return NNB_OK;
+  return launch_early(project_kernel<T, BN>, grid, kThreads, C::kSmem, 1, stream, a, maps, plan.parts);
 }
 
 // Tile width: the one whose waves of tiles take least, a tile's time being the larger of its MMAs' and its
@@ -1206,14 +1420,12 @@ int launch_project(nnb_project_args a, cudaStream_t stream) {
   }
   const LowPlan plan = low_plan(a);
   if (const int rc = launch_low<T>(a, plan, dev, stream)) return rc;
-  if (plan.few)
-    return (a.n + 31) / 32 <= 2 * sms ? launch_tiles<T, 32, true>(a, plan, sms, dev, stream)
-                                      : launch_tiles<T, 64, true>(a, plan, sms, dev, stream);
+  if (plan.few) return launch_few<T>(a, plan, sms, dev, stream);
   switch (tile_columns(a, sms)) {
-    case 32: return launch_tiles<T, 32, false>(a, plan, sms, dev, stream);
-    case 64: return launch_tiles<T, 64, false>(a, plan, sms, dev, stream);
-    case 128: return launch_tiles<T, 128, false>(a, plan, sms, dev, stream);
-    default: return launch_tiles<T, 256, false>(a, plan, sms, dev, stream);
+    case 32: return launch_tiles<T, 32>(a, plan, sms, dev, stream);
+    case 64: return launch_tiles<T, 64>(a, plan, sms, dev, stream);
+    case 128: return launch_tiles<T, 128>(a, plan, sms, dev, stream);
+    default: return launch_tiles<T, 256>(a, plan, sms, dev, stream);
   }
 }
 

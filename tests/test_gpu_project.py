@@ -109,6 +109,11 @@ SHAPES = [  # rows, k, n, ranks, index
     (3000, 40, 24, [5], "none"),
     (700, 4096, 16, [16, 16], "runs"),
     (260, 16, 2000, [16, 16, 2], "mixed"),
+    (100, 4096, 320, [16] * 20, "mixed"),      # up to 128 rows: clusters of every size, shares of few and many rows
+    (128, 640, 129, [144, 80], "mixed"),
+    (3, 192, 4000, [24, 256], "mixed"),
+    (128, 136, 40000, [16], "runs"),
+    (17, 520, 10001, [8, 8], "mixed"),
     (5000, 128, 128, [32, 16, 7], "runs"),     # projections of few channels: every group count of 32
     (333, 127, 97, [40, 16, 7], "mixed"),
     (1, 96, 64, [200], "one"),

@@ -1400,9 +1400,14 @@ int launch_narrow_columns(const nnb_project_args& a, int sms, int dev, cudaStrea
 template <typename T>
 int launch_project(nnb_project_args a, cudaStream_t stream) {
   a.rows_per_index = std::min(a.rows_per_index, a.rows);
-  int dev = 0, sms = 0;
+  int dev = 0;
   NNB_CUDA_CHECK(cudaGetDevice(&dev));
-  NNB_CUDA_CHECK(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
+  static int counted[64] = {0};
+  int sms = dev < 64 ? counted[dev] : 0;
+  if (sms == 0) {
+    NNB_CUDA_CHECK(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
+    if (dev < 64) counted[dev] = sms;
+  }
   if (!rows_in_place(a)) {
     uint16_t* rows = reinterpret_cast<uint16_t*>(reinterpret_cast<uint8_t*>(a.low) + low_bytes(a));
     const int64_t blocks = (a.rows * a.weight_stride + 255) / 256;

@@ -984,21 +984,25 @@ class ChannelNorm:
             raise ContractError(f"unknown channel norm {self.kind!r}: one of {', '.join(_CHANNEL_NORMS)}")
         if not 0.0 < float(self.eps) < math.inf:
             raise ContractError(f"a channel norm's eps must be positive, got {self.eps}")
+        for name, p in (("weight", self.weight), ("bias", self.bias)):
+            if p is not None:
+                _check_tensor(p, f"norm {name}")
 
     def arguments(self, channels: int, device: torch.device) -> _native.ChannelNorm:
-        for name, p in (("weight", self.weight), ("bias", self.bias)):
-            _check_channels(p, f"norm {name}", channels, device)
-        return _native.ChannelNorm(_CHANNEL_NORMS[self.kind], self.eps, _ptr(self.weight), _ptr(self.bias))
+        w = _channels_pointer(self.weight, "norm weight", channels, device)
+        b = _channels_pointer(self.bias, "norm bias", channels, device)
+        return _native.ChannelNorm(_CHANNEL_NORMS[self.kind], self.eps, w, b)
 
 
-def _check_channels(p: torch.Tensor | None, name: str, channels: int, device: torch.device) -> None:
-    """A per-channel float32 parameter, or none."""
+def _channels_pointer(p: torch.Tensor | None, name: str, channels: int, device: torch.device) -> int:
+    """The address of a per-channel float32 parameter, or 0 for none."""
     if p is None:
-        return
+        return 0
     _check_tensor(p, name)
     if p.shape != (channels,) or p.device != device:
         raise ContractError(f"{name} must hold {channels} values on {device}, "
                             f"got {tuple(p.shape)} on {p.device}")
+    return p.data_ptr()
 
 
 def _check_rows(t: torch.Tensor, name: str) -> None:
@@ -1022,6 +1026,11 @@ def _row_stride(t: torch.Tensor, name: str) -> int:
             return axes[-1][1] if axes else channels
     raise ContractError(f"the rows of {name} must be evenly spaced with contiguous channels, "
                         f"got shape {tuple(t.shape)} with strides {t.stride()}")
+
+
+def _empty_rows(like: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
+    """A contiguous tensor of ``like``'s shape (``empty_like`` is the quickest way to one, where it keeps that)."""
+    return torch.empty_like(like, dtype=dtype) if like.is_contiguous() else like.new_empty(like.shape, dtype=dtype)
 
 
 def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
@@ -1048,12 +1057,19 @@ def _check_out(out: torch.Tensor, name: str, shape, dtype: torch.dtype, device: 
 
 
 def _call_rows(function, args, device: torch.device, what: str) -> None:
-    """A row operator's launch, on ``device``'s current stream."""
-    if device.index == torch.cuda.current_device():
-        _native.check(function(ctypes.byref(args), _stream()), what)
+    """A row operator's launch, on ``device``'s current stream.
+
+    The stream is asked for as a plain handle: the Stream object that
+    ``torch.cuda.current_stream`` builds costs as much host time as a launch.
+    """
+    index = device.index
+    if index == torch.cuda.current_device():
+        status = function(ctypes.byref(args), torch._C._cuda_getCurrentRawStream(index))
     else:
         with torch.cuda.device(device):
-            _native.check(function(ctypes.byref(args), _stream()), what)
+            status = function(ctypes.byref(args), torch._C._cuda_getCurrentRawStream(index))
+    if status != 0:
+        _native.check(status, what)
 
 
 def channel_norm(x: torch.Tensor, norm: ChannelNorm, *, out_dtype: torch.dtype | None = None,
@@ -1074,7 +1090,7 @@ def channel_norm(x: torch.Tensor, norm: ChannelNorm, *, out_dtype: torch.dtype |
     x_stride = _row_stride(x, "x")
     n = norm.arguments(channels, device)
     if out is None:
-        out, out_stride = torch.empty(shape, dtype=dtype, device=device), channels
+        out, out_stride = _empty_rows(x, dtype), channels
     else:
         out_stride = _check_out(out, "out", shape, dtype, device)
         same = out.data_ptr() == x.data_ptr() and out_stride == x_stride and dtype == x.dtype
@@ -1086,7 +1102,9 @@ def channel_norm(x: torch.Tensor, norm: ChannelNorm, *, out_dtype: torch.dtype |
         return out
     args = _native.NormArgs(x.data_ptr(), out.data_ptr(), rows, x_stride, out_stride, channels,
                             _ROW_TYPES[x.dtype], _ROW_TYPES[dtype], 0, n)
-    token = PROFILE.start("channel_norm", 0.0, float(rows * channels * (x.element_size() + out.element_size())))
+    token = None
+    if PROFILE.active:
+        token = PROFILE.start("channel_norm", 0.0, float(rows * channels * (x.element_size() + out.element_size())))
     _call_rows(_native.load().nnb_channel_norm_rows, args, device, "channel_norm")
     PROFILE.stop(token)
     return out
@@ -1126,8 +1144,8 @@ def gated_residual_join(branch: torch.Tensor, skip: torch.Tensor, *, post: Chann
     if gate_act not in _GATE_ACTS:
         raise ContractError(f"unknown gate activation {gate_act!r}: one of {', '.join(_GATE_ACTS)}")
     channels = shape[-1]
-    _check_channels(scale, "scale", channels, device)
-    rows = math.prod(shape[:-1])
+    scale_pointer = _channels_pointer(scale, "scale", channels, device)
+    rows = branch.numel() // channels
     mode, gate_stride, per_sample = 0, 0, 0
     if gate is not None:
         _check_rows(gate, "gate")
@@ -1147,7 +1165,7 @@ def gated_residual_join(branch: torch.Tensor, skip: torch.Tensor, *, post: Chann
     post_args = _NO_NORM if post is None else post.arguments(channels, device)
     next_args = _NO_NORM if next_norm is None else next_norm.arguments(channels, device)
     if out is None:
-        out, out_stride = torch.empty(shape, dtype=skip.dtype, device=device), channels
+        out, out_stride = _empty_rows(skip, skip.dtype), channels
     else:
         out_stride = _check_out(out, "out", shape, skip.dtype, device)
         same = out.data_ptr() == skip.data_ptr() and out_stride == skip_stride
@@ -1162,16 +1180,18 @@ def gated_residual_join(branch: torch.Tensor, skip: torch.Tensor, *, post: Chann
         dtype = next_dtype or branch.dtype
         if dtype not in _ROW_TYPES:
             raise ContractError(f"next_dtype must be float32, bfloat16 or float16, got {dtype}")
-        normed, normed_type = torch.empty(shape, dtype=dtype, device=device), _ROW_TYPES[dtype]
+        normed, normed_type = _empty_rows(branch, dtype), _ROW_TYPES[dtype]
     if rows == 0:
         return out, normed
     args = _native.JoinArgs(branch.data_ptr(), skip.data_ptr(), _ptr(gate), out.data_ptr(), _ptr(normed), rows,
                             branch_stride, skip_stride, gate_stride, out_stride, channels, per_sample, channels,
                             _ROW_TYPES[branch.dtype], _ROW_TYPES[skip.dtype], normed_type, mode,
-                            _GATE_ACTS[gate_act], residual_scale, 0, _ptr(scale), post_args, next_args)
-    nbytes = (branch.element_size() + 2 * skip.element_size() + (0 if normed is None else normed.element_size())
-              + (gate.element_size() if mode == 1 else 0))
-    token = PROFILE.start("gated_residual_join", 0.0, float(nbytes) * rows * channels)
+                            _GATE_ACTS[gate_act], residual_scale, 0, scale_pointer, post_args, next_args)
+    token = None
+    if PROFILE.active:
+        nbytes = (branch.element_size() + 2 * skip.element_size() + (0 if normed is None else normed.element_size())
+                  + (gate.element_size() if mode == 1 else 0))
+        token = PROFILE.start("gated_residual_join", 0.0, float(nbytes) * rows * channels)
     _call_rows(_native.load().nnb_gated_join, args, device, "gated_residual_join")
     PROFILE.stop(token)
     return out, normed
@@ -1233,7 +1253,7 @@ def pack_projection(weight: torch.Tensor, adapters: list[Adapter],
         raise ContractError("an adapted projection needs at least one adapter")
     n, k = (int(v) for v in weight.shape)
     device, dtype = weight.device, weight.dtype
-    _check_channels(bias, "projection bias", n, device)
+    _channels_pointer(bias, "projection bias", n, device)
     for i, a in enumerate(adapters):
         if a.down.shape[1] != k or a.up.shape != (n, a.down.shape[0]):
             raise ContractError(f"adapter {i}: down {tuple(a.down.shape)} and up {tuple(a.up.shape)} do not fit a "
@@ -1292,32 +1312,36 @@ def adapted_projection(x: torch.Tensor, projection: AdaptedProjection, index: to
             or not 1 <= axes < len(shape) or index.shape != shape[:axes]:
         raise ContractError(f"index must be a contiguous int32 tensor over leading axes of {tuple(shape)} on {device}, "
                             f"got {tuple(index.shape)} {index.dtype} on {index.device}")
-    n, rank = int(weight.shape[0]), int(projection.down.shape[1])
+    down = projection.down
+    (n, weight_stride), (adapters, rank, _) = weight.shape, down.shape
     x_stride = _row_stride(x, "x")
     if out is None:
-        out, out_stride = torch.empty((*shape[:-1], n), dtype=x.dtype, device=device), n
+        out, out_stride = x.new_empty((*shape[:-1], n)), n
     else:
         out_stride = _check_out(out, "out", (*shape[:-1], n), x.dtype, device)
-        for name, t in (("x", x), ("index", index), ("the projection", weight), ("the projection", projection.down),
+        for name, t in (("x", x), ("index", index), ("the projection", weight), ("the projection", down),
                         ("the projection", projection.up), ("the projection", projection.bias)):
             if t is not None and _overlap(out, t):
                 raise ContractError(f"out overlaps {name}")
     rows = out.numel() // n
     if rows == 0:
         return out
-    args = _native.ProjectArgs(x.data_ptr(), weight.data_ptr(), projection.down.data_ptr(),
-                               projection.up.data_ptr(), projection.scales.data_ptr(), _ptr(projection.bias),
-                               index.data_ptr(), out.data_ptr(), 0, rows, x_stride, out_stride,
-                               math.prod(shape[axes:-1]), weight.shape[1], shape[-1], n, projection.down.shape[0],
-                               rank, _ROW_TYPES[x.dtype], 0)
-    nbytes = int(_native.load().nnb_project_workspace_bytes(ctypes.byref(args)))
+    lib = _native.load()
+    args = _native.ProjectArgs(x.data_ptr(), weight.data_ptr(), down.data_ptr(), projection.up.data_ptr(),
+                               projection.scales.data_ptr(), _ptr(projection.bias), index.data_ptr(), out.data_ptr(),
+                               0, rows, x_stride, out_stride, rows // index.numel(), weight_stride, shape[-1], n,
+                               adapters, rank, _ROW_TYPES[x.dtype], 0)
+    nbytes = lib.nnb_project_workspace_bytes(ctypes.byref(args))
     if nbytes < 0:
         _native.check(nbytes, "adapted_projection")
     if nbytes > 0:
-        workspace = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        workspace = x.new_empty(nbytes, dtype=torch.uint8)
         args.low = workspace.data_ptr()
-    token = PROFILE.start("adapted_projection", 2.0 * rows * (n * shape[-1] + rank * (n + shape[-1])),
-                          2.0 * (rows * (n + shape[-1]) + n * shape[-1]), launches=2)
-    _call_rows(_native.load().nnb_project, args, device, "adapted_projection")
+    token = None
+    if PROFILE.active:
+        k = shape[-1]
+        token = PROFILE.start("adapted_projection", 2.0 * rows * (n * k + rank * (n + k)),
+                              2.0 * (rows * (n + k) + n * k), launches=2 if nbytes > 0 else 1)
+    _call_rows(lib.nnb_project, args, device, "adapted_projection")
     PROFILE.stop(token)
     return out

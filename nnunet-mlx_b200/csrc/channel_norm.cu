@@ -14,6 +14,12 @@
 // around the exact mean, not a difference of squares.  All values, sums and
 // statistics are float32; the only roundings to 16 bits are the stored stream
 // and the stored normed rows.
+//
+// Two things keep the loads coming while a row's sums and products are taken:
+// the next row's operands are on their way before the present one's are used
+// (up to two chunks a thread), and rows of one chunk a thread keep their
+// per-channel parameters in registers (from L1 they were more bytes than the
+// row itself, and the instructions to fetch them what bound the short rows).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -30,6 +36,15 @@ __device__ __forceinline__ float to_float(T v) {
     return v;
   else
     return (float)v;
+}
+
+__device__ __forceinline__ uint32_t pair(float a, float b, __nv_bfloat16) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ uint32_t pair(float a, float b, __half) {
+  const __half2 v = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&v);
 }
 
 template <typename T>
@@ -71,12 +86,13 @@ __device__ __forceinline__ void store_chunk(T* row, const float (&v)[8], int ch,
   if constexpr (ALIGNED) {
     const int c = channel_of<true, TPR>(ch, 0, lane);
     if (c >= channels) return;
-    Chunk<T> out;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) out.v[j] = T(v[j]);
-#pragma unroll
-    for (int i = 0; i < (int)sizeof(T) / 2; ++i)
-      reinterpret_cast<uint4*>(row + c)[i] = reinterpret_cast<const uint4*>(out.v)[i];
+    if constexpr (sizeof(T) == 4) {
+      reinterpret_cast<float4*>(row + c)[0] = make_float4(v[0], v[1], v[2], v[3]);
+      reinterpret_cast<float4*>(row + c)[1] = make_float4(v[4], v[5], v[6], v[7]);
+    } else {
+      *reinterpret_cast<uint4*>(row + c) =
+          make_uint4(pair(v[0], v[1], T()), pair(v[2], v[3], T()), pair(v[4], v[5], T()), pair(v[6], v[7], T()));
+    }
   } else {
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
@@ -120,16 +136,67 @@ __device__ __forceinline__ float row_sum(float v, float* buffers, int& turn) {
   return v;
 }
 
+// A norm's per-channel parameters, times a per-channel factor where one follows: held for all rows when a thread
+// has one chunk, else read again with each row.
 template <bool ALIGNED, int TPR, int NCH>
-__device__ __forceinline__ void normalize(float (&v)[NCH][8], const nnb_channel_norm& n, int lane, int channels,
-                                          float* buffers, int& turn) {
+struct Params {
+  static constexpr bool kHeld = NCH == 1;
+  const float* weight;
+  const float* bias;
+  const float* factor;
+  float w[8], b[8];  // held
+
+  __device__ __forceinline__ void load(float (&lw)[8], float (&lb)[8], int ch, int lane, int channels) const {
+    if (weight != nullptr) {
+      load_param<ALIGNED, TPR>(lw, weight, ch, lane, channels);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) lw[j] = 1.f;
+    }
+    if (bias != nullptr) {
+      load_param<ALIGNED, TPR>(lb, bias, ch, lane, channels);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) lb[j] = 0.f;
+    }
+    if (factor != nullptr) {
+      float f[8];
+      load_param<ALIGNED, TPR>(f, factor, ch, lane, channels);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) lw[j] *= f[j], lb[j] *= f[j];
+    }
+  }
+
+  __device__ __forceinline__ Params(const float* weight_, const float* bias_, const float* factor_, int lane,
+                                    int channels)
+      : weight(weight_), bias(bias_), factor(factor_) {
+    if constexpr (kHeld) load(w, b, 0, lane, channels);
+  }
+
+  __device__ __forceinline__ void get(float (&lw)[8], float (&lb)[8], int ch, int lane, int channels) const {
+    if constexpr (kHeld) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) lw[j] = w[j], lb[j] = b[j];
+    } else {
+      load(lw, lb, ch, lane, channels);
+    }
+  }
+};
+
+// The row's inverse deviation (layer, whose mean is taken off v) or inverse root mean square.
+template <bool ALIGNED, int TPR, int NCH>
+__device__ __forceinline__ float deviation(float (&v)[NCH][8], int kind, float eps, int lane, int channels,
+                                           float* buffers, int& turn) {
+  const float per_channel = 1.f / (float)channels;
   float sum = 0.f;
-  if (n.kind == NNB_CHANNEL_NORM_LAYER) {
+  if (kind == NNB_CHANNEL_NORM_LAYER) {
 #pragma unroll
     for (int ch = 0; ch < NCH; ++ch)
 #pragma unroll
       for (int j = 0; j < 8; ++j) sum += v[ch][j];
-    const float mean = row_sum<TPR>(sum, buffers, turn) / (float)channels;
+    sum = row_sum<TPR>(sum, buffers, turn);
+    float mean = sum * per_channel;
+    mean = fmaf(fmaf(-mean, (float)channels, sum), per_channel, mean);  // the quotient's last bits: exact for a constant row
     sum = 0.f;
 #pragma unroll
     for (int ch = 0; ch < NCH; ++ch)
@@ -144,23 +211,20 @@ __device__ __forceinline__ void normalize(float (&v)[NCH][8], const nnb_channel_
 #pragma unroll
       for (int j = 0; j < 8; ++j) sum = fmaf(v[ch][j], v[ch][j], sum);
   }
-  const float inv = 1.f / sqrtf(row_sum<TPR>(sum, buffers, turn) / (float)channels + n.eps);
+  return rsqrtf(fmaf(row_sum<TPR>(sum, buffers, turn), per_channel, eps));
+}
+
+template <bool ALIGNED, int TPR, int NCH>
+__device__ __forceinline__ void normalize(float (&v)[NCH][8], int kind, float eps,
+                                          const Params<ALIGNED, TPR, NCH>& params, int lane, int channels,
+                                          float* buffers, int& turn) {
+  const float inv = deviation<ALIGNED, TPR, NCH>(v, kind, eps, lane, channels, buffers, turn);
 #pragma unroll
   for (int ch = 0; ch < NCH; ++ch) {
-    float w[8];
-    if (n.weight != nullptr) {
-      load_param<ALIGNED, TPR>(w, n.weight, ch, lane, channels);
+    float w[8], b[8];
+    params.get(w, b, ch, lane, channels);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[ch][j] *= inv * w[j];
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[ch][j] *= inv;
-    }
-    if (n.bias != nullptr) {
-      load_param<ALIGNED, TPR>(w, n.bias, ch, lane, channels);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[ch][j] += w[j];
-    }
+    for (int j = 0; j < 8; ++j) v[ch][j] = fmaf(v[ch][j] * inv, w[j], b[j]);
   }
 }
 
@@ -178,38 +242,58 @@ __device__ __forceinline__ void store_row(void* base, int type, int64_t offset, 
   }
 }
 
-__device__ __forceinline__ float gate_value(float g, int act) {
-  // the sigmoid's exponential and quotient are within a few float32 roundings of the exact value
-  if (act == NNB_GATE_SIGMOID) return __fdividef(1.f, 1.f + __expf(-g));
-  if (act == NNB_GATE_SILU) return g * __fdividef(1.f, 1.f + __expf(-g));
-  if (act == NNB_GATE_TANH) return tanhf(g);
-  return g;
+// Multiplies f by the gate's values.  The sigmoid's exponential and quotient are within a few float32 roundings.
+__device__ __forceinline__ float sigmoid(float g) { return __fdividef(1.f, 1.f + __expf(-g)); }
+
+template <typename T, int N>
+__device__ __forceinline__ void apply_gate(float (&f)[N], const T* gate, int act) {
+  if (act == NNB_GATE_SIGMOID) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) f[j] *= sigmoid(to_float(gate[j]));
+  } else if (act == NNB_GATE_SILU) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) f[j] *= to_float(gate[j]) * sigmoid(to_float(gate[j]));
+  } else if (act == NNB_GATE_TANH) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) f[j] *= tanhf(to_float(gate[j]));
+  } else {
+#pragma unroll
+    for (int j = 0; j < N; ++j) f[j] *= to_float(gate[j]);
+  }
 }
 
-constexpr int block_threads(int tpr) { return tpr < 128 ? 128 : tpr; }
+// Rows of more than a warp have a block of their own, whose barrier their sums use.
+constexpr int block_threads(int tpr) { return tpr <= 32 ? 128 : tpr; }
 
 template <typename T, bool ALIGNED, int TPR, int NCH>
 __global__ void __launch_bounds__(block_threads(TPR)) channel_norm_kernel(const nnb_norm_args a) {
   constexpr int kRows = block_threads(TPR) / TPR;
+  constexpr bool kAhead = NCH <= 2;
   __shared__ float buffers[2 * (TPR > 32 ? TPR / 32 : 1)];
   int turn = 0;
-  const int lane = threadIdx.x % TPR;
-  for (int64_t first = (int64_t)blockIdx.x * kRows; first < a.rows; first += (int64_t)gridDim.x * kRows) {
-    const int64_t row = first + threadIdx.x / TPR;
-    const bool live = row < a.rows;  // a warp's rows past the end still take part in its shuffles
-    const T* src = reinterpret_cast<const T*>(a.x) + (live ? row : 0) * a.x_stride;
+  const int lane = threadIdx.x % TPR, channels = a.channels;
+  const Params<ALIGNED, TPR, NCH> params(a.norm.weight, a.norm.bias, nullptr, lane, channels);
+  const int64_t step = (int64_t)gridDim.x * kRows;
+  int64_t row = (int64_t)blockIdx.x * kRows + threadIdx.x / TPR;
+  Chunk<T> raw[NCH];
+  auto load = [&](int64_t at) {
+    const T* src = reinterpret_cast<const T*>(a.x) + (at < a.rows ? at : 0) * a.x_stride;
+#pragma unroll
+    for (int ch = 0; ch < NCH; ++ch) load_chunk<ALIGNED, TPR>(raw[ch], src, ch, lane, channels);
+  };
+  load(row);
+  // the block's first row decides, so that a warp's rows past the end still take part in its shuffles
+  for (; row - threadIdx.x / TPR < a.rows; row += step) {
     float v[NCH][8];
-    {
-      Chunk<T> raw[NCH];
 #pragma unroll
-      for (int ch = 0; ch < NCH; ++ch) load_chunk<ALIGNED, TPR>(raw[ch], src, ch, lane, a.channels);
+    for (int ch = 0; ch < NCH; ++ch)
 #pragma unroll
-      for (int ch = 0; ch < NCH; ++ch)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[ch][j] = to_float(raw[ch].v[j]);
-    }
-    normalize<ALIGNED, TPR, NCH>(v, a.norm, lane, a.channels, buffers, turn);
-    if (live) store_row<ALIGNED, TPR, NCH>(a.out, a.out_type, row * a.out_stride, v, lane, a.channels);
+      for (int j = 0; j < 8; ++j) v[ch][j] = to_float(raw[ch].v[j]);
+    const bool more = row - threadIdx.x / TPR + step < a.rows;
+    if (kAhead && more) load(row + step);
+    normalize<ALIGNED, TPR, NCH>(v, a.norm.kind, a.norm.eps, params, lane, channels, buffers, turn);
+    if (row < a.rows) store_row<ALIGNED, TPR, NCH>(a.out, a.out_type, row * a.out_stride, v, lane, channels);
+    if (!kAhead && more) load(row + step);
   }
 }
 
@@ -217,69 +301,87 @@ __global__ void __launch_bounds__(block_threads(TPR)) channel_norm_kernel(const 
 template <typename TS, typename TB, bool ALIGNED, int TPR, int NCH>
 __global__ void __launch_bounds__(block_threads(TPR)) gated_join_kernel(const nnb_join_args a) {
   constexpr int kRows = block_threads(TPR) / TPR;
+  constexpr bool kAhead = NCH <= 2;
   __shared__ float buffers[2 * (TPR > 32 ? TPR / 32 : 1)];
   int turn = 0;
-  const int lane = threadIdx.x % TPR;
-  const int channels = a.channels;
-  for (int64_t first = (int64_t)blockIdx.x * kRows; first < a.rows; first += (int64_t)gridDim.x * kRows) {
-    const int64_t row = first + threadIdx.x / TPR;
-    const bool live = row < a.rows;
-    const int64_t at = live ? row : 0;
-    // every operand of the row is asked for before the first is used: one trip to HBM per row
-    Chunk<TB> braw[NCH], graw[NCH];
-    Chunk<TS> sraw[NCH];
-    const TB* branch = reinterpret_cast<const TB*>(a.branch) + at * a.branch_stride;
-    const TS* skip = reinterpret_cast<const TS*>(a.skip) + at * a.skip_stride;
+  const int lane = threadIdx.x % TPR, channels = a.channels;
+  // scale times the post norm's parameters: v -> v * w + b there, or v * scale without a norm
+  const Params<ALIGNED, TPR, NCH> post(a.post.kind != NNB_CHANNEL_NORM_NONE ? a.post.weight : nullptr,
+                                       a.post.kind != NNB_CHANNEL_NORM_NONE ? a.post.bias : nullptr, a.scale, lane,
+                                       channels);
+  const Params<ALIGNED, TPR, NCH> next(a.next.kind != NNB_CHANNEL_NORM_NONE ? a.next.weight : nullptr,
+                                       a.next.kind != NNB_CHANNEL_NORM_NONE ? a.next.bias : nullptr, nullptr, lane,
+                                       channels);
+  const bool wide_gate = a.gate_mode == NNB_GATE_FULL || a.gate_mode == NNB_GATE_SAMPLE;
+  const int64_t step = (int64_t)gridDim.x * kRows;
+  int64_t row = (int64_t)blockIdx.x * kRows + threadIdx.x / TPR;
+  Chunk<TB> branch[NCH], gate[NCH];
+  Chunk<TS> skip[NCH];
+  TB row_gate = TB(0.f);
+  // every operand of a row at once: one trip to HBM per row
+  auto load = [&](int64_t row) {
+    const int64_t at = row < a.rows ? row : 0;
+    const TB* b = reinterpret_cast<const TB*>(a.branch) + at * a.branch_stride;
+    const TS* s = reinterpret_cast<const TS*>(a.skip) + at * a.skip_stride;
 #pragma unroll
-    for (int ch = 0; ch < NCH; ++ch) load_chunk<ALIGNED, TPR>(braw[ch], branch, ch, lane, channels);
+    for (int ch = 0; ch < NCH; ++ch) load_chunk<ALIGNED, TPR>(branch[ch], b, ch, lane, channels);
 #pragma unroll
-    for (int ch = 0; ch < NCH; ++ch) load_chunk<ALIGNED, TPR>(sraw[ch], skip, ch, lane, channels);
-    float row_gate = a.residual_scale;
-    if (a.gate_mode == NNB_GATE_FULL || a.gate_mode == NNB_GATE_SAMPLE) {
-      const int64_t grow = a.gate_mode == NNB_GATE_FULL ? at : at / a.rows_per_sample;
-      const TB* gate = reinterpret_cast<const TB*>(a.gate) + grow * a.gate_stride;
+    for (int ch = 0; ch < NCH; ++ch) load_chunk<ALIGNED, TPR>(skip[ch], s, ch, lane, channels);
+    if (wide_gate) {
+      int64_t at_gate = at;
+      if (a.gate_mode == NNB_GATE_SAMPLE)
+        at_gate = a.rows <= UINT32_MAX ? (uint32_t)at / (uint32_t)a.rows_per_sample : at / a.rows_per_sample;
+      const TB* g = reinterpret_cast<const TB*>(a.gate) + at_gate * a.gate_stride;
 #pragma unroll
-      for (int ch = 0; ch < NCH; ++ch) load_chunk<ALIGNED, TPR>(graw[ch], gate, ch, lane, channels);
+      for (int ch = 0; ch < NCH; ++ch) load_chunk<ALIGNED, TPR>(gate[ch], g, ch, lane, channels);
     } else if (a.gate_mode == NNB_GATE_ROW) {
-      row_gate *= gate_value(to_float(reinterpret_cast<const TB*>(a.gate)[at * a.gate_stride]), a.gate_act);
+      row_gate = reinterpret_cast<const TB*>(a.gate)[at * a.gate_stride];
     }
+  };
+  load(row);
+  for (; row - threadIdx.x / TPR < a.rows; row += step) {
     float v[NCH][8];
 #pragma unroll
     for (int ch = 0; ch < NCH; ++ch)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[ch][j] = to_float(braw[ch].v[j]);
-    if (a.post.kind != NNB_CHANNEL_NORM_NONE) normalize<ALIGNED, TPR, NCH>(v, a.post, lane, channels, buffers, turn);
+      for (int j = 0; j < 8; ++j) v[ch][j] = to_float(branch[ch].v[j]);
+    float s[NCH][8];
+    Chunk<TB> g[NCH];
 #pragma unroll
     for (int ch = 0; ch < NCH; ++ch) {
-      float f[8];
-      if (a.scale != nullptr) {
-        load_param<ALIGNED, TPR>(f, a.scale, ch, lane, channels);
+      g[ch] = gate[ch];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) f[j] *= row_gate;
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) f[j] = row_gate;
-      }
-      if (a.gate_mode == NNB_GATE_FULL || a.gate_mode == NNB_GATE_SAMPLE) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) f[j] *= gate_value(to_float(graw[ch].v[j]), a.gate_act);
-      }
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        // a channel past the row's end holds zero in both operands, but not after a norm with a bias
-        const float s = fmaf(f[j], v[ch][j], to_float(sraw[ch].v[j]));
-        v[ch][j] = channel_of<ALIGNED, TPR>(ch, j, lane) < channels ? s : 0.f;
-      }
+      for (int j = 0; j < 8; ++j) s[ch][j] = to_float(skip[ch].v[j]);
     }
-    if (live) {
+    float alpha[1] = {a.residual_scale};
+    if (a.gate_mode == NNB_GATE_ROW) apply_gate(alpha, &row_gate, a.gate_act);
+    const bool more = row - threadIdx.x / TPR + step < a.rows;
+    if (kAhead && more) load(row + step);
+    float inv = 1.f;
+    if (a.post.kind != NNB_CHANNEL_NORM_NONE)
+      inv = deviation<ALIGNED, TPR, NCH>(v, a.post.kind, a.post.eps, lane, channels, buffers, turn);
+#pragma unroll
+    for (int ch = 0; ch < NCH; ++ch) {
+      float w[8], b[8];
+      post.get(w, b, ch, lane, channels);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[ch][j] = alpha[0] * fmaf(v[ch][j] * inv, w[j], b[j]);
+      if (wide_gate) apply_gate(v[ch], g[ch].v, a.gate_act);
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        // a channel past the row's end holds zero in both operands, but not after a norm with a bias
+        v[ch][j] = channel_of<ALIGNED, TPR>(ch, j, lane) < channels ? s[ch][j] + v[ch][j] : 0.f;
+    }
+    if (row < a.rows) {
       TS* out = reinterpret_cast<TS*>(a.stream) + row * a.stream_stride;
 #pragma unroll
       for (int ch = 0; ch < NCH; ++ch) store_chunk<ALIGNED, TPR>(out, v[ch], ch, lane, channels);
     }
     if (a.next.kind != NNB_CHANNEL_NORM_NONE) {
-      normalize<ALIGNED, TPR, NCH>(v, a.next, lane, channels, buffers, turn);
-      if (live) store_row<ALIGNED, TPR, NCH>(a.normed, a.normed_type, row * a.normed_stride, v, lane, channels);
+      normalize<ALIGNED, TPR, NCH>(v, a.next.kind, a.next.eps, next, lane, channels, buffers, turn);
+      if (row < a.rows) store_row<ALIGNED, TPR, NCH>(a.normed, a.normed_type, row * a.normed_stride, v, lane, channels);
     }
+    if (!kAhead && more) load(row + step);
   }
 }
 
@@ -316,35 +418,39 @@ int launch_join(const nnb_join_args& a, cudaStream_t stream) {
                      block_threads(TPR) / TPR, a, stream);
 }
 
-// Threads per row and chunks per thread by the row's length: up to a warp per row (512 channels) the sums need
-// no barrier; beyond, the row is spread over one block so that a thread holds at most 32 channels.
-#define NNB_BY_CHANNELS(channels, CALL)  \
-  do {                                   \
-    const int chunks = ((channels) + 7) / 8; \
-    if (chunks <= 4) return CALL(4, 1);      \
-    if (chunks <= 8) return CALL(8, 1);      \
-    if (chunks <= 16) return CALL(16, 1);    \
-    if (chunks <= 32) return CALL(32, 1);    \
-    if (chunks <= 64) return CALL(32, 2);    \
-    if (chunks <= 128) return CALL(128, 1);  \
-    if (chunks <= 256) return CALL(128, 2);  \
-    if (chunks <= 512) return CALL(256, 2);  \
-    if (chunks <= 1024) return CALL(512, 2); \
-    return CALL(512, 4);                     \
-  } while (0)
-
+// Threads per row and chunks per thread by the row's length.  Up to 256 channels a warp or less has a row, and
+// its sums need no barrier.  Beyond, two chunks a thread carry more loads; a join, with its registers for three
+// operands and their successors, does better with one chunk and more threads where both fit (B200, bfloat16 rows:
+// norm of 2048 channels 128 x 2 44 us, 256 x 1 53 us; join of 512 channels 32 x 2 140 us, 64 x 1 119 us; join of
+// 4096 channels 256 x 2 146 us, 512 x 1 161 us).
 template <typename T, bool ALIGNED>
 int norm_by_channels(const nnb_norm_args& a, cudaStream_t stream) {
-#define NNB_CALL(TPR, NCH) (launch_norm<T, ALIGNED, TPR, NCH>(a, stream))
-  NNB_BY_CHANNELS(a.channels, NNB_CALL);
-#undef NNB_CALL
+  const int chunks = (a.channels + 7) / 8;
+  if (chunks <= 4) return launch_norm<T, ALIGNED, 4, 1>(a, stream);
+  if (chunks <= 8) return launch_norm<T, ALIGNED, 8, 1>(a, stream);
+  if (chunks <= 16) return launch_norm<T, ALIGNED, 16, 1>(a, stream);
+  if (chunks <= 32) return launch_norm<T, ALIGNED, 32, 1>(a, stream);
+  if (chunks <= 64) return launch_norm<T, ALIGNED, 32, 2>(a, stream);
+  if (chunks <= 128) return launch_norm<T, ALIGNED, 64, 2>(a, stream);
+  if (chunks <= 256) return launch_norm<T, ALIGNED, 128, 2>(a, stream);
+  if (chunks <= 512) return launch_norm<T, ALIGNED, 256, 2>(a, stream);
+  if (chunks <= 1024) return launch_norm<T, ALIGNED, 512, 2>(a, stream);
+  return launch_norm<T, ALIGNED, 512, 4>(a, stream);
 }
 
 template <typename TS, typename TB, bool ALIGNED>
 int join_by_channels(const nnb_join_args& a, cudaStream_t stream) {
-#define NNB_CALL(TPR, NCH) (launch_join<TS, TB, ALIGNED, TPR, NCH>(a, stream))
-  NNB_BY_CHANNELS(a.channels, NNB_CALL);
-#undef NNB_CALL
+  const int chunks = (a.channels + 7) / 8;
+  if (chunks <= 4) return launch_join<TS, TB, ALIGNED, 4, 1>(a, stream);
+  if (chunks <= 8) return launch_join<TS, TB, ALIGNED, 8, 1>(a, stream);
+  if (chunks <= 16) return launch_join<TS, TB, ALIGNED, 16, 1>(a, stream);
+  if (chunks <= 32) return launch_join<TS, TB, ALIGNED, 32, 1>(a, stream);
+  if (chunks <= 64) return launch_join<TS, TB, ALIGNED, 64, 1>(a, stream);
+  if (chunks <= 128) return launch_join<TS, TB, ALIGNED, 128, 1>(a, stream);
+  if (chunks <= 256) return launch_join<TS, TB, ALIGNED, 256, 1>(a, stream);
+  if (chunks <= 512) return launch_join<TS, TB, ALIGNED, 256, 2>(a, stream);
+  if (chunks <= 1024) return launch_join<TS, TB, ALIGNED, 512, 2>(a, stream);
+  return launch_join<TS, TB, ALIGNED, 512, 4>(a, stream);
 }
 
 int type_bytes(int type) { return type == NNB_F32 ? 4 : 2; }

@@ -268,7 +268,7 @@ constexpr int block_threads(int tpr) { return tpr <= 32 ? 128 : tpr; }
 template <typename T, bool ALIGNED, int TPR, int NCH>
 __global__ void __launch_bounds__(block_threads(TPR)) channel_norm_kernel(const nnb_norm_args a) {
   constexpr int kRows = block_threads(TPR) / TPR;
-  constexpr bool kAhead = NCH <= 2;
+  constexpr bool kAhead = NCH <= 3;
   __shared__ float buffers[2 * (TPR > 32 ? TPR / 32 : 1)];
   int turn = 0;
   const int lane = threadIdx.x % TPR, channels = a.channels;
@@ -301,7 +301,7 @@ __global__ void __launch_bounds__(block_threads(TPR)) channel_norm_kernel(const 
 template <typename TS, typename TB, bool ALIGNED, int TPR, int NCH>
 __global__ void __launch_bounds__(block_threads(TPR)) gated_join_kernel(const nnb_join_args a) {
   constexpr int kRows = block_threads(TPR) / TPR;
-  constexpr bool kAhead = NCH <= 2;
+  constexpr bool kAhead = NCH <= 3;
   __shared__ float buffers[2 * (TPR > 32 ? TPR / 32 : 1)];
   int turn = 0;
   const int lane = threadIdx.x % TPR, channels = a.channels;
@@ -419,23 +419,42 @@ int launch_join(const nnb_join_args& a, cudaStream_t stream) {
 }
 
 // Threads per row and chunks per thread by the row's length.  Up to 256 channels a warp or less has a row, and
-// its sums need no barrier.  Beyond, two chunks a thread carry more loads; a join, with its registers for three
-// operands and their successors, does better with one chunk and more threads where both fit (B200, bfloat16 rows:
-// norm of 2048 channels 128 x 2 44 us, 256 x 1 53 us; join of 512 channels 32 x 2 140 us, 64 x 1 119 us; join of
-// 4096 channels 256 x 2 146 us, 512 x 1 161 us).
+// its sums need no barrier.  A thread wants some 32 bytes of every operand on the way: two chunks of 16-bit values
+// (B200, bfloat16 norm of 256 channels: 16 x 2 44.5 us, 32 x 1 53.5 us), and as many threads as that leaves on
+// longer rows (2048 channels: 128 x 2 44 us, 256 x 1 53 us).  A join, with registers for three operands and their
+// successors, does better with one chunk and more threads where both fit (512 channels: 64 x 1 119 us, 32 x 2
+// 140 us; 4096: 256 x 2 146 us, 512 x 1 161 us).  Rows that are not aligned fetch single elements and want threads
+// (1001 channels: 128 x 1 56 us, 64 x 2 68 us).  Up to 384 channels, 16 x 3 leaves fewer of them idle than the
+// next power of two (320 channels: join 16 x 3 149 us, 64 x 1 177 us).
 template <typename T, bool ALIGNED>
 int norm_by_channels(const nnb_norm_args& a, cudaStream_t stream) {
   const int chunks = (a.channels + 7) / 8;
-  if (chunks <= 4) return launch_norm<T, ALIGNED, 4, 1>(a, stream);
-  if (chunks <= 8) return launch_norm<T, ALIGNED, 8, 1>(a, stream);
-  if (chunks <= 16) return launch_norm<T, ALIGNED, 16, 1>(a, stream);
-  if (chunks <= 32) return launch_norm<T, ALIGNED, 32, 1>(a, stream);
-  if (chunks <= 64) return launch_norm<T, ALIGNED, 32, 2>(a, stream);
-  if (chunks <= 128) return launch_norm<T, ALIGNED, 64, 2>(a, stream);
-  if (chunks <= 256) return launch_norm<T, ALIGNED, 128, 2>(a, stream);
-  if (chunks <= 512) return launch_norm<T, ALIGNED, 256, 2>(a, stream);
+  constexpr bool kShort = ALIGNED && sizeof(T) == 2;  // a chunk of 16 bytes: two make a thread's load
+  if constexpr (kShort) {
+    if (chunks <= 4) return launch_norm<T, ALIGNED, 2, 2>(a, stream);
+    if (chunks <= 8) return launch_norm<T, ALIGNED, 4, 2>(a, stream);
+    if (chunks <= 16) return launch_norm<T, ALIGNED, 8, 2>(a, stream);
+    if (chunks <= 32) return launch_norm<T, ALIGNED, 16, 2>(a, stream);
+  } else {
+    if (chunks <= 4) return launch_norm<T, ALIGNED, 4, 1>(a, stream);
+    if (chunks <= 8) return launch_norm<T, ALIGNED, 8, 1>(a, stream);
+    if (chunks <= 16) return launch_norm<T, ALIGNED, 16, 1>(a, stream);
+    if (chunks <= 32) return launch_norm<T, ALIGNED, 32, 1>(a, stream);
+  }
+  if constexpr (ALIGNED) {
+    if (chunks <= 48) return launch_norm<T, ALIGNED, 16, 3>(a, stream);
+    if (chunks <= 64) return launch_norm<T, ALIGNED, 32, 2>(a, stream);
+    if (chunks <= 128) return launch_norm<T, ALIGNED, 64, 2>(a, stream);
+    if (chunks <= 256) return launch_norm<T, ALIGNED, 128, 2>(a, stream);
+    if (chunks <= 512) return launch_norm<T, ALIGNED, 256, 2>(a, stream);
+  } else {
+    if (chunks <= 64) return launch_norm<T, ALIGNED, 64, 1>(a, stream);
+    if (chunks <= 128) return launch_norm<T, ALIGNED, 128, 1>(a, stream);
+    if (chunks <= 256) return launch_norm<T, ALIGNED, 256, 1>(a, stream);
+    if (chunks <= 512) return launch_norm<T, ALIGNED, 512, 1>(a, stream);
+  }
   if (chunks <= 1024) return launch_norm<T, ALIGNED, 512, 2>(a, stream);
-  return launch_norm<T, ALIGNED, 512, 4>(a, stream);
+  return launch_norm<T, ALIGNED, 1024, 2>(a, stream);
 }
 
 template <typename TS, typename TB, bool ALIGNED>
@@ -445,6 +464,7 @@ int join_by_channels(const nnb_join_args& a, cudaStream_t stream) {
   if (chunks <= 8) return launch_join<TS, TB, ALIGNED, 8, 1>(a, stream);
   if (chunks <= 16) return launch_join<TS, TB, ALIGNED, 16, 1>(a, stream);
   if (chunks <= 32) return launch_join<TS, TB, ALIGNED, 32, 1>(a, stream);
+  if (ALIGNED && chunks <= 48) return launch_join<TS, TB, ALIGNED, 16, 3>(a, stream);
   if (chunks <= 64) return launch_join<TS, TB, ALIGNED, 64, 1>(a, stream);
   if (chunks <= 128) return launch_join<TS, TB, ALIGNED, 128, 1>(a, stream);
   if (chunks <= 256) return launch_join<TS, TB, ALIGNED, 256, 1>(a, stream);

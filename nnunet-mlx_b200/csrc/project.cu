@@ -182,13 +182,18 @@ __global__ void __launch_bounds__(128) project_low_kernel(const nnb_project_args
   }
 }
 
-// Four low-rank values of a row from rank j on: the sum of its parts.
+// Four low-rank values of a row from rank j on: the sum of its parts, four parts' loads at a time.
 __device__ __forceinline__ float4 low_values(const nnb_project_args& a, int parts, int64_t row, int j) {
   const float* src = a.low + row * a.rank + j;
-  float4 v = *reinterpret_cast<const float4*>(src);
-  for (int p = 1; p < parts; ++p) {
-    const float4 w = *reinterpret_cast<const float4*>(src + p * a.rows * a.rank);
-    v.x += w.x, v.y += w.y, v.z += w.z, v.w += w.w;
+  const int64_t stride = a.rows * a.rank;
+  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int p = 0; p < parts; p += 4) {
+    float4 w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      w[i] = p + i < parts ? *reinterpret_cast<const float4*>(src + (p + i) * stride) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v.x += w[i].x, v.y += w[i].y, v.z += w[i].z, v.w += w[i].w;
   }
   return v;
 }
@@ -637,13 +642,19 @@ __global__ void __launch_bounds__(kThreads, Tile<BN>::kCtas)
       all = adapter_barrier(alive);  // also makes the list visible
       for (int i = 0; i < count * blocks && all; ++i) {
         const int adapter = listed[i / blocks], j0 = (i % blocks) * kRankBlock;
-        float v[kRankBlock];
-        const bool own = mine == adapter;
+        float v[kRankBlock] = {};
+        if (mine == adapter) {
+          const int ranks = min(kRankBlock, a.rank - j0);
+          const float* src = a.low + row * a.rank + j0;
+          for (int p = 0; p < parts; ++p, src += a.rows * a.rank) {  // a part's loads all on their way together
+            float4 f[kRankBlock / 4];
 #pragma unroll
-        for (int j = 0; j < kRankBlock; j += 4) {
-          float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
-          if (own && j0 + j < a.rank) f = low_values(a, parts, row, j0 + j);
-          v[j] = f.x, v[j + 1] = f.y, v[j + 2] = f.z, v[j + 3] = f.w;
+            for (int j = 0; j < kRankBlock / 4; ++j)
+              f[j] = j * 4 < ranks ? *reinterpret_cast<const float4*>(src + j * 4) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int j = 0; j < kRankBlock / 4; ++j)
+              v[j * 4] += f[j].x, v[j * 4 + 1] += f[j].y, v[j * 4 + 2] += f[j].z, v[j * 4 + 3] += f[j].w;
+          }
         }
         alive = alive && mbar_wait(smem_u32(&low_empty[ring.s]), ring.phase ^ 1, abort_flag, 50);
         uint8_t* at = low_stages + ring.s * C::kStage;

@@ -6,22 +6,22 @@
 // down_a has the adapter's rank of rows, up_a that many columns; both are
 // padded with zeros to a common multiple of 16.
 //
-// Low-rank rows scale_a down_a x_t come first, in float32, as partial sums over
-// parts of the channels that their readers add up: project_low_kernel (a dot
-// product per warp) for up to 128 rows, project_low_tile_kernel (tcgen05) for
-// more.  Then, by the number of rows alone (so a row's value does not depend on
-// the rows beside it):
+// Low-rank rows scale_a down_a x_t come first, then, by the number of rows alone
+// (so a row's value does not depend on the rows beside it):
 //
-//  * more than 128 rows, project_kernel: a tcgen05 GEMM over tiles of 128 rows x
-//    BN columns whose K axis goes on past W's channels.  For every adapter among
-//    a tile's rows it appends the adapter's ranks, with the rows of other
+//  * more than 128 rows: project_low_tile_kernel (tcgen05) and project_kernel, a
+//    tcgen05 GEMM over tiles of 128 rows x 64 or 128 columns, or of 256 x 256 by
+//    pairs of CTAs, whose K axis goes on past W's channels.  For every adapter
+//    among a tile's rows it appends the adapter's ranks, with the rows of other
 //    requests set to zero, into the same accumulator.  It needs neither sorting
 //    of the rows nor a pass over the output; requests whose rows follow one
 //    another keep the adapters of a tile few.
 //  * up to 128 rows (serving: a row or some per request, each with another
-//    adapter), project_few_kernel: W's rows are the MMA's 128 and the requests'
-//    its columns, so that nearly every byte staged is W's; clusters split K.
-//    The product with up is a float32 dot product per output while W streams.
+//    adapter): project_low_kernel (a dot product per warp) and
+//    project_few_kernel.  W's rows are the MMA's 128 and the requests' its
+//    columns, so that nearly every byte staged is W's; clusters split K.  The
+//    product with up is a float32 dot product per output while W streams.
+//  * up to 128 channels on either side: project_narrow_kernel does it all at once.
 //
 // Roles of project_kernel's warps:
 //   0      TMA producer of x and W chunks (64 channels a stage, 128-byte swizzle)
@@ -30,12 +30,10 @@
 //          the rows' low-rank values into a stage, a thread per row, as two
 //          bfloat16 parts hi + lo (2^-17 of the value at most is lost; a single
 //          bfloat16 would cost the output as much as its own rounding)
-//   6-9    epilogue: TMEM -> bias -> 16-bit rows, one of two accumulators each
+//   6-13   epilogue: TMEM -> bias -> 16-bit rows; warps 6-9 one of the two accumulators, 10-13 the other
 // W's chunks and the adapters' have rings of their own, so each producer runs
 // ahead as far as its ring allows; warps 2-5 announce the number of adapters of
 // a tile, which only the MMA issuer needs.
-//
-// Up to 128 channels on either side project_narrow_kernel does it all at once.
 #include <cuda.h>
 #include <cudaTypedefs.h>
 #include <cuda_bf16.h>
@@ -64,22 +62,27 @@ using namespace tc;
 
 constexpr int kBadIndex = 41;  // site number of an adapter index out of range; 42-63 are waits
 
-constexpr int kThreads = 320;
+constexpr int kThreads = 448;
 constexpr int kStageA = BM * 128;
 constexpr int kRankBlock = 32;  // ranks of an adapter stage: a 128-byte row of 32 hi and 32 lo parts
 
-template <int BN>
+// PAIR: two CTAs of a cluster make a tile of 256 rows (cta_group::2): each loads and keeps its 128 rows and half of
+// W's, and the tensor cores read the other half from the peer.
+template <typename T, int BN, bool PAIR>
 struct Tile {
-  // Stages as shared memory allows beside the staging rows; the narrowest tile leaves room for a second CTA.
-  static constexpr int kStages = BN == 256 ? 3 : BN == 128 ? 4 : BN == 64 ? 6 : 3;
-  static constexpr int kLowStages = BN == 256 ? 1 : 2;
-  static constexpr int kCtas = BN == 32 ? 2 : 1;
-  static constexpr int kStageB = BN * 128;
+  static constexpr bool kF16 = !std::is_same<T, __nv_bfloat16>::value;
+  static constexpr int kPeers = PAIR ? 2 : 1;
+  static constexpr int kRows = BM * kPeers;
+  static constexpr int kStageB = BN / kPeers * 128;
   static constexpr int kStage = kStageA + kStageB;
-  static constexpr int kColumns = BN < 64 ? BN : 64;  // columns an epilogue warp stages at a time
-  static constexpr int kStaging = 32 * kColumns * 2;
+  static constexpr int kPlane = BN / kPeers * 64;  // one part of up: 64-byte rows of 32 ranks
+  static constexpr int kLowStage = kStageA + kPlane * (kF16 ? 2 : 1);
+  static constexpr int kStages = BN == 64 ? 6 : 4;  // as shared memory allows
+  static constexpr int kLowStages = 2;
+  static constexpr int kStaging = 32 * 32 * 2;  // an epilogue warp's 32 rows of 32 columns
   static constexpr int kTmem = 2 * BN;
-  static constexpr int kSmem = 1024 + (kStages + kLowStages) * kStage + 4 * (kStaging + BN * 4) + 1024;
+  static constexpr int kSmem =
+      1024 + kStages * kStage + kLowStages * kLowStage + 8 * kStaging + 4 * BN * 4 + 3072;
 };
 
 constexpr int kCounts = 4;  // tiles whose number of adapters may be announced ahead
@@ -112,14 +115,22 @@ __device__ __forceinline__ uint32_t pack2(float a, float b, __half) {
   return *reinterpret_cast<const uint32_t*>(&v);
 }
 
-// The adapter of a row, -1 for none.  An index out of range counts as none and is recorded.
-__device__ __forceinline__ int row_adapter(const nnb_project_args& a, int64_t row) {
-  const int v = __ldg(a.index + (a.rows_per_index == 1 ? row : (uint32_t)row / (uint32_t)a.rows_per_index));
+// What the index holds for a row.
+__device__ __forceinline__ int row_index(const nnb_project_args& a, int64_t row) {
+  return __ldg(a.index + (a.rows_per_index == 1 ? row : (uint32_t)row / (uint32_t)a.rows_per_index));
+}
+
+// The adapter that an index names, -1 for none.  One out of range counts as none and is recorded.
+__device__ __forceinline__ int checked_adapter(const nnb_project_args& a, int v) {
   if (v >= a.adapters || v < -1) {
     if (atomicCAS(&g_device_status, 0, NNB_E_DEVICE) == 0) g_device_status_where = kBadIndex;
     return -1;
   }
   return v;
+}
+
+__device__ __forceinline__ int row_adapter(const nnb_project_args& a, int64_t row) {
+  return checked_adapter(a, row_index(a, row));
 }
 
 // ---------------------------------------------------------------------------
@@ -138,6 +149,30 @@ __global__ void __launch_bounds__(256) align_rows_kernel(const uint16_t* x, int6
 // ---------------------------------------------------------------------------
 // low[p][t][j] = scale_a sum over part p of k of down_a[j][k] x[t][k]: a warp takes four ranks of one row.
 // ---------------------------------------------------------------------------
+// 32 TMEM columns of this thread's lane, asked for and waited for apart.
+__device__ __forceinline__ void tmem_load32(uint32_t taddr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+      "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr));
+}
+
+// The registers pass through the wait, so that nothing reads them before it.
+__device__ __forceinline__ void tmem_loaded32(uint32_t (&r)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
+                 "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]),
+                 "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]),
+                 "+r"(r[30]), "+r"(r[31])
+               :
+               : "memory");
+}
+
 template <typename T>
 __device__ __forceinline__ void widen(float (&v)[8], const uint4& raw) {
   const T* t = reinterpret_cast<const T*>(&raw);
@@ -157,7 +192,7 @@ __global__ void __launch_bounds__(128) project_low_kernel(const nnb_project_args
   float sum[4] = {0.f, 0.f, 0.f, 0.f};
   const int begin = blockIdx.z * part, end = min(a.k, begin + part);
   const int whole = begin + ((end - begin) & ~7);
-#pragma unroll 2
+#pragma unroll 4
   for (int k = begin + lane * 8; k < whole; k += 256) {
     float v[8], d[8];
     widen<T>(v, *reinterpret_cast<const uint4*>(x + k));
@@ -215,6 +250,31 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map
       : "memory");
 }
 
+// Loads of a pair's CTA that complete on a barrier of the cluster's CTA 0 (its shared::cluster address).
+__device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const CUtensorMap* map, int c0, int c1, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, "
+      "%3}], [%4];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(bar)
+      : "memory");
+}
+
+__device__ __forceinline__ void tma_load_3d_pair(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2,
+                                                 uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, "
+      "%3, %4}], [%5];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(bar)
+      : "memory");
+}
+
+// The shared::cluster address of this place in CTA 0.
+__device__ __forceinline__ uint32_t in_first_cta(uint32_t at) {
+  uint32_t remote;
+  asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(remote) : "r"(at));
+  return remote;
+}
+
 __device__ __forceinline__ void mbar_expect_tx(uint32_t bar, uint32_t bytes) {
   asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
@@ -228,50 +288,125 @@ __device__ __forceinline__ void mma_f16(uint32_t d_tmem, uint64_t a_desc, uint64
       : "memory");
 }
 
-// Barrier of the four adapter warps; true when every one of their threads passed `ok`.
-__device__ __forceinline__ bool adapter_barrier(bool ok) {
+__device__ __forceinline__ void mma_f16_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                             uint32_t accumulate) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// Commit of the pair's MMAs to the barrier at this place in both CTAs' shared memory.
+__device__ __forceinline__ void mma_commit_pair(uint32_t bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
+      "h"((uint16_t)3)
+      : "memory");
+}
+
+// Arrival at the barrier of the same place in the cluster's CTA 0.  What it announces lies in this SM (a stage
+// behind a proxy fence, TMEM columns read): a release to the cluster's scope would first wait, some 1800 cycles,
+// for every global access of the thread.
+__device__ __forceinline__ void mbar_arrive_first(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(in_first_cta(bar)) : "memory");
+}
+
+// Bounded wait for arrivals that may come from the cluster's other CTA.
+__device__ __forceinline__ bool mbar_wait_cluster(uint32_t bar, uint32_t parity, volatile int* abort_flag, int where) {
+  if (!mbar_wait(bar, parity, abort_flag, where)) return false;
+  uint32_t ok;  // the phase is over: this only orders what follows after the peer's writes
+  asm volatile(
+      "{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n"
+      " selp.u32 %0, 1, 0, p;\n}\n"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+
+__device__ __forceinline__ void cluster_barrier() {
+  asm volatile("barrier.cluster.arrive.release;\n barrier.cluster.wait.acquire;" ::: "memory");
+}
+
+// Barrier of four warps; true when every one of their threads passed `ok`.  Barrier 1: the adapter warps.
+template <int ID>
+__device__ __forceinline__ bool four_warps_barrier(bool ok) {
   uint32_t all;
   asm volatile(
-      "{\n .reg .pred p, q;\n setp.ne.u32 p, %1, 0;\n barrier.cta.red.and.pred q, 1, 128, p;\n"
+      "{\n .reg .pred p, q;\n setp.ne.u32 p, %1, 0;\n barrier.cta.red.and.pred q, %2, 128, p;\n"
       " selp.u32 %0, 1, 0, q;\n}\n"
       : "=r"(all)
-      : "r"((uint32_t)ok)
+      : "r"((uint32_t)ok), "n"(ID)
       : "memory");
   return all != 0;
 }
 
-// The adapters among a tile's rows in ascending order, by the four adapter warps (thread r holds row r's in
-// `mine`, -1 for none); returns their number.  One adapter per turn; two buffers of minima need one barrier a turn.
-__device__ __forceinline__ int list_adapters(int mine, int r, volatile int* smallest, volatile int* listed,
-                                             int& turn) {
-  int count = 0;
-  for (int low = -1;;) {
-    const int least = __reduce_min_sync(0xffffffffu, mine > low ? mine : INT_MAX);
-    if ((r & 31) == 0) smallest[turn * 4 + (r >> 5)] = least;
-    adapter_barrier(true);
-    low = min(min(smallest[turn * 4], smallest[turn * 4 + 1]), min(smallest[turn * 4 + 2], smallest[turn * 4 + 3]));
-    turn ^= 1;
-    if (low == INT_MAX) return count;
-    if (r == 0) listed[count] = low;
-    ++count;
+__device__ __forceinline__ bool adapter_barrier(bool ok) { return four_warps_barrier<1>(ok); }
+
+// One thread of a converged warp.  The warp walks a kernel's loops together and this thread issues: with loops of
+// a single lane the compiler takes every descriptor through a vector register, and an MMA takes 120 cycles to
+// issue; so its operands stay uniform.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(p));
+  return p != 0;
+}
+
+// The MMAs of a chunk: `steps` of 16 channels, 32 bytes further along every row each.
+template <bool PAIR>
+__device__ __forceinline__ void chunk_mmas(uint32_t d, uint64_t x, uint64_t w, uint32_t idesc, int steps,
+                                           uint32_t accumulate) {
+  if (steps == 4) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if constexpr (PAIR)
+        mma_f16_pair(d, x + k * 2, w + k * 2, idesc, k > 0 ? 1 : accumulate);
+      else
+        mma_f16(d, x + k * 2, w + k * 2, idesc, k > 0 ? 1 : accumulate);
+    }
+  } else {
+    for (int k = 0; k < steps; ++k) {
+      if constexpr (PAIR)
+        mma_f16_pair(d, x + k * 2, w + k * 2, idesc, k > 0 ? 1 : accumulate);
+      else
+        mma_f16(d, x + k * 2, w + k * 2, idesc, k > 0 ? 1 : accumulate);
+    }
   }
 }
 
-// ---------------------------------------------------------------------------
-// Low-rank rows of more than 128 rows.  A CTA takes 128 rows and a part of the
-// channels: x's chunk against the down rows of the tile's adapters, as many as
-// fit 128 columns of one MMA at a time.  Bound by reading x once, so two CTAs
-// share an SM to keep its loads coming while one starts or ends.
-// ---------------------------------------------------------------------------
-constexpr int kLowColumns = 128;
-constexpr int kLowStage = kStageA + kLowColumns * 128;
-constexpr int kLowStages = 3;
-constexpr int kLowThreads = 192;
-constexpr int kLowSmem = 1024 + kLowStages * kLowStage + 1024;
-
-struct LowMaps {
-  CUtensorMap x, down;
-};
+// The adapters among a tile's rows in ascending order, by the four adapter warps (thread r holds row r's in
+// `mine` and a pair's other row's in `other`, -1 for none); returns their number.  Each warp lists its own, and
+// every thread merges the four lists.  `heads`: 4 counts, then 4 lists of ROWS / 4.
+template <int ROWS>
+__device__ __forceinline__ int list_adapters(int mine, int other, int r, volatile int* heads, volatile int* listed) {
+  constexpr int kList = ROWS / 4;
+  const int warp = r >> 5;
+  volatile int* own = heads + 4 + warp * kList;
+  int count = 0;
+  for (int low = -1;;) {
+    low = __reduce_min_sync(0xffffffffu, min(mine > low ? mine : INT_MAX, other > low ? other : INT_MAX));
+    if (low == INT_MAX) break;
+    if ((r & 31) == 0) own[count] = low;
+    ++count;
+  }
+  if ((r & 31) == 0) heads[warp] = count;
+  adapter_barrier(true);
+  int at[4] = {0, 0, 0, 0}, total = 0;
+  const int counts[4] = {heads[0], heads[1], heads[2], heads[3]};
+  int next[4];
+#pragma unroll
+  for (int w = 0; w < 4; ++w) next[w] = counts[w] > 0 ? heads[4 + w * kList] : INT_MAX;
+  for (;;) {
+    const int low = min(min(next[0], next[1]), min(next[2], next[3]));
+    if (low == INT_MAX) return total;
+    if (r == 0) listed[total] = low;
+    ++total;
+#pragma unroll
+    for (int w = 0; w < 4; ++w)
+      if (next[w] == low) next[w] = ++at[w] < counts[w] ? heads[4 + w * kList + at[w]] : INT_MAX;
+  }
+}
 
 __device__ __forceinline__ void tmem_ld16(uint32_t taddr, float (&v)[16]) {
   uint32_t r[16];
@@ -286,27 +421,71 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, float (&v)[16]) {
   for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
 }
 
+// Two low-rank values as two bfloat16 parts each, hi + lo.  What an infinity leaves would be no number.
+__device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t& lo) {
+  const float ha = __bfloat162float(__float2bfloat16_rn(a)), hb = __bfloat162float(__float2bfloat16_rn(b));
+  hi = pack2(ha, hb, __nv_bfloat16());
+  lo = pack2(isfinite(ha) ? a - ha : 0.f, isfinite(hb) ? b - hb : 0.f, __nv_bfloat16());
+}
+
+// ---------------------------------------------------------------------------
+// Low-rank rows of more than 128 rows, as the GEMM's stages take them: per row
+// and block of 32 ranks 128 bytes, 32 hi parts and 32 lo parts.
+//
+// A cluster takes 128 rows, a CTA of it a part of the channels: x's chunk
+// against the down rows of the tile's adapters, as many as fit the MMA's
+// columns at a time.  The CTAs add their parts up through shared memory.  Bound
+// by reading x once, so two CTAs share an SM (up to rank 64) to keep its loads
+// coming while one starts or ends.
+// ---------------------------------------------------------------------------
+constexpr int kLowThreads = 192;
+
+struct LowMaps {
+  CUtensorMap x, down;
+};
+
+struct LowTilePlan {
+  int part;     // chunks of 64 channels of a CTA
+  int columns;  // of the MMA: 64, or 128 beyond rank 64
+  int stages;
+  int smem;
+};
+
+LowTilePlan low_tile_plan(int rank) {
+  LowTilePlan p;
+  p.part = 0;
+  p.columns = rank <= 64 ? 64 : 128;
+  p.stages = rank <= 128 ? 3 : 2;
+  p.smem = 1024 + p.stages * (kStageA + p.columns * 128) + BM * (rank + 4) * 4 + 2048;
+  return p;
+}
+
 template <typename T>
 __global__ void __launch_bounds__(kLowThreads, 2)
-    project_low_tile_kernel(const nnb_project_args a, const __grid_constant__ LowMaps maps, const int part) {
+    project_low_tile_kernel(const nnb_project_args a, const __grid_constant__ LowMaps maps, const LowTilePlan plan) {
   constexpr bool kF16 = !std::is_same<T, __nv_bfloat16>::value;
-  constexpr int S = kLowStages;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* stages = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint64_t* full = reinterpret_cast<uint64_t*>(stages + S * kLowStage);
+  const int S = plan.stages, stage = kStageA + plan.columns * 128;
+  const int pitch = a.rank + 4;  // floats of a row of sums: neighbouring rows 16 bytes apart modulo the banks
+  float* sums = reinterpret_cast<float*>(stages + S * stage);
+  float* scales = sums + BM * pitch;  // of each row's adapter; negative infinity for none
+  uint64_t* full = reinterpret_cast<uint64_t*>(scales + BM);
   uint64_t* empty = full + S;
   uint64_t* acc_full = empty + S;
   uint64_t* acc_empty = acc_full + 1;
   uint64_t* drain = acc_empty + 1;
-  volatile int* smallest = reinterpret_cast<volatile int*>(drain + 1);
-  volatile int* listed = smallest + 8;
-  volatile int* list_count = listed + BM;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(const_cast<int*>(list_count + 1));
+  volatile int* heads = reinterpret_cast<volatile int*>(drain + 1);
+  volatile int* listed = heads + 4 + BM;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(const_cast<int*>(listed + BM));
   int* abort_flag = reinterpret_cast<int*>(tmem_slot + 1);
+  volatile int* list_count = abort_flag + 1;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t row0 = (int64_t)blockIdx.x * BM;
-  const int first_chunk = blockIdx.y * part, chunks = min((a.k + 63) / 64 - first_chunk, part);
+  const int total_chunks = (a.k + 63) / 64;
+  const int first_chunk = min((int)blockIdx.y * plan.part, total_chunks);
+  const int chunks = min(total_chunks - first_chunk, plan.part);
   if (threadIdx.x == 0) {
     for (int s = 0; s < S; ++s) {
       mbar_init(smem_u32(&full[s]), 1);
@@ -320,16 +499,16 @@ __global__ void __launch_bounds__(kLowThreads, 2)
   }
   if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
-                 "r"(kLowColumns)
+                 "r"(plan.columns)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
-  const int r = threadIdx.x - 64;
+  const int r = (warp & 3) * 32 + lane;  // warps 2-5: the TMEM row a thread may read
   int mine = -1;
   if (warp >= 2) {
     if (row0 + r < a.rows) mine = row_adapter(a, row0 + r);
-    int turn = 0;
-    const int count = list_adapters(mine, r, smallest, listed, turn);
+    scales[r] = mine < 0 ? -INFINITY : __ldg(a.scales + mine);
+    const int count = list_adapters<BM>(mine, -1, r, heads, listed);
     if (r == 0) *list_count = count;
   }
   fence_before();
@@ -341,31 +520,31 @@ __global__ void __launch_bounds__(kLowThreads, 2)
   // columns first would keep them until this grid has ended.
   asm volatile("griddepcontrol.launch_dependents;");
   // a pass: `together` adapters of all their ranks, or 128 ranks (the last of them fewer) of one
-  const int blocks = (a.rank + kLowColumns - 1) / kLowColumns;
-  const int together = max(1, kLowColumns / a.rank);
+  const int blocks = (a.rank + plan.columns - 1) / plan.columns;
+  const int together = max(1, plan.columns / a.rank);
   const int passes = blocks > 1 ? count * blocks : (count + together - 1) / together;
-  const int box = min(a.rank, kLowColumns);
+  const int box = min(a.rank, plan.columns);
 
   if (warp == 0) {
     if (lane == 0) {
-      Ring<S> ring;
-      int issued = 0;
+      int s = 0, issued = 0;
+      uint32_t phase = 0;
       bool alive = true;
       for (int p = 0; p < passes && alive; ++p) {
         const int from = blocks > 1 ? p / blocks : p * together;
         const int to = blocks > 1 ? from + 1 : min(count, from + together);
         for (int c = first_chunk; c < first_chunk + chunks; ++c) {
-          if (!mbar_wait(smem_u32(&empty[ring.s]), ring.phase ^ 1, abort_flag, 53)) {
+          if (!mbar_wait(smem_u32(&empty[s]), phase ^ 1, abort_flag, 53)) {
             alive = false;
             break;
           }
-          const uint32_t bar = smem_u32(&full[ring.s]), at = smem_u32(stages + ring.s * kLowStage);
+          const uint32_t bar = smem_u32(&full[s]), at = smem_u32(stages + s * stage);
           mbar_arrive_expect_tx(bar, kStageA + (to - from) * box * 128);
           tma_load_2d(at, &maps.x, c * 64, (int)row0, bar);
           for (int i = from; i < to; ++i)
-            tma_load_3d(at + kStageA + (i - from) * box * 128, &maps.down, c * 64, (p % blocks) * kLowColumns,
+            tma_load_3d(at + kStageA + (i - from) * box * 128, &maps.down, c * 64, (p % blocks) * plan.columns,
                         listed[i], bar);
-          ring.next();
+          if (++s == S) s = 0, phase ^= 1u;
           ++issued;
         }
       }
@@ -375,64 +554,57 @@ __global__ void __launch_bounds__(kLowThreads, 2)
     }
     __syncwarp();
   } else if (warp == 1) {
-    if (lane == 0) {
-      Ring<S> ring;
-      bool alive = true;
-      for (int p = 0; p < passes && alive; ++p) {
-        if (!mbar_wait(smem_u32(acc_empty), (uint32_t)(p & 1) ^ 1, abort_flag, 55)) break;
+    const bool issuer = elect_one();
+    int s = 0;
+    uint32_t phase = 0;
+    bool alive = true;
+    for (int p = 0; p < passes && alive; ++p) {
+      alive = __all_sync(0xffffffffu, mbar_wait(smem_u32(acc_empty), (uint32_t)(p & 1) ^ 1, abort_flag, 55));
+      if (!alive) break;
+      fence_after();
+      const int columns = blocks > 1 ? min(plan.columns, a.rank - (p % blocks) * plan.columns)
+                                     : (min(count, (p + 1) * together) - p * together) * a.rank;
+      const uint32_t idesc = kF16 ? idesc_f16(BM, columns) : idesc_bf16(BM, columns);
+      for (int c = first_chunk; c < first_chunk + chunks; ++c) {
+        alive = __all_sync(0xffffffffu, mbar_wait(smem_u32(&full[s]), phase, abort_flag, 56));
+        if (!alive) break;
         fence_after();
-        const int columns = blocks > 1 ? min(kLowColumns, a.rank - (p % blocks) * kLowColumns)
-                                       : (min(count, (p + 1) * together) - p * together) * a.rank;
-        const uint32_t idesc = kF16 ? idesc_f16(BM, columns) : idesc_bf16(BM, columns);
-        uint32_t accumulate = 0;
-        for (int c = first_chunk; c < first_chunk + chunks; ++c) {
-          if (!mbar_wait(smem_u32(&full[ring.s]), ring.phase, abort_flag, 56)) {
-            alive = false;
-            break;
-          }
-          fence_after();
-          const uint32_t at = smem_u32(stages + ring.s * kLowStage);
-          const uint64_t ad = sw128_desc(at), bd = sw128_desc(at + kStageA);
-          const int steps = min(4, (a.k - c * 64 + 15) / 16);
-          for (int k = 0; k < steps; ++k) {
-            mma_f16(tmem, ad + k * 2, bd + k * 2, idesc, accumulate);
-            accumulate = 1;
-          }
-          mma_commit(smem_u32(&empty[ring.s]));
-          ring.next();
+        const uint32_t at = smem_u32(stages + s * stage);
+        if (issuer) {
+          chunk_mmas<false>(tmem, sw128_desc(at), sw128_desc(at + kStageA), idesc, min(4, (a.k - c * 64 + 15) / 16),
+                            c > first_chunk);
+          mma_commit(smem_u32(&empty[s]));
         }
-        if (alive) mma_commit(smem_u32(acc_full));
+        __syncwarp();
+        if (++s == S) s = 0, phase ^= 1u;
       }
-      if (*reinterpret_cast<volatile int*>(abort_flag)) {
-        mma_commit(smem_u32(drain));
-        mbar_wait(smem_u32(drain), 0, abort_flag, 57, false);
-      }
+      if (alive && issuer) mma_commit(smem_u32(acc_full));
+      __syncwarp();
+    }
+    if (issuer && *reinterpret_cast<volatile int*>(abort_flag)) {
+      mma_commit(smem_u32(drain));
+      mbar_wait(smem_u32(drain), 0, abort_flag, 57, false);
     }
     __syncwarp();
   } else {
-    const int quarter = warp & 3;
-    const int64_t row = row0 + quarter * 32 + lane;
-    const int own = row < a.rows ? row_adapter(a, row) : -1;  // the lane's TMEM row, not the listed one
-    float* out = a.low + (blockIdx.y * a.rows + row) * a.rank;
-    const float scale = own < 0 ? 0.f : __ldg(a.scales + own);
     for (int p = 0; p < passes; ++p) {
       const int from = blocks > 1 ? p / blocks : p * together;
       const int to = blocks > 1 ? from + 1 : min(count, from + together);
-      const int j0 = (p % blocks) * kLowColumns, width = min(kLowColumns, a.rank - j0);
+      const int j0 = (p % blocks) * plan.columns, width = min(plan.columns, a.rank - j0);
       const bool ok = mbar_wait(smem_u32(acc_full), (uint32_t)p & 1, abort_flag, 58);
       if (!__all_sync(0xffffffffu, ok)) break;
       fence_after();
       for (int i = from; i < to; ++i) {
         const int adapter = listed[i];
-        if (!__any_sync(0xffffffffu, own == adapter)) continue;
+        if (!__any_sync(0xffffffffu, mine == adapter)) continue;
         for (int j = 0; j < width; j += 16) {
           float v[16];
-          tmem_ld16(tmem + ((uint32_t)quarter << 21) + (i - from) * box + j, v);
-          if (own == adapter) {
+          tmem_ld16(tmem + ((uint32_t)(warp & 3) << 21) + (i - from) * box + j, v);
+          if (mine == adapter) {
 #pragma unroll
             for (int e = 0; e < 16; e += 4)
-              *reinterpret_cast<float4*>(out + j0 + j + e) =
-                  make_float4(v[e] * scale, v[e + 1] * scale, v[e + 2] * scale, v[e + 3] * scale);
+              *reinterpret_cast<float4*>(sums + r * pitch + j0 + j + e) =
+                  chunks > 0 ? make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]) : make_float4(0.f, 0.f, 0.f, 0.f);
           }
         }
       }
@@ -441,10 +613,42 @@ __global__ void __launch_bounds__(kLowThreads, 2)
       if (lane == 0) mbar_arrive(smem_u32(acc_empty));
     }
   }
-  __syncthreads();
+  cluster_barrier();
+  if (warp >= 2 && *reinterpret_cast<volatile int*>(abort_flag) == 0) {
+    // this CTA's share of the rows: four ranks a thread and turn, summed over the cluster in order
+    const int parts = gridDim.y, share = (BM + parts - 1) / parts;
+    const int begin = blockIdx.y * share, end = min(BM, begin + share);
+    const int fours = a.rank / 4, low_blocks = (a.rank + kRankBlock - 1) / kRankBlock;
+    const uint32_t base = smem_u32(sums);
+    for (int i = r; i < (end - begin) * fours; i += 128) {
+      const int row = begin + i / fours, j = i % fours * 4;
+      const float scale = scales[row];
+      if (scale == -INFINITY) continue;
+      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int c = 0; c < parts; ++c) {
+        uint32_t peer;
+        asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(peer) : "r"(base + (row * pitch + j) * 4), "r"(c));
+        float4 w;
+        asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                     : "=f"(w.x), "=f"(w.y), "=f"(w.z), "=f"(w.w)
+                     : "r"(peer)
+                     : "memory");
+        v.x += w.x, v.y += w.y, v.z += w.z, v.w += w.w;
+      }
+      uint2 hi, lo;
+      split2(v.x * scale, v.y * scale, hi.x, lo.x);
+      split2(v.z * scale, v.w * scale, hi.y, lo.y);
+      uint8_t* out = reinterpret_cast<uint8_t*>(a.low) + ((row0 + row) * low_blocks + j / kRankBlock) * 128 +
+                     j % kRankBlock * 2;
+      *reinterpret_cast<uint2*>(out) = hi;
+      *reinterpret_cast<uint2*>(out + 64) = lo;
+    }
+  }
+  cluster_barrier();  // a CTA's sums stay until its peers have read them
+  __syncwarp();
   if (warp == 1) {
     fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kLowColumns) : "memory");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(plan.columns) : "memory");
   }
 }
 
@@ -456,25 +660,28 @@ struct TileAt {
   int col0;
 };
 
-// Tiles in groups of 16 row tiles, rows first: the tiles in flight at a time share few rows and few columns.
-__device__ __forceinline__ TileAt tile_at(int64_t tile, int64_t row_tiles, int col_tiles, int bn) {
-  const int64_t group = tile / (16 * (int64_t)col_tiles);
-  const int64_t rest = tile - group * 16 * col_tiles;
-  const int64_t rows = min((int64_t)16, row_tiles - group * 16);
-  return {(group * 16 + rest % rows) * BM, (int)(rest / rows) * bn};
+// Tiles in groups of 2048 rows, rows first: the tiles in flight at a time share few rows and few columns.  32-bit
+// numbers: every role finds its next tile on the way to its first load, and a 64-bit quotient takes 400 cycles.
+template <typename C>
+__device__ __forceinline__ TileAt tile_at(uint32_t tile, uint32_t row_tiles, uint32_t col_tiles, int bn) {
+  constexpr uint32_t kGroup = 2048 / C::kRows;
+  const uint32_t group = tile / (kGroup * col_tiles), rest = tile - group * kGroup * col_tiles;
+  const uint32_t rows = min(kGroup, row_tiles - group * kGroup);
+  const uint32_t col = rest / rows;
+  return {(int64_t)(group * kGroup + rest - col * rows) * C::kRows, (int)col * bn};
 }
 
-template <typename T, int BN>
-__global__ void __launch_bounds__(kThreads, Tile<BN>::kCtas)
-    project_kernel(const nnb_project_args a, const __grid_constant__ Maps maps, const int parts) {
-  using C = Tile<BN>;
+template <typename T, int BN, bool PAIR>
+__global__ void __launch_bounds__(kThreads, 1)
+    project_kernel(const nnb_project_args a, const __grid_constant__ Maps maps) {
+  using C = Tile<T, BN, PAIR>;
   constexpr int S = C::kStages, SL = C::kLowStages;
   constexpr bool kF16 = !std::is_same<T, __nv_bfloat16>::value;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* stages = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* low_stages = stages + S * C::kStage;
-  uint8_t* staging = low_stages + SL * C::kStage;
-  float* bias_rows = reinterpret_cast<float*>(staging + 4 * C::kStaging);
+  uint8_t* staging = low_stages + SL * C::kLowStage;
+  float* bias_rows = reinterpret_cast<float*>(staging + 8 * C::kStaging);  // by tile modulo 4
   uint64_t* full = reinterpret_cast<uint64_t*>(bias_rows + 4 * BN);
   uint64_t* empty = full + S;
   uint64_t* low_full = empty + S;
@@ -485,16 +692,17 @@ __global__ void __launch_bounds__(kThreads, Tile<BN>::kCtas)
   uint64_t* count_empty = count_full + kCounts;
   uint64_t* drain = count_empty + kCounts;
   volatile int* counts = reinterpret_cast<volatile int*>(drain + 1);  // adapters of the tiles announced
-  volatile int* smallest = counts + kCounts;                          // 2 x 4 warps
-  volatile int* listed = smallest + 8;                                // the tile's adapters, ascending
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(const_cast<int*>(listed + BM));
+  volatile int* heads = counts + kCounts;                             // the adapter warps' lists
+  volatile int* listed = heads + 4 + C::kRows;                        // the tile's adapters, ascending
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(const_cast<int*>(listed + C::kRows));
   int* abort_flag = reinterpret_cast<int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t row_tiles = (a.rows + BM - 1) / BM;
-  const int col_tiles = (a.n + BN - 1) / BN;
-  const int64_t tiles = row_tiles * col_tiles;
-  const int my_tiles = (int)((tiles - blockIdx.x + gridDim.x - 1) / gridDim.x);
+  const int cta = PAIR ? (int)blockIdx.x & 1 : 0;
+  const uint32_t first_tile = blockIdx.x / C::kPeers, tile_step = gridDim.x / C::kPeers;
+  const uint32_t row_tiles = (uint32_t)((a.rows + C::kRows - 1) / C::kRows), col_tiles = (a.n + BN - 1) / BN;
+  const uint32_t tiles = row_tiles * col_tiles;  // fits: the host checks
+  const int my_tiles = (int)((tiles - first_tile + tile_step - 1) / tile_step);
   const int chunks = (a.k + 63) / 64;
   const int blocks = (a.rank + kRankBlock - 1) / kRankBlock;
 
@@ -504,12 +712,12 @@ __global__ void __launch_bounds__(kThreads, Tile<BN>::kCtas)
       mbar_init(smem_u32(&empty[s]), 1);
     }
     for (int s = 0; s < SL; ++s) {
-      mbar_init(smem_u32(&low_full[s]), 1);
+      mbar_init(smem_u32(&low_full[s]), C::kPeers);  // the adapter warps of both CTAs
       mbar_init(smem_u32(&low_empty[s]), 1);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(smem_u32(&acc_full[i]), 1);
-      mbar_init(smem_u32(&acc_empty[i]), 4);  // the epilogue's warps
+      mbar_init(smem_u32(&acc_empty[i]), 4 * C::kPeers);  // the epilogues' warps
     }
     for (int i = 0; i < kCounts; ++i) {
       mbar_init(smem_u32(&count_full[i]), 1);
@@ -520,13 +728,21 @@ __global__ void __launch_bounds__(kThreads, Tile<BN>::kCtas)
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 1) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
-                 "r"(C::kTmem)
-                 : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    if constexpr (PAIR) {
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                   "r"(C::kTmem)
+                   : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    } else {
+      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                   "r"(C::kTmem)
+                   : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
   }
   fence_before();
   __syncthreads();
+  if constexpr (PAIR) cluster_barrier();  // the peer's barriers and TMEM are there
   fence_after();
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(tmem_slot);
 
@@ -537,16 +753,22 @@ __global__ void __launch_bounds__(kThreads, Tile<BN>::kCtas)
       int issued = 0;
       bool alive = true;
       for (int it = 0; it < my_tiles && alive; ++it) {
-        const TileAt t = tile_at(blockIdx.x + (int64_t)it * gridDim.x, row_tiles, col_tiles, BN);
+        const TileAt t = tile_at<C>(first_tile + it * tile_step, row_tiles, col_tiles, BN);
         for (int c = 0; c < chunks; ++c) {
           if (!mbar_wait(smem_u32(&empty[ring.s]), ring.phase ^ 1, abort_flag, 42)) {
             alive = false;
             break;
           }
           const uint32_t bar = smem_u32(&full[ring.s]), at = smem_u32(stages + ring.s * C::kStage);
-          mbar_arrive_expect_tx(bar, C::kStage);
-          tma_load_2d(at, &maps.x, c * 64, (int)t.row0, bar);
-          tma_load_2d(at + kStageA, &maps.weight, c * 64, t.col0, bar);
+          if (cta == 0) mbar_arrive_expect_tx(bar, C::kStage * C::kPeers);
+          if constexpr (PAIR) {
+            const uint32_t first = in_first_cta(bar);
+            tma_load_2d_pair(at, &maps.x, c * 64, (int)t.row0 + cta * BM, first);
+            tma_load_2d_pair(at + kStageA, &maps.weight, c * 64, t.col0 + cta * (BN / 2), first);
+          } else {
+            tma_load_2d(at, &maps.x, c * 64, (int)t.row0, bar);
+            tma_load_2d(at + kStageA, &maps.weight, c * 64, t.col0, bar);
+          }
           ring.next();
           ++issued;
         }
@@ -558,60 +780,71 @@ __global__ void __launch_bounds__(kThreads, Tile<BN>::kCtas)
     __syncwarp();
   } else if (warp == 1) {
     // ------------------------------ MMA issuer -------------------------------
-    if (lane == 0) {
-      const uint32_t main_idesc = kF16 ? idesc_f16(BM, BN) : idesc_bf16(BM, BN);
-      const uint32_t low_idesc = idesc_bf16(BM, BN);
+    if (cta == 0) {  // a pair's MMAs are CTA 0's
+      const uint32_t main_idesc = kF16 ? idesc_f16(C::kRows, BN) : idesc_bf16(C::kRows, BN);
+      const uint32_t low_idesc = idesc_bf16(C::kRows, BN);
+      auto commit = [](uint64_t* bar) {
+        if constexpr (PAIR)
+          mma_commit_pair(smem_u32(bar));
+        else
+          mma_commit(smem_u32(bar));
+      };
+      auto wait = [&](uint64_t* bar, uint32_t parity, int where) {  // for arrivals from either CTA
+        const bool ok = PAIR ? mbar_wait_cluster(smem_u32(bar), parity, abort_flag, where)
+                             : mbar_wait(smem_u32(bar), parity, abort_flag, where);
+        return (bool)__all_sync(0xffffffffu, ok);
+      };
+      const bool issuer = elect_one();
       Ring<S> ring;
       Ring<SL> low_ring;
       Ring<kCounts> counted;
       bool alive = true;
       for (int it = 0; it < my_tiles && alive; ++it) {
         const int acc = it & 1;
-        if (!mbar_wait(smem_u32(&acc_empty[acc]), (uint32_t)((it >> 1) & 1) ^ 1, abort_flag, 44)) break;
+        if (!wait(&acc_empty[acc], (uint32_t)((it >> 1) & 1) ^ 1, 44)) break;
         fence_after();
         const uint32_t d = tmem + acc * BN;
-        uint32_t accumulate = 0;
         for (int c = 0; c < chunks; ++c) {
-          if (!mbar_wait(smem_u32(&full[ring.s]), ring.phase, abort_flag, 45)) {
-            alive = false;
-            break;
-          }
+          alive = __all_sync(0xffffffffu, mbar_wait(smem_u32(&full[ring.s]), ring.phase, abort_flag, 45));
+          if (!alive) break;
           fence_after();
           const uint32_t at = smem_u32(stages + ring.s * C::kStage);
-          const uint64_t ad = sw128_desc(at), bd = sw128_desc(at + kStageA);
-          const int steps = min(4, (a.k - c * 64 + 15) / 16);
-          for (int k = 0; k < steps; ++k) {  // 16 channels: 32 bytes of every row
-            mma_f16(d, ad + k * 2, bd + k * 2, main_idesc, accumulate);
-            accumulate = 1;
+          if (issuer) {
+            chunk_mmas<PAIR>(d, sw128_desc(at), sw128_desc(at + kStageA), main_idesc,
+                             min(4, (a.k - c * 64 + 15) / 16), c > 0);
+            commit(&empty[ring.s]);
           }
-          mma_commit(smem_u32(&empty[ring.s]));
+          __syncwarp();
           ring.next();
         }
-        if (!alive || !mbar_wait(smem_u32(&count_full[counted.s]), counted.phase, abort_flag, 46)) break;
+        if (!alive ||
+            !__all_sync(0xffffffffu, mbar_wait(smem_u32(&count_full[counted.s]), counted.phase, abort_flag, 46)))
+          break;
         const int low_stages_due = counts[counted.s] * blocks;
-        mbar_arrive(smem_u32(&count_empty[counted.s]));
+        __syncwarp();
+        if (issuer) mbar_arrive(smem_u32(&count_empty[counted.s]));
         counted.next();
         for (int i = 0; i < low_stages_due; ++i) {
-          if (!mbar_wait(smem_u32(&low_full[low_ring.s]), low_ring.phase, abort_flag, 47)) {
-            alive = false;
-            break;
-          }
+          alive = wait(&low_full[low_ring.s], low_ring.phase, 47);
+          if (!alive) break;
           fence_after();
-          const uint32_t at = smem_u32(low_stages + low_ring.s * C::kStage);
-          const uint64_t hi = sw128_desc(at), lo = hi + 4, up = sw64_desc(at + kStageA);
-          const int steps = min(2, (a.rank - (i % blocks) * kRankBlock) / 16);
-          for (int k = 0; k < steps; ++k) {
-            mma_f16(d, hi + k * 2, up + k * 2, low_idesc, 1);
-            mma_f16(d, lo + k * 2, up + k * 2, low_idesc, 1);
-            if constexpr (kF16) mma_f16(d, hi + k * 2, up + (BN * 64 >> 4) + k * 2, low_idesc, 1);
+          const uint32_t at = smem_u32(low_stages + low_ring.s * C::kLowStage);
+          if (issuer) {
+            const uint64_t hi = sw128_desc(at), lo = hi + 4, up = sw64_desc(at + kStageA);
+            const int steps = min(2, (a.rank - (i % blocks) * kRankBlock) / 16);
+            chunk_mmas<PAIR>(d, hi, up, low_idesc, steps, 1);
+            chunk_mmas<PAIR>(d, lo, up, low_idesc, steps, 1);
+            if constexpr (kF16) chunk_mmas<PAIR>(d, hi, up + (C::kPlane >> 4), low_idesc, steps, 1);
+            commit(&low_empty[low_ring.s]);
           }
-          mma_commit(smem_u32(&low_empty[low_ring.s]));
+          __syncwarp();
           low_ring.next();
         }
-        if (alive) mma_commit(smem_u32(&acc_full[acc]));
+        if (alive && issuer) commit(&acc_full[acc]);
+        __syncwarp();
       }
-      if (*reinterpret_cast<volatile int*>(abort_flag)) {  // wait (bounded) for every MMA issued
-        mma_commit(smem_u32(drain));
+      if (issuer && *reinterpret_cast<volatile int*>(abort_flag)) {  // wait (bounded) for every MMA issued
+        commit(drain);
         mbar_wait(smem_u32(drain), 0, abort_flag, 48, false);
       }
     }
@@ -625,69 +858,85 @@ __global__ void __launch_bounds__(kThreads, Tile<BN>::kCtas)
     Ring<SL> ring;
     Ring<kCounts> counted;
     int issued = 0;
-    int turn = 0;
     bool alive = true;  // this thread; `all`: the four warps, which go on together or stop together
     bool all = true;
+    // A tile's rows are asked for their adapters, and for the 128 bytes of their first block of ranks, while the
+    // tile before is filled in (whether the row has an adapter or not, so that neither load waits for the other);
+    // each next block is asked for when the one before has been written.
+    int next_mine, next_other;
+    const uint4 *low = nullptr, *next_low;
+    uint4 v[8];
+    auto ask = [&](int it) {
+      next_mine = next_other = -1;
+      if (it >= my_tiles) return;
+      const TileAt t = tile_at<C>(first_tile + it * tile_step, row_tiles, col_tiles, BN);
+      const int64_t row = t.row0 + cta * BM + r, peer_row = t.row0 + (cta ^ 1) * BM + r;
+      next_low = row < a.rows ? reinterpret_cast<const uint4*>(a.low) + row * blocks * 8 : nullptr;
+      if (row < a.rows) next_mine = row_index(a, row);
+      if (PAIR && peer_row < a.rows) next_other = row_index(a, peer_row);
+    };
+    auto fetch = [&](const uint4* from) {
+      if (from != nullptr) {
+#pragma unroll
+        for (int c = 0; c < 8; ++c) v[c] = from[c];
+      }
+    };
+    next_low = nullptr;
+    ask(0);
+    fetch(next_low);
     for (int it = 0; it < my_tiles && all; ++it) {
-      const TileAt t = tile_at(blockIdx.x + (int64_t)it * gridDim.x, row_tiles, col_tiles, BN);
-      const int64_t row = t.row0 + r;
-      const int mine = row < a.rows ? row_adapter(a, row) : -1;
-      const int count = list_adapters(mine, r, smallest, listed, turn);
-      if (leader) {
+      const TileAt t = tile_at<C>(first_tile + it * tile_step, row_tiles, col_tiles, BN);
+      const int mine = checked_adapter(a, next_mine), other = checked_adapter(a, next_other);
+      low = next_low;
+      next_low = nullptr;
+      ask(it + 1);
+      if (mine < 0) fetch(next_low);
+      const int count = list_adapters<C::kRows>(mine, other, r, heads, listed);
+      if (leader && cta == 0) {
         alive = mbar_wait(smem_u32(&count_empty[counted.s]), counted.phase ^ 1, abort_flag, 49);
         counts[counted.s] = count;
         mbar_arrive(smem_u32(&count_full[counted.s]));
       }
       counted.next();
       all = adapter_barrier(alive);  // also makes the list visible
-      for (int i = 0; i < count * blocks && all; ++i) {
-        const int adapter = listed[i / blocks], j0 = (i % blocks) * kRankBlock;
-        float v[kRankBlock] = {};
-        if (mine == adapter) {
-          const int ranks = min(kRankBlock, a.rank - j0);
-          const float* src = a.low + row * a.rank + j0;
-          for (int p = 0; p < parts; ++p, src += a.rows * a.rank) {  // a part's loads all on their way together
-            float4 f[kRankBlock / 4];
-#pragma unroll
-            for (int j = 0; j < kRankBlock / 4; ++j)
-              f[j] = j * 4 < ranks ? *reinterpret_cast<const float4*>(src + j * 4) : make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-            for (int j = 0; j < kRankBlock / 4; ++j)
-              v[j * 4] += f[j].x, v[j * 4 + 1] += f[j].y, v[j * 4 + 2] += f[j].z, v[j * 4 + 3] += f[j].w;
+      for (int i = 0; i < count && all; ++i) {
+        const int adapter = listed[i];
+        const bool own = mine == adapter;
+        for (int block = 0; block < blocks && all; ++block) {
+          alive = alive && mbar_wait(smem_u32(&low_empty[ring.s]), ring.phase ^ 1, abort_flag, 50);
+          uint8_t* at = low_stages + ring.s * C::kLowStage;
+          const uint32_t bar = smem_u32(&low_full[ring.s]);
+          if (leader && alive) {
+            const uint32_t dst = smem_u32(at) + kStageA;
+            const int j0 = block * kRankBlock;
+            if (cta == 0) mbar_expect_tx(bar, C::kPlane * (kF16 ? 2 : 1) * C::kPeers);
+            if constexpr (PAIR) {
+              const uint32_t first = in_first_cta(bar);
+              const int col = t.col0 + cta * (BN / 2);
+              tma_load_3d_pair(dst, &maps.up, j0, col, adapter, first);
+              if constexpr (kF16) tma_load_3d_pair(dst + C::kPlane, &maps.up, a.rank + j0, col, adapter, first);
+            } else {
+              tma_load_3d(dst, &maps.up, j0, t.col0, adapter, bar);
+              if constexpr (kF16) tma_load_3d(dst + C::kPlane, &maps.up, a.rank + j0, t.col0, adapter, bar);
+            }
+            ++issued;
           }
-        }
-        alive = alive && mbar_wait(smem_u32(&low_empty[ring.s]), ring.phase ^ 1, abort_flag, 50);
-        uint8_t* at = low_stages + ring.s * C::kStage;
-        const uint32_t bar = smem_u32(&low_full[ring.s]);
-        if (leader && alive) {
-          const uint32_t dst = smem_u32(at) + kStageA;
-          mbar_expect_tx(bar, BN * 64 * (kF16 ? 2 : 1));
-          tma_load_3d(dst, &maps.up, j0, t.col0, adapter, bar);
-          if constexpr (kF16) tma_load_3d(dst + BN * 64, &maps.up, a.rank + j0, t.col0, adapter, bar);
-          ++issued;
-        }
-        if (alive) {
-          uint32_t hi[kRankBlock / 2], lo[kRankBlock / 2];
+          if (alive) {
+            uint4* line = reinterpret_cast<uint4*>(at + r * 128);
 #pragma unroll
-          for (int j = 0; j < kRankBlock / 2; ++j) {
-            const float h0 = __bfloat162float(__float2bfloat16_rn(v[2 * j]));
-            const float h1 = __bfloat162float(__float2bfloat16_rn(v[2 * j + 1]));
-            hi[j] = pack2(h0, h1, __nv_bfloat16());
-            // what an infinity leaves would be no number
-            lo[j] = pack2(isfinite(h0) ? v[2 * j] - h0 : 0.f, isfinite(h1) ? v[2 * j + 1] - h1 : 0.f,
-                          __nv_bfloat16());
+            for (int c = 0; c < 8; ++c) line[c ^ (r & 7)] = own ? v[c] : make_uint4(0, 0, 0, 0);
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
           }
-          uint4* line = reinterpret_cast<uint4*>(at + r * 128);
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            line[c ^ (r & 7)] = make_uint4(hi[4 * c], hi[4 * c + 1], hi[4 * c + 2], hi[4 * c + 3]);
-            line[(c + 4) ^ (r & 7)] = make_uint4(lo[4 * c], lo[4 * c + 1], lo[4 * c + 2], lo[4 * c + 3]);
+          if (own) fetch(block + 1 < blocks ? low + (block + 1) * 8 : next_low);
+          all = adapter_barrier(alive);
+          if (leader && alive) {  // also on the way out, so that the copy's phase completes
+            if constexpr (PAIR)
+              mbar_arrive_first(bar);
+            else
+              mbar_arrive(bar);
           }
-          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          ring.next();
         }
-        all = adapter_barrier(alive);
-        if (leader && alive) mbar_arrive(bar);  // also on the way out, so that the copy's phase completes
-        ring.next();
       }
     }
     if (leader && *reinterpret_cast<volatile int*>(abort_flag))
@@ -696,59 +945,70 @@ __global__ void __launch_bounds__(kThreads, Tile<BN>::kCtas)
     __syncwarp();
   } else {
     // -------------------------------- epilogue -------------------------------
-    const int quarter = warp & 3;  // the TMEM lanes a warp may read
+    const int quarter = warp & 3;      // the TMEM lanes a warp may read
+    const int acc = (warp - 6) >> 2;   // its accumulator: every other tile
     uint8_t* stage_rows = staging + (warp - 6) * C::kStaging;
-    float* bias = bias_rows + (warp - 6) * BN;
     const bool vector = (reinterpret_cast<uintptr_t>(a.out) % 16 == 0) && (a.rows == 1 || a.out_stride % 8 == 0);
-    for (int it = 0; it < my_tiles; ++it) {
-      const TileAt t = tile_at(blockIdx.x + (int64_t)it * gridDim.x, row_tiles, col_tiles, BN);
-      const int acc = it & 1;
-      __syncwarp();
-      for (int c = lane; c < BN; c += 32) bias[c] = a.bias != nullptr && t.col0 + c < a.n ? a.bias[t.col0 + c] : 0.f;
-      __syncwarp();
+    const int chunk = lane & 3, at_row = lane >> 2;  // a store covers 64 bytes of 8 rows
+    // 16-byte chunks permuted by row so that neither side meets in a bank
+    auto place = [](int row, int c) { return c ^ ((row >> 1) & 3); };
+    for (int it = acc; it < my_tiles; it += 2) {
+      const TileAt t = tile_at<C>(first_tile + it * tile_step, row_tiles, col_tiles, BN);
+      // two buffers of bias a group, written in turn: one barrier a tile, past which the buffer before is free
+      float* bias = bias_rows + (it & 3) * BN;
+      for (int c = quarter * 32 + lane; c < BN; c += 128)
+        bias[c] = a.bias != nullptr && t.col0 + c < a.n ? a.bias[t.col0 + c] : 0.f;
       const bool ok = mbar_wait(smem_u32(&acc_full[acc]), (uint32_t)(it >> 1) & 1, abort_flag, 52);
-      if (!__all_sync(0xffffffffu, ok)) break;
+      if (!(acc == 0 ? four_warps_barrier<2>(ok) : four_warps_barrier<3>(ok))) break;
       fence_after();
       const uint32_t src = tmem + acc * BN + ((uint32_t)quarter << 21);
-      const int64_t row0 = t.row0 + quarter * 32;
+      const int64_t row0 = t.row0 + cta * BM + quarter * 32;
+      const int live = (int)min((int64_t)32, a.rows - row0), columns = min(BN, a.n - t.col0);
+      const bool whole = vector && live == 32 && columns == BN;
+      T* out = reinterpret_cast<T*>(a.out) + (row0 + at_row) * a.out_stride + t.col0 + chunk * 8;
+      const int64_t eight = 8 * a.out_stride;
+      uint32_t raw[32];
+      tmem_load32(src, raw);
 #pragma unroll 1
-      for (int c0 = 0; c0 < BN; c0 += C::kColumns) {
-        if (t.col0 + c0 >= a.n) break;
-        constexpr int kChunks = C::kColumns / 8;  // 16-byte chunks of a staged row
+      for (int c0 = 0; c0 < columns; c0 += 32, out += 32) {
+        tmem_loaded32(raw);
+        float v[32];
 #pragma unroll
-        for (int h = 0; h < C::kColumns; h += 32) {
-          float v[32];
-          tmem_ld32(src + c0 + h, v);
-          uint4* line = reinterpret_cast<uint4*>(stage_rows + lane * C::kColumns * 2);
+        for (int c = 0; c < 32; ++c) v[c] = __uint_as_float(raw[c]);
+        if (c0 + 32 < columns) tmem_load32(src + c0 + 32, raw);  // on its way while these are stored
+        uint4* line = reinterpret_cast<uint4*>(stage_rows + lane * 64);
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            uint32_t p[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const float2 b = *reinterpret_cast<const float2*>(bias + c0 + h + c * 8 + j * 2);
-              p[j] = pack2(v[c * 8 + j * 2] + b.x, v[c * 8 + j * 2 + 1] + b.y, T());
-            }
-            // chunks permuted by row so that neither side meets in a bank
-            const int swap = kChunks == 8 ? lane & 7 : (lane >> 1) & 3;
-            line[(h / 8 + c) ^ swap] = make_uint4(p[0], p[1], p[2], p[3]);
-          }
+        for (int c = 0; c < 4; ++c) {
+          const float4 b0 = *reinterpret_cast<const float4*>(bias + c0 + c * 8);
+          const float4 b1 = *reinterpret_cast<const float4*>(bias + c0 + c * 8 + 4);
+          line[place(lane, c)] = make_uint4(pack2(v[c * 8] + b0.x, v[c * 8 + 1] + b0.y, T()),
+                                            pack2(v[c * 8 + 2] + b0.z, v[c * 8 + 3] + b0.w, T()),
+                                            pack2(v[c * 8 + 4] + b1.x, v[c * 8 + 5] + b1.y, T()),
+                                            pack2(v[c * 8 + 6] + b1.z, v[c * 8 + 7] + b1.w, T()));
         }
         __syncwarp();
+        uint4 packed[4];
 #pragma unroll
-        for (int i = 0; i < kChunks; ++i) {
-          const int r = (i * 32 + lane) / kChunks, c = (i * 32 + lane) % kChunks;
-          const int swap = kChunks == 8 ? r & 7 : (r >> 1) & 3;
-          const uint4 packed = reinterpret_cast<const uint4*>(stage_rows + r * C::kColumns * 2)[c ^ swap];
-          const int col = t.col0 + c0 + c * 8;
-          if (row0 + r < a.rows && col < a.n) {
-            T* out = reinterpret_cast<T*>(a.out) + (row0 + r) * a.out_stride + col;
-            if (vector && col + 8 <= a.n) {
-              *reinterpret_cast<uint4*>(out) = packed;
+        for (int i = 0; i < 4; ++i) {
+          const int r = i * 8 + at_row;
+          packed[i] = reinterpret_cast<const uint4*>(stage_rows + r * 64)[place(r, chunk)];
+        }
+        if (whole) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4*>(out + i * eight) = packed[i];
+        } else {
+          const int col = c0 + chunk * 8;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            if (i * 8 + at_row >= live || col >= columns) continue;
+            T* to = out + i * eight;
+            if (vector && col + 8 <= columns) {
+              *reinterpret_cast<uint4*>(to) = packed[i];
             } else {
-              const T* values = reinterpret_cast<const T*>(&packed);
+              const T* values = reinterpret_cast<const T*>(&packed[i]);
 #pragma unroll
               for (int j = 0; j < 8; ++j)
-                if (col + j < a.n) out[j] = values[j];
+                if (col + j < columns) to[j] = values[j];
             }
           }
         }
@@ -756,13 +1016,23 @@ __global__ void __launch_bounds__(kThreads, Tile<BN>::kCtas)
       }
       fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&acc_empty[acc]));
+      if (lane == 0) {
+        if constexpr (PAIR)
+          mbar_arrive_first(smem_u32(&acc_empty[acc]));
+        else
+          mbar_arrive(smem_u32(&acc_empty[acc]));
+      }
     }
   }
   __syncthreads();
+  if constexpr (PAIR) cluster_barrier();  // neither CTA's memory is in use by the other
   if (warp == 1) {
+    __syncwarp();
     fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(C::kTmem) : "memory");
+    if constexpr (PAIR)
+      asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(C::kTmem) : "memory");
+    else
+      asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(C::kTmem) : "memory");
   }
 }
 
@@ -792,32 +1062,27 @@ struct FewPlan {
   int share;    // rows a CTA of the cluster writes
 };
 
-__device__ __forceinline__ void cluster_barrier() {
-  asm volatile("barrier.cluster.arrive.release;\n barrier.cluster.wait.acquire;" ::: "memory");
-}
-
 // The adapters' share of rows [t0, t0 + N) in one column, into sums[t - t0][128].
 template <bool F16, int N>
 __device__ __forceinline__ void few_dots(const nnb_project_args& a, int parts, int t0, int end, int col, int r,
-                                         float* values, volatile int* adapters, float* sums) {
+                                         float* values, const volatile int* adapters, float* sums) {
   constexpr int kPlanes = F16 ? 2 : 1;
   float acc[N] = {};
   for (int j0 = 0; j0 < a.rank; j0 += kFewRanks) {
     const int fours = min(kFewRanks, a.rank - j0) / 4;
     adapter_barrier(true);  // the values of the block before have been read
-    if (r < N) adapters[r] = t0 + r < end ? row_adapter(a, t0 + r) : -1;
     for (int i = r; i < N * fours; i += 128) {
       const int t = i / fours, j = (i - t * fours) * 4;
-      const bool some = t0 + t < end && row_adapter(a, t0 + t) >= 0;
+      const bool some = t0 + t < end && adapters[t] >= 0;
       *reinterpret_cast<float4*>(values + t * kFewRanks + j) =
           some ? low_values(a, parts, t0 + t, j0 + j) : make_float4(0.f, 0.f, 0.f, 0.f);
     }
     adapter_barrier(true);
     const __nv_bfloat16* up[N];
 #pragma unroll
-    for (int t = 0; t < N; ++t)  // a row without adapter multiplies zeros
+    for (int t = 0; t < N; ++t)  // a row without adapter, or past the share, multiplies zeros
       up[t] = reinterpret_cast<const __nv_bfloat16*>(a.up) +
-              ((int64_t)max(adapters[t], 0) * a.n + col) * kPlanes * a.rank + j0;
+              ((int64_t)max(t0 + t < end ? adapters[t] : 0, 0) * a.n + col) * kPlanes * a.rank + j0;
     for (int j = 0; j < fours * 4; j += 8) {
       uint4 raw[N], rest[F16 ? N : 1];
 #pragma unroll
@@ -864,7 +1129,7 @@ __global__ void __launch_bounds__(kFewThreads, 2)
   uint64_t* acc_full = empty + S;
   uint64_t* drain = acc_full + 1;
   volatile int* adapters = reinterpret_cast<volatile int*>(drain + 1);
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(const_cast<int*>(adapters + 16));
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(const_cast<int*>(adapters + BM));
   int* abort_flag = reinterpret_cast<int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -912,46 +1177,53 @@ __global__ void __launch_bounds__(kFewThreads, 2)
     }
     __syncwarp();
   } else if (warp == 1) {
-    if (lane == 0) {
-      const uint32_t idesc = kF16 ? idesc_f16(BM, plan.columns) : idesc_bf16(BM, plan.columns);
-      int s = 0;
-      uint32_t phase = 0, accumulate = 0;
-      bool alive = true;
-      for (int c = first; c < last; ++c) {
-        if (!mbar_wait(smem_u32(&full[s]), phase, abort_flag, 61)) {
-          alive = false;
-          break;
-        }
-        fence_after();
-        const uint32_t at = smem_u32(stages + s * stage);
-        const uint64_t ad = sw128_desc(at), bd = sw128_desc(at + BM * 128);
-        const int steps = min(4, (a.k - c * 64 + 15) / 16);
-        for (int k = 0; k < steps; ++k) {
-          mma_f16(tmem, ad + k * 2, bd + k * 2, idesc, accumulate);
-          accumulate = 1;
-        }
+    const uint32_t idesc = kF16 ? idesc_f16(BM, plan.columns) : idesc_bf16(BM, plan.columns);
+    const bool issuer = elect_one();
+    int s = 0;
+    uint32_t phase = 0;
+    bool alive = true;
+    for (int c = first; c < last; ++c) {
+      alive = __all_sync(0xffffffffu, mbar_wait(smem_u32(&full[s]), phase, abort_flag, 61));
+      if (!alive) break;
+      fence_after();
+      const uint32_t at = smem_u32(stages + s * stage);
+      if (issuer) {
+        chunk_mmas<false>(tmem, sw128_desc(at), sw128_desc(at + BM * 128), idesc, min(4, (a.k - c * 64 + 15) / 16),
+                          c > first);
         mma_commit(smem_u32(&empty[s]));
-        if (++s == S) s = 0, phase ^= 1u;
       }
-      if (alive) mma_commit(smem_u32(acc_full));
-      if (*reinterpret_cast<volatile int*>(abort_flag)) {
-        mma_commit(smem_u32(drain));
-        mbar_wait(smem_u32(drain), 0, abort_flag, 62, false);
-      }
+      __syncwarp();
+      if (++s == S) s = 0, phase ^= 1u;
+    }
+    if (alive && issuer) mma_commit(smem_u32(acc_full));
+    if (issuer && *reinterpret_cast<volatile int*>(abort_flag)) {
+      mma_commit(smem_u32(drain));
+      mbar_wait(smem_u32(drain), 0, abort_flag, 62, false);
     }
     __syncwarp();
   }
   const int r = threadIdx.x - 64, col = n0 + r;
   const int begin = part * plan.share, end = min((int)a.rows, begin + plan.share);
   if (warp >= 2) {
+    // the share's adapters, and their up rows on the way to L2, before the low-rank rows are there
+    if (begin + r < end) adapters[r] = row_adapter(a, begin + r);
+    adapter_barrier(true);
+    const int bytes = a.rank * (kF16 ? 4 : 2);
+    for (int t = begin; t < end; ++t) {
+      const int adapter = adapters[t - begin];
+      if (adapter < 0 || col >= a.n) continue;
+      const uint8_t* row = reinterpret_cast<const uint8_t*>(a.up) + ((int64_t)adapter * a.n + col) * bytes;
+      for (int b = 0; b < bytes; b += 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(row + b));
+    }
     // the low-rank rows are the previous kernel's, which may still run; every CTA waits for its end
     asm volatile("griddepcontrol.wait;" ::: "memory");
     for (int t = begin; t < end; t += 16) {
       float* to = sums + (t - begin) * BM;
+      const volatile int* of = adapters + (t - begin);
       if (end - t <= 4)
-        few_dots<kF16, 4>(a, plan.parts, t, end, min(col, a.n - 1), r, values, adapters, to);
+        few_dots<kF16, 4>(a, plan.parts, t, end, min(col, a.n - 1), r, values, of, to);
       else
-        few_dots<kF16, 16>(a, plan.parts, t, end, min(col, a.n - 1), r, values, adapters, to);
+        few_dots<kF16, 16>(a, plan.parts, t, end, min(col, a.n - 1), r, values, of, to);
     }
     const bool ok = mbar_wait(smem_u32(acc_full), 0, abort_flag, 63);
     if (__all_sync(0xffffffffu, ok)) {
@@ -976,7 +1248,7 @@ __global__ void __launch_bounds__(kFewThreads, 2)
       asm("mapa.shared::cluster.u32 %0, %1, %2;"
           : "=r"(peer[c])
           : "r"(smem_u32(partial) + r * 4), "r"(c < plan.split ? c : 0));
-#pragma unroll 2
+#pragma unroll 4
     for (int t = begin; t < end; ++t) {
       float v[8];
 #pragma unroll
@@ -1041,27 +1313,32 @@ bool narrow(const nnb_project_args& a) { return a.k <= 128 && a.n <= 128; }
 // How the low-rank rows are computed: by tiles or by rows, in how many parts of the channels.
 struct LowPlan {
   bool few;   // up to one tile of rows
-  int parts;  // partial sums
+  int parts;  // partial sums (few), or CTAs of a cluster
   int part;   // channels (few) or chunks of 64 of a part
 };
 
 // Enough parts that some 300 CTAs run (two per SM), of at least 512 channels (four loads of a lane) or four
-// chunks, and no more than eight, which their readers add up.
+// chunks, and no more than eight.
 LowPlan low_plan(const nnb_project_args& a) {
   LowPlan p;
   p.few = a.rows <= BM;
   const int64_t units = p.few ? a.rows * (a.rank / 16) : (a.rows + BM - 1) / BM;
   const int total = p.few ? a.k : (a.k + 63) / 64, least = p.few ? 512 : 4;
-  const int wanted = (int)std::min<int64_t>(8, std::max<int64_t>(1, 300 / units));
-  const int parts = std::max(1, std::min(wanted, total / least));
-  p.part = (total + parts - 1) / parts;
-  if (p.few) p.part = (p.part + 255) / 256 * 256;  // whole loads of a warp
-  p.parts = (total + p.part - 1) / p.part;
+  p.parts = 1;
+  while (p.parts < 8 && total / (p.parts * 2) >= least && units * p.parts * 2 <= 320) p.parts *= 2;
+  p.part = (total + p.parts - 1) / p.parts;
+  if (p.few) {
+    p.part = (p.part + 255) / 256 * 256;  // whole loads of a warp
+    p.parts = (total + p.part - 1) / p.part;
+  }
   return p;
 }
 
 int64_t low_bytes(const nnb_project_args& a) {
-  return narrow(a) ? 0 : low_plan(a).parts * a.rows * a.rank * (int64_t)sizeof(float);
+  if (narrow(a)) return 0;
+  const LowPlan p = low_plan(a);
+  return p.few ? p.parts * a.rows * a.rank * (int64_t)sizeof(float)
+               : a.rows * ((a.rank + kRankBlock - 1) / kRankBlock) * 128;
 }
 
 // A GEMM kernel's launch while the low-rank kernel before it still runs: only the warps that read its rows wait
@@ -1107,21 +1384,33 @@ int launch_low(const nnb_project_args& a, const LowPlan& plan, int dev, cudaStre
     NNB_LAUNCH_CHECK();
     return NNB_OK;
   }
+  LowTilePlan tile = low_tile_plan(a.rank);
+  tile.part = plan.part;
   static bool configured[64] = {false};
   if (dev >= 64 || !configured[dev]) {
     NNB_CUDA_CHECK(
-        cudaFuncSetAttribute(project_low_tile_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kLowSmem));
+        cudaFuncSetAttribute(project_low_tile_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem));
     if (dev < 64) configured[dev] = true;
   }
+  NNB_REQUIRE(tile.smem <= kMaxSmem, "project: internal: plan exceeds shared memory (%d bytes)", tile.smem);
   LowMaps maps;
   if (const int rc = encode_rows(&maps.x, kF16, a, BM)) return rc;
   const cuuint64_t dims[3] = {(cuuint64_t)a.k, (cuuint64_t)a.rank, (cuuint64_t)a.adapters};
   const cuuint64_t strides[2] = {(cuuint64_t)a.weight_stride * 2, (cuuint64_t)a.weight_stride * 2 * a.rank};
-  const cuuint32_t box[3] = {64, (cuuint32_t)std::min(a.rank, kLowColumns), 1};
+  const cuuint32_t box[3] = {64, (cuuint32_t)std::min(a.rank, tile.columns), 1};
   if (const int rc = encode(&maps.down, kF16, 3, a.down, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B)) return rc;
-  const dim3 grid((unsigned)((a.rows + BM - 1) / BM), plan.parts);
-  project_low_tile_kernel<T><<<grid, kLowThreads, kLowSmem, stream>>>(a, maps, plan.part);
-  NNB_LAUNCH_CHECK();
+  cudaLaunchAttribute cluster[1];
+  cluster[0].id = cudaLaunchAttributeClusterDimension;
+  cluster[0].val.clusterDim.x = cluster[0].val.clusterDim.z = 1;
+  cluster[0].val.clusterDim.y = plan.parts;
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3((unsigned)((a.rows + BM - 1) / BM), plan.parts);
+  config.blockDim = dim3(kLowThreads);
+  config.dynamicSmemBytes = tile.smem;
+  config.stream = stream;
+  config.attrs = cluster;
+  config.numAttrs = 1;
+  NNB_CUDA_CHECK(cudaLaunchKernelEx(&config, project_low_tile_kernel<T>, a, maps, tile));
   return NNB_OK;
 }
 
@@ -1136,7 +1425,7 @@ int launch_few(const nnb_project_args& a, const LowPlan& low, int sms, int dev, 
   while (plan.split < 8 && plan.split * 2 <= chunks && tiles * plan.split * 2 <= 2 * sms) plan.split *= 2;
   plan.share = ((int)a.rows + plan.split - 1) / plan.split;
   const int stage = BM * 128 + plan.columns * 128;
-  const int fixed = 1024 + plan.share * BM * 4 + 16 * kFewRanks * 4 + 512;
+  const int fixed = 1024 + plan.share * BM * 4 + 16 * kFewRanks * 4 + 1024;
   // stages for two CTAs an SM, but room for the partial sums ([rows][128] floats over the stages) and at least two
   plan.stages = std::max(2, std::min({8, (112 * 1024 - fixed) / stage, (chunks + plan.split - 1) / plan.split}));
   while (plan.stages * stage < (int)a.rows * BM * 4) ++plan.stages;
@@ -1153,44 +1442,46 @@ int launch_few(const nnb_project_args& a, const LowPlan& low, int sms, int dev, 
   return launch_early(project_few_kernel<T>, tiles * plan.split, kFewThreads, smem, plan.split, stream, a, maps, plan);
 }
 
-template <typename T, int BN>
-int launch_tiles(const nnb_project_args& a, const LowPlan& plan, int sms, int dev, cudaStream_t stream) {
-  using C = Tile<BN>;
+template <typename T, int BN, bool PAIR>
+int launch_tiles(const nnb_project_args& a, int sms, int dev, cudaStream_t stream) {
+  using C = Tile<T, BN, PAIR>;
   constexpr bool kF16 = !std::is_same<T, __nv_bfloat16>::value;
   static bool configured[64] = {false};
   if (dev >= 64 || !configured[dev]) {
     NNB_CUDA_CHECK(
-        cudaFuncSetAttribute(project_kernel<T, BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
+        cudaFuncSetAttribute(project_kernel<T, BN, PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
     if (dev < 64) configured[dev] = true;
   }
-  static_assert(C::kSmem * C::kCtas <= kMaxSmem + 1024 * (C::kCtas - 1), "the tile's stages exceed shared memory");
+  static_assert(C::kSmem <= kMaxSmem, "the tile's stages exceed shared memory");
   Maps maps;
   if (const int rc = encode_rows(&maps.x, kF16, a, BM)) return rc;
-  if (const int rc = encode_weight(&maps.weight, kF16, a, BN)) return rc;
+  if (const int rc = encode_weight(&maps.weight, kF16, a, BN / C::kPeers)) return rc;
   {
     const cuuint64_t width = (cuuint64_t)a.rank * (kF16 ? 2 : 1);
     const cuuint64_t dims[3] = {width, (cuuint64_t)a.n, (cuuint64_t)a.adapters};
     const cuuint64_t strides[2] = {width * 2, width * 2 * (cuuint64_t)a.n};
-    const cuuint32_t box[3] = {kRankBlock, BN, 1};
+    const cuuint32_t box[3] = {kRankBlock, BN / C::kPeers, 1};
     if (const int rc = encode(&maps.up, false, 3, a.up, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_64B)) return rc;
   }
-  const int64_t tiles = (a.rows + BM - 1) / BM * ((a.n + BN - 1) / BN);
-  const int grid = (int)std::min<int64_t>(tiles, (int64_t)sms * C::kCtas);
-  return launch_early(project_kernel<T, BN>, grid, kThreads, C::kSmem, 1, stream, a, maps, plan.parts);
+  const int64_t tiles = (a.rows + C::kRows - 1) / C::kRows * ((a.n + BN - 1) / BN);
+  NNB_REQUIRE(tiles < (int64_t)1 << 30, "project: %lld tiles", (long long)tiles);
+  const int grid = (int)std::min<int64_t>(tiles, (int64_t)sms / C::kPeers) * C::kPeers;
+  return launch_early(project_kernel<T, BN, PAIR>, grid, kThreads, C::kSmem, C::kPeers, stream, a, maps);
 }
 
-// Tile width: the one whose waves of tiles take least, a tile's time being the larger of its MMAs' and its
-// loads' (cycles per 64 channels), plus a fixed start and epilogue.
+// Tile width: the one whose waves of tiles take least, by the time of a tile measured on B200 with every SM busy:
+// so many ns per chunk of 64 channels, and so many beside them.  (8192 rows, 4096 columns, 4096 channels: width 64
+// 425 us, 128 289 us, pairs of 256 203 us; 8192 x 160 columns: 46.5, 35.6 and 39.3 us.)
 int tile_columns(const nnb_project_args& a, int sms) {
-  const int widths[4] = {32, 64, 128, 256};
-  const int chunk_cycles[4] = {320, 384, 512, 768};
-  int best = 32;
+  struct { int width, rows, ctas, chunk, fixed; } const kinds[3] = {
+      {64, BM, sms, 237, 2100}, {128, BM, sms, 323, 2350}, {256, 2 * BM, sms / 2, 450, 3950}};
+  int best = 64;
   int64_t least = INT64_MAX;
-  for (int i = 0; i < 4; ++i) {
-    const int64_t tiles = (a.rows + BM - 1) / BM * ((a.n + widths[i] - 1) / widths[i]);
-    const int64_t waves = (tiles + sms - 1) / sms;
-    const int64_t cost = waves * (chunk_cycles[i] * (int64_t)((a.k + 63) / 64) + 2 * widths[i]) + 2000;
-    if (cost < least) least = cost, best = widths[i];
+  for (const auto& kind : kinds) {
+    const int64_t tiles = (a.rows + kind.rows - 1) / kind.rows * ((a.n + kind.width - 1) / kind.width);
+    const int64_t waves = (tiles + kind.ctas - 1) / kind.ctas;
+    const int64_t cost = waves * (kind.chunk * (int64_t)((a.k + 63) / 64) + kind.fixed);
+    if (cost < least) least = cost, best = kind.width;
   }
   return best;
 }
@@ -1330,10 +1621,7 @@ __global__ void __launch_bounds__(kNarrowThreads, 2) project_narrow_kernel(const
             for (int h = 0; h < 2; ++h) {
               const bool own = mine[m][h] == listed;
               const float v0 = own ? low[m][t][h * 2] * scale : 0.f, v1 = own ? low[m][t][h * 2 + 1] * scale : 0.f;
-              const float h0 = __bfloat162float(__float2bfloat16_rn(v0));
-              const float h1 = __bfloat162float(__float2bfloat16_rn(v1));
-              hi[m][t * 2 + h] = pack2(h0, h1, __nv_bfloat16());
-              lo[m][t * 2 + h] = pack2(isfinite(h0) ? v0 - h0 : 0.f, isfinite(h1) ? v1 - h1 : 0.f, __nv_bfloat16());
+              split2(v0, v1, hi[m][t * 2 + h], lo[m][t * 2 + h]);
             }
 #pragma unroll
         for (int t = 0; t < NN * 4; ++t) {
@@ -1438,10 +1726,9 @@ int launch_project(nnb_project_args a, cudaStream_t stream) {
   if (const int rc = launch_low<T>(a, plan, dev, stream)) return rc;
   if (plan.few) return launch_few<T>(a, plan, sms, dev, stream);
   switch (tile_columns(a, sms)) {
-    case 32: return launch_tiles<T, 32>(a, plan, sms, dev, stream);
-    case 64: return launch_tiles<T, 64>(a, plan, sms, dev, stream);
-    case 128: return launch_tiles<T, 128>(a, plan, sms, dev, stream);
-    default: return launch_tiles<T, 256>(a, plan, sms, dev, stream);
+    case 64: return launch_tiles<T, 64, false>(a, sms, dev, stream);
+    case 128: return launch_tiles<T, 128, false>(a, sms, dev, stream);
+    default: return launch_tiles<T, 256, true>(a, sms, dev, stream);
   }
 }
 

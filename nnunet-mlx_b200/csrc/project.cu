@@ -421,11 +421,12 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, float (&v)[16]) {
   for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
 }
 
-// Two low-rank values as two bfloat16 parts each, hi + lo.  What an infinity leaves would be no number.
+// Two low-rank values as two bfloat16 parts each, hi + lo.  What an infinity leaves would be no number: the larger
+// of it and a bound below every true remainder (half a step of the largest value is 2^119) is that bound.
 __device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t& lo) {
-  const float ha = __bfloat162float(__float2bfloat16_rn(a)), hb = __bfloat162float(__float2bfloat16_rn(b));
-  hi = pack2(ha, hb, __nv_bfloat16());
-  lo = pack2(isfinite(ha) ? a - ha : 0.f, isfinite(hb) ? b - hb : 0.f, __nv_bfloat16());
+  hi = pack2(a, b, __nv_bfloat16());
+  lo = pack2(a - __uint_as_float(hi << 16), b - __uint_as_float(hi & 0xffff0000u), __nv_bfloat16());
+  asm("max.bf16x2 %0, %0, %1;" : "+r"(lo) : "r"(0xfb80fb80u));  // -2^120
 }
 
 // ---------------------------------------------------------------------------
@@ -964,7 +965,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint32_t src = tmem + acc * BN + ((uint32_t)quarter << 21);
       const int64_t row0 = t.row0 + cta * BM + quarter * 32;
       const int live = (int)min((int64_t)32, a.rows - row0), columns = min(BN, a.n - t.col0);
-      const bool whole = vector && live == 32 && columns == BN;
       T* out = reinterpret_cast<T*>(a.out) + (row0 + at_row) * a.out_stride + t.col0 + chunk * 8;
       const int64_t eight = 8 * a.out_stride;
       uint32_t raw[32];
@@ -987,30 +987,21 @@ __global__ void __launch_bounds__(kThreads, 1)
                                             pack2(v[c * 8 + 6] + b1.z, v[c * 8 + 7] + b1.w, T()));
         }
         __syncwarp();
-        uint4 packed[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int r = i * 8 + at_row;
-          packed[i] = reinterpret_cast<const uint4*>(stage_rows + r * 64)[place(r, chunk)];
-        }
-        if (whole) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4*>(out + i * eight) = packed[i];
-        } else {
-          const int col = c0 + chunk * 8;
+        if (vector && c0 + 32 <= columns) {
+          uint4 packed[4];
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            if (i * 8 + at_row >= live || col >= columns) continue;
-            T* to = out + i * eight;
-            if (vector && col + 8 <= columns) {
-              *reinterpret_cast<uint4*>(to) = packed[i];
-            } else {
-              const T* values = reinterpret_cast<const T*>(&packed[i]);
-#pragma unroll
-              for (int j = 0; j < 8; ++j)
-                if (col + j < columns) to[j] = values[j];
-            }
+            const int r = i * 8 + at_row;
+            packed[i] = reinterpret_cast<const uint4*>(stage_rows + r * 64)[place(r, chunk)];
           }
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (i * 8 + at_row < live) *reinterpret_cast<uint4*>(out + i * eight) = packed[i];
+        } else if (c0 + lane < columns) {  // a store covers 64 bytes of one row
+          T* to = reinterpret_cast<T*>(a.out) + row0 * a.out_stride + t.col0 + c0 + lane;
+#pragma unroll 8
+          for (int r = 0; r < live; ++r, to += a.out_stride)
+            *to = reinterpret_cast<const T*>(stage_rows + r * 64 + place(r, lane >> 3) * 16)[lane & 7];
         }
         __syncwarp();
       }
@@ -1499,20 +1490,24 @@ int tile_columns(const nnb_project_args& a, int sms) {
 // warp's rows.  The tensor rate is no bound here (some 20 operations per byte),
 // so the plain warp MMAs serve, and no stage or barrier stands between x and out.
 // ---------------------------------------------------------------------------
-__device__ __forceinline__ void warp_mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1,
-                                         __nv_bfloat16) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
-      "{%0, %1, %2, %3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+// d = a b + c of 16 rows, 8 columns and 16 channels.
+__device__ __forceinline__ void warp_mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, float c0,
+                                         float c1, float c2, float c3, __nv_bfloat16) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%10, %11, %12, %13};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
 }
-__device__ __forceinline__ void warp_mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, __half) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
-      "{%0, %1, %2, %3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+__device__ __forceinline__ void warp_mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, float c0,
+                                         float c1, float c2, float c3, __half) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%10, %11, %12, %13};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
+}
+template <typename T>
+__device__ __forceinline__ void warp_mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, T type) {
+  warp_mma(d, a, b0, b1, d[0], d[1], d[2], d[3], type);
 }
 
 // Eight channels of a row from column k on; zero from column `width` on.
@@ -1529,163 +1524,333 @@ __device__ __forceinline__ uint4 row_chunk(const T* row, int k, int width) {
 
 constexpr int kNarrowThreads = 256;
 
-// NK, NN: groups of 32 channels and columns; M: 16-row fragments per warp.
-template <typename T, int NK, int NN, int M>
+// NK, NN: groups of 32 channels and columns; M: 16-row fragments per warp; RUNS: an index covers so many rows that a
+// warp's have one adapter or two.
+template <typename T, int NK, int NN, int M, bool RUNS>
 __global__ void __launch_bounds__(kNarrowThreads, 2) project_narrow_kernel(const nnb_project_args a) {
   constexpr bool kF16 = !std::is_same<T, __nv_bfloat16>::value;
   constexpr int kPitch = 4 * (NK | 1);  // 16-byte chunks of a W row in shared memory: neighbouring rows 64 bytes
                                         // apart modulo the banks' 128
+  constexpr int kRows = 16 * M;
+  // One group of either: fragments of W, and of an adapter of 16 ranks, stay in registers between tiles.
+  constexpr bool kHold = NK * NN == 1;
+  constexpr bool kAhead = kHold && RUNS;  // the next tile's loads early, where registers allow
   __shared__ uint4 weight[NN * 32 * kPitch];
-  __shared__ float bias[NN * 32];
+  __shared__ float2 bias[NN * 16];
+  __shared__ uint4 staging[kNarrowThreads / 32][32];  // 8 rows of 32 columns, for rows that are not aligned
   for (int i = threadIdx.x; i < NN * 32 * NK * 4; i += kNarrowThreads) {
     const int n = i / (NK * 4), c = i % (NK * 4);
     weight[n * kPitch + c] =
         n < a.n ? row_chunk(reinterpret_cast<const T*>(a.weight) + n * a.weight_stride, c * 8, (int)a.weight_stride)
                 : make_uint4(0, 0, 0, 0);
   }
-  for (int i = threadIdx.x; i < NN * 32; i += kNarrowThreads) bias[i] = a.bias != nullptr && i < a.n ? a.bias[i] : 0.f;
+  for (int i = threadIdx.x; i < NN * 32; i += kNarrowThreads)
+    reinterpret_cast<float*>(bias)[i] = a.bias != nullptr && i < a.n ? a.bias[i] : 0.f;
   __syncthreads();
 
   const int lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
   const int spread = (g >> 1) * 8 + (g & 1);  // of 32 columns, the one of B fragment row g of tile 0; tile j: + 2 j
   const bool vector = reinterpret_cast<uintptr_t>(a.out) % 16 == 0 && (a.rows == 1 || a.out_stride % 8 == 0);
-  const int64_t step = (int64_t)gridDim.x * (kNarrowThreads / 32) * 16 * M;
-  for (int64_t row0 = ((int64_t)blockIdx.x * (kNarrowThreads / 32) + (threadIdx.x >> 5)) * 16 * M; row0 < a.rows;
-       row0 += step) {
-    // A fragments of x: of each 32 channels, words 0-1 are the first K-step's and 2-3 the second's
-    uint4 x[M][2][NK];
-    int mine[M][2];
-#pragma unroll
-    for (int m = 0; m < M; ++m)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int64_t row = row0 + m * 16 + h * 8 + g;
-        const bool live = row < a.rows;
-#pragma unroll
-        for (int c = 0; c < NK; ++c)
-          x[m][h][c] = live ? row_chunk(reinterpret_cast<const T*>(a.x) + row * a.x_stride, c * 32 + q * 8, a.k)
-                            : make_uint4(0, 0, 0, 0);
-        mine[m][h] = live ? row_adapter(a, row) : -1;
-      }
-    float acc[M][NN * 4][4] = {};
-#pragma unroll
-    for (int c = 0; c < NK; ++c)
-#pragma unroll
-      for (int t = 0; t < NN * 4; ++t) {
-        const uint4 w = weight[((t >> 2) * 32 + spread + (t & 3) * 2) * kPitch + c * 4 + q];
-#pragma unroll
-        for (int m = 0; m < M; ++m) {
-          const uint4 &u = x[m][0][c], &v = x[m][1][c];
-          const uint32_t first[4] = {u.x, v.x, u.y, v.y}, second[4] = {u.z, v.z, u.w, v.w};
-          warp_mma(acc[m][t], first, w.x, w.y, T());
-          warp_mma(acc[m][t], second, w.z, w.w, T());
-        }
-      }
-    int listed = -1;
-    for (;;) {
-      int least = INT_MAX;
+  const bool whole_k = a.k == NK * 32, whole_n = vector && a.n == NN * 32;
+  const int rows = (int)a.rows, per_index = (int)a.rows_per_index;  // below 2^31
+  const int64_t step = (int64_t)gridDim.x * (kNarrowThreads / 32) * kRows;
+  const int64_t x_eight = 8 * a.x_stride, out_eight = 8 * a.out_stride;
+
+  // A fragments of x: of each 32 channels, words 0-1 are the first K-step's and 2-3 the second's
+  uint4 x[M][2][NK];
+  int index[M][2];      // not RUNS
+  int64_t run_end = 0;  // RUNS: where the rows of adapter `first` end; those behind have `second`
+  int first = -1, second = -1;
+  auto load = [&](uint4 (&to)[M][2][NK], int64_t row0) {
+    const T* src = reinterpret_cast<const T*>(a.x) + (row0 + g) * a.x_stride + q * 8;
+    if (whole_k && row0 + kRows <= rows) {
 #pragma unroll
       for (int m = 0; m < M; ++m)
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
-          if (mine[m][h] > listed) least = min(least, mine[m][h]);
-      listed = __reduce_min_sync(0xffffffffu, least);
-      if (listed == INT_MAX) break;
-      const float scale = __ldg(a.scales + listed);
-      const T* down = reinterpret_cast<const T*>(a.down) + (int64_t)listed * a.rank * a.weight_stride;
-      const __nv_bfloat16* up =
-          reinterpret_cast<const __nv_bfloat16*>(a.up) + (int64_t)listed * a.n * a.rank * (kF16 ? 2 : 1);
-      for (int j0 = 0; j0 < a.rank; j0 += 16) {
-        float low[M][2][4] = {};
+        for (int h = 0; h < 2; ++h, src += x_eight)
 #pragma unroll
-        for (int c = 0; c < NK; ++c)
+          for (int c = 0; c < NK; ++c) to[m][h][c] = *reinterpret_cast<const uint4*>(src + c * 32);
+    } else {
+#pragma unroll
+      for (int m = 0; m < M; ++m)
+#pragma unroll
+        for (int h = 0; h < 2; ++h, src += x_eight)
+#pragma unroll
+          for (int c = 0; c < NK; ++c)
+            to[m][h][c] = row0 + m * 16 + h * 8 + g < rows ? row_chunk(src - q * 8, c * 32 + q * 8, a.k)
+                                                           : make_uint4(0, 0, 0, 0);
+    }
+    if constexpr (!RUNS) {
+#pragma unroll
+      for (int m = 0; m < M; ++m)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int64_t row = row0 + m * 16 + h * 8 + g;
+          index[m][h] = row < rows ? row_index(a, row) : -1;
+        }
+    }
+  };
+
+  // B fragments: W's of one group of channels and tile, and of 16 ranks down's rows and up's columns.  (asm, and
+  // strides that the compiler cannot see through, lest it keep all of them or their addresses in registers.)
+  const uint32_t weight_at = smem_u32(weight + spread * kPitch + q);
+  auto weights = [&](int c, int t) {
+    uint4 w;
+    if constexpr (kHold)
+      w = weight[spread * kPitch + q + ((t >> 2) * 32 + (t & 3) * 2) * kPitch + c * 4];
+    else
+      asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                   : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w)
+                   : "r"(weight_at + (((t >> 2) * 32 + (t & 3) * 2) * kPitch + c * 4) * 16));
+    return w;
+  };
+  auto down_rows = [&](const T* src, int stride, int c, int t) {
+    return c * 32 + q * 8 < a.weight_stride
+               ? __ldg(reinterpret_cast<const uint4*>(src + (uint32_t)(t * 2 * stride + c * 32)))
+               : make_uint4(0, 0, 0, 0);
+  };
+  auto up_columns = [&](const __nv_bfloat16* src, int width, int t) {
+    const int col = min((t >> 2) * 32 + (t & 3) * 2, a.n - 1 - spread);  // columns past n are not stored
+    return __ldg(reinterpret_cast<const uint2*>(src + col * width));
+  };
+  uint4 held_down[kHold ? 2 : 1];
+  uint2 held_up[kHold ? 4 : 1], held_rest[kHold && kF16 ? 4 : 1];
+  int held = -1;
+
+  int64_t row0 = ((int64_t)blockIdx.x * (kNarrowThreads / 32) + (threadIdx.x >> 5)) * kRows;
+  if (row0 >= rows) return;
+  load(x, row0);
+  for (; row0 < rows; row0 += step) {
+    int mine[M][2];
+    int border = kRows;  // RUNS: the tile's rows from here on have `second`
+    if constexpr (RUNS) {
+      if (row0 + kRows > run_end) {  // (the first tile's, and where a run ends)
+        const int sample = (uint32_t)row0 / (uint32_t)per_index;
+        run_end = (int64_t)(sample + 1) * per_index;
+        first = checked_adapter(a, __ldg(a.index + sample));
+        second = run_end < rows && run_end < row0 + kRows ? checked_adapter(a, __ldg(a.index + sample + 1)) : -1;
+        if (run_end < row0 + kRows) border = (int)(run_end - row0);
+        if (second == first) border = kRows;
+      }
+    } else {
+#pragma unroll
+      for (int m = 0; m < M; ++m)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) mine[m][h] = checked_adapter(a, index[m][h]);
+    }
+    uint4 ahead[M][2][NK];
+    if (kAhead && row0 + step < rows) load(ahead, row0 + step);  // on its way while this tile's products are taken
+
+    // (MMAs into different accumulators follow one another: one into the same waits for the one before)
+    float acc[M][NN * 4][4];
+#pragma unroll
+    for (int c = 0; c < NK; ++c)
+#pragma unroll
+      for (int p = 0; p < NN; ++p) {
+        uint4 w[4];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) w[t] = weights(c, p * 4 + t);
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          const float2 b = c == 0 ? bias[p * 16 + q * 4 + t] : make_float2(0.f, 0.f);
+#pragma unroll
+          for (int m = 0; m < M; ++m) {
+            const uint32_t one[4] = {x[m][0][c].x, x[m][1][c].x, x[m][0][c].y, x[m][1][c].y};
+            if (c == 0)
+              warp_mma(acc[m][p * 4 + t], one, w[t].x, w[t].y, b.x, b.y, b.x, b.y, T());
+            else
+              warp_mma(acc[m][p * 4 + t], one, w[t].x, w[t].y, T());
+          }
+        }
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+          for (int m = 0; m < M; ++m) {
+            const uint32_t two[4] = {x[m][0][c].z, x[m][1][c].z, x[m][0][c].w, x[m][1][c].w};
+            warp_mma(acc[m][p * 4 + t], two, w[t].z, w[t].w, T());
+          }
+      }
+    int listed = -1;
+#pragma unroll 1
+    for (int turn = 0;; ++turn) {
+      if constexpr (RUNS) {
+        if (turn == 2) break;
+        listed = turn == 0 ? first : border < kRows ? second : -1;
+        if (listed < 0) continue;
+      } else {
+        int least = INT_MAX;
+#pragma unroll
+        for (int m = 0; m < M; ++m)
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+            if (mine[m][h] > listed) least = min(least, mine[m][h]);
+        listed = __reduce_min_sync(0xffffffffu, least);
+        if (listed == INT_MAX) break;
+      }
+      const bool mixed = !RUNS || border < kRows;  // else every row is the adapter's
+      const float scale = __ldg(a.scales + listed);
+#pragma unroll 1
+      for (int j0 = 0; j0 < a.rank; j0 += 16) {
+        int down_stride = (int)a.weight_stride, up_width = a.rank * (kF16 ? 2 : 1);
+        if constexpr (!kHold) asm volatile("" : "+r"(down_stride), "+r"(up_width));
+        const T* down = reinterpret_cast<const T*>(a.down) +
+                        ((int64_t)listed * a.rank + j0 + (g >> 1) * 4 + (g & 1)) * a.weight_stride + q * 8;
+        const __nv_bfloat16* up = reinterpret_cast<const __nv_bfloat16*>(a.up) +
+                                  ((int64_t)listed * a.n + spread) * up_width + j0 + q * 4;
+        if constexpr (kHold) {
+          if (held != listed || a.rank > 16) {
+#pragma unroll
+            for (int t = 0; t < 2; ++t) held_down[t] = down_rows(down, down_stride, 0, t);
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+              held_up[t] = up_columns(up, up_width, t);
+              if constexpr (kF16) held_rest[t] = up_columns(up + a.rank, up_width, t);
+            }
+            held = listed;
+          }
+        }
+        float low[M][2][4];
+#pragma unroll
+        for (int c = 0; c < NK; ++c) {
+          uint4 w[2];
 #pragma unroll
           for (int t = 0; t < 2; ++t) {
-            const int k = c * 32 + q * 8;
-            const T* src = down + (j0 + (g >> 1) * 4 + t * 2 + (g & 1)) * a.weight_stride + k;
-            const uint4 w = k < a.weight_stride ? __ldg(reinterpret_cast<const uint4*>(src)) : make_uint4(0, 0, 0, 0);
+            if constexpr (kHold)
+              w[t] = held_down[t];
+            else
+              w[t] = down_rows(down, down_stride, c, t);
+          }
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
 #pragma unroll
             for (int m = 0; m < M; ++m) {
-              const uint4 &u = x[m][0][c], &v = x[m][1][c];
-              const uint32_t first[4] = {u.x, v.x, u.y, v.y}, second[4] = {u.z, v.z, u.w, v.w};
-              warp_mma(low[m][t], first, w.x, w.y, T());
-              warp_mma(low[m][t], second, w.z, w.w, T());
+              const uint32_t one[4] = {x[m][0][c].x, x[m][1][c].x, x[m][0][c].y, x[m][1][c].y};
+              if (c == 0)
+                warp_mma(low[m][t], one, w[t].x, w[t].y, 0.f, 0.f, 0.f, 0.f, T());
+              else
+                warp_mma(low[m][t], one, w[t].x, w[t].y, T());
             }
-          }
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int m = 0; m < M; ++m) {
+              const uint32_t two[4] = {x[m][0][c].z, x[m][1][c].z, x[m][0][c].w, x[m][1][c].w};
+              warp_mma(low[m][t], two, w[t].z, w[t].w, T());
+            }
+        }
+        if (mixed) {
+#pragma unroll
+          for (int m = 0; m < M; ++m)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const bool own = RUNS ? (m * 16 + h * 8 + g < border) == (turn == 0) : mine[m][h] == listed;
+#pragma unroll
+              for (int t = 0; t < 2; ++t) {
+                low[m][t][h * 2] = own ? low[m][t][h * 2] : 0.f;
+                low[m][t][h * 2 + 1] = own ? low[m][t][h * 2 + 1] : 0.f;
+              }
+            }
+        }
         uint32_t hi[M][4], lo[M][4];
 #pragma unroll
         for (int m = 0; m < M; ++m)
 #pragma unroll
           for (int t = 0; t < 2; ++t)
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const bool own = mine[m][h] == listed;
-              const float v0 = own ? low[m][t][h * 2] * scale : 0.f, v1 = own ? low[m][t][h * 2 + 1] * scale : 0.f;
-              split2(v0, v1, hi[m][t * 2 + h], lo[m][t * 2 + h]);
+            for (int h = 0; h < 2; ++h)
+              split2(low[m][t][h * 2] * scale, low[m][t][h * 2 + 1] * scale, hi[m][t * 2 + h], lo[m][t * 2 + h]);
+#pragma unroll
+        for (int p = 0; p < NN; ++p) {
+          uint2 w[4], rest[kF16 ? 4 : 1];
+#pragma unroll
+          for (int t = 0; t < 4; ++t) {
+            if constexpr (kHold) {
+              w[t] = held_up[t];
+              if constexpr (kF16) rest[t] = held_rest[t];
+            } else {
+              w[t] = up_columns(up, up_width, p * 4 + t);
+              if constexpr (kF16) rest[t] = up_columns(up + a.rank, up_width, p * 4 + t);
             }
-#pragma unroll
-        for (int t = 0; t < NN * 4; ++t) {
-          const int col = min((t >> 2) * 32 + spread + (t & 3) * 2, a.n - 1);  // columns past n are not stored
-          const __nv_bfloat16* src = up + (int64_t)col * a.rank * (kF16 ? 2 : 1) + j0 + q * 4;
-          const uint2 w = __ldg(reinterpret_cast<const uint2*>(src));
-#pragma unroll
-          for (int m = 0; m < M; ++m) {
-            warp_mma(acc[m][t], hi[m], w.x, w.y, __nv_bfloat16());
-            warp_mma(acc[m][t], lo[m], w.x, w.y, __nv_bfloat16());
           }
-          if constexpr (kF16) {
-            const uint2 rest = __ldg(reinterpret_cast<const uint2*>(src + a.rank));
 #pragma unroll
-            for (int m = 0; m < M; ++m) warp_mma(acc[m][t], hi[m], rest.x, rest.y, __nv_bfloat16());
+          for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int m = 0; m < M; ++m) warp_mma(acc[m][p * 4 + t], hi[m], w[t].x, w[t].y, __nv_bfloat16());
+#pragma unroll
+          for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int m = 0; m < M; ++m) warp_mma(acc[m][p * 4 + t], lo[m], w[t].x, w[t].y, __nv_bfloat16());
+          if constexpr (kF16) {
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+#pragma unroll
+              for (int m = 0; m < M; ++m) warp_mma(acc[m][p * 4 + t], hi[m], rest[t].x, rest[t].y, __nv_bfloat16());
           }
         }
       }
     }
+    T* out = reinterpret_cast<T*>(a.out) + (row0 + g) * a.out_stride + q * 8;
+    const bool whole = whole_n && row0 + kRows <= rows;
 #pragma unroll
     for (int m = 0; m < M; ++m)
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int64_t row = row0 + m * 16 + h * 8 + g;
-        if (row >= a.rows) continue;
+      for (int h = 0; h < 2; ++h, out += out_eight)
 #pragma unroll
         for (int p = 0; p < NN; ++p) {
-          const int col = p * 32 + q * 8;
           uint4 packed;
           uint32_t* words = reinterpret_cast<uint32_t*>(&packed);
 #pragma unroll
-          for (int t = 0; t < 4; ++t)
-            words[t] = pack2(acc[m][p * 4 + t][h * 2] + bias[col + t * 2],
-                             acc[m][p * 4 + t][h * 2 + 1] + bias[col + t * 2 + 1], T());
-          T* out = reinterpret_cast<T*>(a.out) + row * a.out_stride + col;
-          if (vector && col + 8 <= a.n) {
-            *reinterpret_cast<uint4*>(out) = packed;
-          } else {
-            const T* values = reinterpret_cast<const T*>(&packed);
+          for (int t = 0; t < 4; ++t) words[t] = pack2(acc[m][p * 4 + t][h * 2], acc[m][p * 4 + t][h * 2 + 1], T());
+          if (whole) {
+            *reinterpret_cast<uint4*>(out + p * 32) = packed;
+          } else {  // rows through shared memory, so that a store covers 64 neighbouring bytes
+            uint4* stage = staging[threadIdx.x >> 5];
+            __syncwarp();
+            stage[g * 4 + q] = packed;
+            __syncwarp();
+            const int64_t first_row = row0 + m * 16 + h * 8;
+            T* to = reinterpret_cast<T*>(a.out) + first_row * a.out_stride + p * 32 + lane;
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-              if (col + j < a.n) out[j] = values[j];
+            for (int r = 0; r < 8; ++r)
+              if (first_row + r < rows && p * 32 + lane < a.n)
+                to[r * a.out_stride] = reinterpret_cast<const T*>(stage)[r * 32 + lane];
           }
         }
-      }
+    if constexpr (kAhead) {
+#pragma unroll
+      for (int m = 0; m < M; ++m)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int c = 0; c < NK; ++c) x[m][h][c] = ahead[m][h][c];
+    } else if (row0 + step < rows) {
+      load(x, row0 + step);
+    }
   }
 }
 
-template <typename T, int NK, int NN>
-int launch_narrow(const nnb_project_args& a, int sms, int dev, cudaStream_t stream) {
-  constexpr int M = NK <= 2 && NN <= 2 ? 2 : 1;  // a second fragment shares W's reads, as registers allow
+template <typename T, int NK, int NN, int M, bool RUNS>
+int launch_narrow_kernel(const nnb_project_args& a, int sms, int dev, cudaStream_t stream) {
   static int resident[64] = {0};
   int blocks = dev < 64 ? resident[dev] : 0;
   if (blocks == 0) {
-    NNB_CUDA_CHECK(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&blocks, project_narrow_kernel<T, NK, NN, M>,
+    NNB_CUDA_CHECK(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&blocks, project_narrow_kernel<T, NK, NN, M, RUNS>,
                                                                  kNarrowThreads, 0));
     blocks = std::max(1, blocks);
     if (dev < 64) resident[dev] = blocks;
   }
   const int64_t groups = (a.rows + kNarrowThreads / 2 * M - 1) / (kNarrowThreads / 2 * M);
-  project_narrow_kernel<T, NK, NN, M>
+  project_narrow_kernel<T, NK, NN, M, RUNS>
       <<<(unsigned)std::min<int64_t>(groups, (int64_t)blocks * sms), kNarrowThreads, 0, stream>>>(a);
   NNB_LAUNCH_CHECK();
   return NNB_OK;
+}
+
+template <typename T, int NK, int NN>
+int launch_narrow(const nnb_project_args& a, int sms, int dev, cudaStream_t stream) {
+  constexpr int M = NK * NN <= 2 ? 2 : 1;  // a second fragment shares W's reads, as registers allow
+  return a.rows_per_index >= 16 * M ? launch_narrow_kernel<T, NK, NN, M, true>(a, sms, dev, stream)
+                                    : launch_narrow_kernel<T, NK, NN, M, false>(a, sms, dev, stream);
 }
 
 template <typename T, int NK>

@@ -733,7 +733,7 @@ typedef struct nnb_project_args {
   int32_t adapters;
   int32_t rank; /* the adapters' largest rank rounded up to a multiple of 16 */
   int32_t type; /* NNB_BF16 or NNB_F16 */
-  int32_t reserved; /* 0 */
+  int32_t used_rank; /* the adapters' largest rank */
 } nnb_project_args;
 
 int64_t nnb_project_workspace_bytes(const nnb_project_args* args);

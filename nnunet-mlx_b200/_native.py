@@ -127,7 +127,7 @@ class ProjectArgs(ctypes.Structure):
                 ("rows", ctypes.c_int64), ("x_stride", ctypes.c_int64), ("out_stride", ctypes.c_int64),
                 ("rows_per_index", ctypes.c_int64), ("weight_stride", ctypes.c_int64), ("k", ctypes.c_int32),
                 ("n", ctypes.c_int32), ("adapters", ctypes.c_int32), ("rank", ctypes.c_int32),
-                ("type", ctypes.c_int32), ("reserved", ctypes.c_int32)]
+                ("type", ctypes.c_int32), ("used_rank", ctypes.c_int32)]
 
 
 SYMBOLS = {

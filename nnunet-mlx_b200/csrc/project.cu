@@ -1525,8 +1525,9 @@ __device__ __forceinline__ uint4 row_chunk(const T* row, int k, int width) {
 constexpr int kNarrowThreads = 256;
 
 // NK, NN: groups of 32 channels and columns; M: 16-row fragments per warp; RUNS: an index covers so many rows that a
-// warp's have one adapter or two.
-template <typename T, int NK, int NN, int M, bool RUNS>
+// warp's have one adapter or two; HALF: no adapter has more than 8 ranks, whose hi and lo parts side by side make the
+// 16 of one MMA.
+template <typename T, int NK, int NN, int M, bool RUNS, bool HALF>
 __global__ void __launch_bounds__(kNarrowThreads, 2) project_narrow_kernel(const nnb_project_args a) {
   constexpr bool kF16 = !std::is_same<T, __nv_bfloat16>::value;
   constexpr int kPitch = 4 * (NK | 1);  // 16-byte chunks of a W row in shared memory: neighbouring rows 64 bytes
@@ -1604,13 +1605,16 @@ __global__ void __launch_bounds__(kNarrowThreads, 2) project_narrow_kernel(const
                    : "r"(weight_at + (((t >> 2) * 32 + (t & 3) * 2) * kPitch + c * 4) * 16));
     return w;
   };
-  auto down_rows = [&](const T* src, int stride, int c, int t) {
-    return c * 32 + q * 8 < a.weight_stride
-               ? __ldg(reinterpret_cast<const uint4*>(src + (uint32_t)(t * 2 * stride + c * 32)))
-               : make_uint4(0, 0, 0, 0);
+  auto down_rows = [&](const T* src, uint32_t offset, int c) {
+    return c * 32 + q * 8 < a.weight_stride ? __ldg(reinterpret_cast<const uint4*>(src + offset + c * 32))
+                                            : make_uint4(0, 0, 0, 0);
   };
   auto up_columns = [&](const __nv_bfloat16* src, int width, int t) {
     const int col = min((t >> 2) * 32 + (t & 3) * 2, a.n - 1 - spread);  // columns past n are not stored
+    if constexpr (HALF) {
+      const uint32_t v = __ldg(reinterpret_cast<const uint32_t*>(src + col * width));
+      return make_uint2(v, v);
+    }
     return __ldg(reinterpret_cast<const uint2*>(src + col * width));
   };
   uint4 held_down[kHold ? 2 : 1];
@@ -1693,14 +1697,15 @@ __global__ void __launch_bounds__(kNarrowThreads, 2) project_narrow_kernel(const
       for (int j0 = 0; j0 < a.rank; j0 += 16) {
         int down_stride = (int)a.weight_stride, up_width = a.rank * (kF16 ? 2 : 1);
         if constexpr (!kHold) asm volatile("" : "+r"(down_stride), "+r"(up_width));
-        const T* down = reinterpret_cast<const T*>(a.down) +
-                        ((int64_t)listed * a.rank + j0 + (g >> 1) * 4 + (g & 1)) * a.weight_stride + q * 8;
+        const T* down = reinterpret_cast<const T*>(a.down) + ((int64_t)listed * a.rank + j0) * a.weight_stride + q * 8;
+        const uint32_t down_at[2] = {(uint32_t)((HALF ? g : (g >> 1) * 4 + (g & 1)) * down_stride),
+                                     (uint32_t)(((g >> 1) * 4 + (g & 1) + 2) * down_stride)};
         const __nv_bfloat16* up = reinterpret_cast<const __nv_bfloat16*>(a.up) +
-                                  ((int64_t)listed * a.n + spread) * up_width + j0 + q * 4;
+                                  ((int64_t)listed * a.n + spread) * up_width + j0 + (HALF ? q * 2 : q * 4);
         if constexpr (kHold) {
           if (held != listed || a.rank > 16) {
 #pragma unroll
-            for (int t = 0; t < 2; ++t) held_down[t] = down_rows(down, down_stride, 0, t);
+            for (int t = 0; t < 2; ++t) held_down[t] = down_rows(down, down_at[t], 0);
 #pragma unroll
             for (int t = 0; t < 4; ++t) {
               held_up[t] = up_columns(up, up_width, t);
@@ -1717,11 +1722,12 @@ __global__ void __launch_bounds__(kNarrowThreads, 2) project_narrow_kernel(const
           for (int t = 0; t < 2; ++t) {
             if constexpr (kHold)
               w[t] = held_down[t];
-            else
-              w[t] = down_rows(down, down_stride, c, t);
+            else if (t == 0 || !HALF)
+              w[t] = down_rows(down, down_at[t], c);
           }
 #pragma unroll
-          for (int t = 0; t < 2; ++t)
+          for (int t = 0; t < 2; ++t) {
+            if (t == 1 && HALF) break;
 #pragma unroll
             for (int m = 0; m < M; ++m) {
               const uint32_t one[4] = {x[m][0][c].x, x[m][1][c].x, x[m][0][c].y, x[m][1][c].y};
@@ -1730,13 +1736,16 @@ __global__ void __launch_bounds__(kNarrowThreads, 2) project_narrow_kernel(const
               else
                 warp_mma(low[m][t], one, w[t].x, w[t].y, T());
             }
+          }
 #pragma unroll
-          for (int t = 0; t < 2; ++t)
+          for (int t = 0; t < 2; ++t) {
+            if (t == 1 && HALF) break;
 #pragma unroll
             for (int m = 0; m < M; ++m) {
               const uint32_t two[4] = {x[m][0][c].z, x[m][1][c].z, x[m][0][c].w, x[m][1][c].w};
               warp_mma(low[m][t], two, w[t].z, w[t].w, T());
             }
+          }
         }
         if (mixed) {
 #pragma unroll
@@ -1757,8 +1766,14 @@ __global__ void __launch_bounds__(kNarrowThreads, 2) project_narrow_kernel(const
 #pragma unroll
           for (int t = 0; t < 2; ++t)
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
-              split2(low[m][t][h * 2] * scale, low[m][t][h * 2 + 1] * scale, hi[m][t * 2 + h], lo[m][t * 2 + h]);
+            for (int h = 0; h < 2; ++h) {
+              if (t == 1 && HALF) {
+                hi[m][2 + h] = lo[m][h];
+                lo[m][2 + h] = 0;
+              } else {
+                split2(low[m][t][h * 2] * scale, low[m][t][h * 2 + 1] * scale, hi[m][t * 2 + h], lo[m][t * 2 + h]);
+              }
+            }
 #pragma unroll
         for (int p = 0; p < NN; ++p) {
           uint2 w[4], rest[kF16 ? 4 : 1];
@@ -1776,15 +1791,18 @@ __global__ void __launch_bounds__(kNarrowThreads, 2) project_narrow_kernel(const
           for (int t = 0; t < 4; ++t)
 #pragma unroll
             for (int m = 0; m < M; ++m) warp_mma(acc[m][p * 4 + t], hi[m], w[t].x, w[t].y, __nv_bfloat16());
-#pragma unroll
-          for (int t = 0; t < 4; ++t)
-#pragma unroll
-            for (int m = 0; m < M; ++m) warp_mma(acc[m][p * 4 + t], lo[m], w[t].x, w[t].y, __nv_bfloat16());
-          if constexpr (kF16) {
+          if constexpr (!HALF) {
 #pragma unroll
             for (int t = 0; t < 4; ++t)
 #pragma unroll
-              for (int m = 0; m < M; ++m) warp_mma(acc[m][p * 4 + t], hi[m], rest[t].x, rest[t].y, __nv_bfloat16());
+              for (int m = 0; m < M; ++m) warp_mma(acc[m][p * 4 + t], lo[m], w[t].x, w[t].y, __nv_bfloat16());
+          }
+          if constexpr (kF16) {  // (HALF: the lo parts meet zeros)
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+#pragma unroll
+              for (int m = 0; m < M; ++m)
+                warp_mma(acc[m][p * 4 + t], hi[m], rest[t].x, HALF ? 0u : rest[t].y, __nv_bfloat16());
           }
         }
       }
@@ -1829,18 +1847,18 @@ __global__ void __launch_bounds__(kNarrowThreads, 2) project_narrow_kernel(const
   }
 }
 
-template <typename T, int NK, int NN, int M, bool RUNS>
+template <typename T, int NK, int NN, int M, bool RUNS, bool HALF>
 int launch_narrow_kernel(const nnb_project_args& a, int sms, int dev, cudaStream_t stream) {
   static int resident[64] = {0};
   int blocks = dev < 64 ? resident[dev] : 0;
   if (blocks == 0) {
-    NNB_CUDA_CHECK(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&blocks, project_narrow_kernel<T, NK, NN, M, RUNS>,
+    NNB_CUDA_CHECK(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&blocks, project_narrow_kernel<T, NK, NN, M, RUNS, HALF>,
                                                                  kNarrowThreads, 0));
     blocks = std::max(1, blocks);
     if (dev < 64) resident[dev] = blocks;
   }
   const int64_t groups = (a.rows + kNarrowThreads / 2 * M - 1) / (kNarrowThreads / 2 * M);
-  project_narrow_kernel<T, NK, NN, M, RUNS>
+  project_narrow_kernel<T, NK, NN, M, RUNS, HALF>
       <<<(unsigned)std::min<int64_t>(groups, (int64_t)blocks * sms), kNarrowThreads, 0, stream>>>(a);
   NNB_LAUNCH_CHECK();
   return NNB_OK;
@@ -1849,8 +1867,14 @@ int launch_narrow_kernel(const nnb_project_args& a, int sms, int dev, cudaStream
 template <typename T, int NK, int NN>
 int launch_narrow(const nnb_project_args& a, int sms, int dev, cudaStream_t stream) {
   constexpr int M = NK * NN <= 2 ? 2 : 1;  // a second fragment shares W's reads, as registers allow
-  return a.rows_per_index >= 16 * M ? launch_narrow_kernel<T, NK, NN, M, true>(a, sms, dev, stream)
-                                    : launch_narrow_kernel<T, NK, NN, M, false>(a, sms, dev, stream);
+  const bool runs = a.rows_per_index >= 16 * M;
+  if constexpr (NK * NN == 1) {  // (where the MMAs are most of the work)
+    if (a.used_rank <= 8)
+      return runs ? launch_narrow_kernel<T, NK, NN, M, true, true>(a, sms, dev, stream)
+                  : launch_narrow_kernel<T, NK, NN, M, false, true>(a, sms, dev, stream);
+  }
+  return runs ? launch_narrow_kernel<T, NK, NN, M, true, false>(a, sms, dev, stream)
+              : launch_narrow_kernel<T, NK, NN, M, false, false>(a, sms, dev, stream);
 }
 
 template <typename T, int NK>
@@ -1933,6 +1957,7 @@ extern "C" int32_t nnb_project(const nnb_project_args* args, void* stream) {
   NNB_REQUIRE(a.adapters >= 1 && a.rank >= 16 && a.rank <= NNB_PROJECT_MAX_RANK && a.rank % 16 == 0,
               "project: %d adapters of padded rank %d (a multiple of 16 up to %d)", a.adapters, a.rank,
               NNB_PROJECT_MAX_RANK);
+  NNB_REQUIRE(a.used_rank >= 1 && a.used_rank <= a.rank, "project: %d used ranks of %d", a.used_rank, a.rank);
   NNB_REQUIRE(a.rows_per_index >= 1 && a.x_stride >= 0 && (a.rows == 1 || a.out_stride >= a.n),
               "project: bad strides");
   NNB_REQUIRE(a.weight_stride >= a.k && a.weight_stride % 8 == 0 &&

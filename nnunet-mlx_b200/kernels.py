@@ -1222,6 +1222,7 @@ class AdaptedProjection:
     scales: torch.Tensor       # (adapters,) float32
     bias: torch.Tensor | None  # (N,) float32
     in_channels: int
+    used_rank: int             # the largest rank
 
     @property
     def out_channels(self) -> int:
@@ -1280,7 +1281,8 @@ def pack_projection(weight: torch.Tensor, adapters: list[Adapter],
         if not bool(torch.isfinite(down).all() & torch.isfinite(up).all()):
             raise ContractError("adapters must be finite")
         scales = torch.tensor([float(a.scale) for a in adapters], dtype=torch.float32, device=device)
-        return AdaptedProjection(packed, down, up, scales, None if bias is None else bias.detach().clone(), k)
+        return AdaptedProjection(packed, down, up, scales, None if bias is None else bias.detach().clone(), k,
+                                 max(int(a.down.shape[0]) for a in adapters))
 
 
 def adapted_projection(x: torch.Tensor, projection: AdaptedProjection, index: torch.Tensor, *,
@@ -1330,7 +1332,7 @@ def adapted_projection(x: torch.Tensor, projection: AdaptedProjection, index: to
     args = _native.ProjectArgs(x.data_ptr(), weight.data_ptr(), down.data_ptr(), projection.up.data_ptr(),
                                projection.scales.data_ptr(), _ptr(projection.bias), index.data_ptr(), out.data_ptr(),
                                0, rows, x_stride, out_stride, rows // index.numel(), weight_stride, shape[-1], n,
-                               adapters, rank, _ROW_TYPES[x.dtype], 0)
+                               adapters, rank, _ROW_TYPES[x.dtype], projection.used_rank)
     nbytes = lib.nnb_project_workspace_bytes(ctypes.byref(args))
     if nbytes < 0:
         _native.check(nbytes, "adapted_projection")

@@ -120,6 +120,9 @@ SHAPES = [  # rows, k, n, ranks, index
     (77, 40, 96, [24] * 30, "mixed"),
     (900, 90, 31, [2], "mixed"),
     (4000, 31, 128, [64, 3], "runs"),
+    (600, 32, 32, [24, 20], "runs"),           # a last block of ranks that is whole, or up to 8
+    (600, 64, 40, [22, 5], "mixed"),
+    (600, 30, 32, [8, 7], "mixed"),
 ]
 
 

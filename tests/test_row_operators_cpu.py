@@ -96,7 +96,7 @@ def test_c_entry_refuses_types_of_a_join():
 
 def _project_args(**over):
     values = dict(x=16, weight=16, down=16, up=16, scales=16, bias=0, index=16, out=16, low=16, rows=2, x_stride=8,
-                  out_stride=8, rows_per_index=1, weight_stride=8, k=8, n=8, adapters=1, rank=16, type=_native.BF16)
+                  out_stride=8, rows_per_index=1, weight_stride=8, k=8, n=8, adapters=1, rank=16, used_rank=9, type=_native.BF16)
     values.update(over)
     return _native.ProjectArgs(**values)
 
@@ -104,7 +104,7 @@ def _project_args(**over):
 @pytest.mark.parametrize("over", [
     *(dict([(name, 0)]) for name in ("x", "weight", "down", "up", "scales", "index", "out", "rows", "k", "n",
                                      "adapters", "rank", "rows_per_index")),
-    dict(rows=2 ** 31), dict(rank=8), dict(rank=272), dict(rank=24), dict(type=_native.F32), dict(x_stride=-1),
+    dict(rows=2 ** 31), dict(used_rank=0), dict(used_rank=17), dict(rank=8), dict(rank=272), dict(rank=24), dict(type=_native.F32), dict(x_stride=-1),
     dict(out_stride=7), dict(weight_stride=0), dict(weight_stride=12), dict(weight=18), dict(down=8), dict(up=4),
     dict(low=20), dict(low=0, k=256, weight_stride=256, x_stride=256)])
 def test_c_entry_refuses_projection(over):

@@ -441,6 +441,11 @@ __device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t&
 // ---------------------------------------------------------------------------
 constexpr int kLowThreads = 192;
 
+// A row's low-rank values in the workspace.
+__device__ __forceinline__ uint8_t* low_row(const nnb_project_args& a, int64_t row) {
+  return reinterpret_cast<uint8_t*>(a.low) + row * ((a.rank + kRankBlock - 1) / kRankBlock) * 128;
+}
+
 struct LowMaps {
   CUtensorMap x, down;
 };
@@ -534,17 +539,19 @@ __global__ void __launch_bounds__(kLowThreads, 2)
       for (int p = 0; p < passes && alive; ++p) {
         const int from = blocks > 1 ? p / blocks : p * together;
         const int to = blocks > 1 ? from + 1 : min(count, from + together);
+        const int j0 = blocks > 1 ? p % blocks * plan.columns : 0, adapter = listed[from];
+        const uint32_t box_bytes = box * 128, bytes = kStageA + (to - from) * box_bytes;
         for (int c = first_chunk; c < first_chunk + chunks; ++c) {
           if (!mbar_wait(smem_u32(&empty[s]), phase ^ 1, abort_flag, 53)) {
             alive = false;
             break;
           }
           const uint32_t bar = smem_u32(&full[s]), at = smem_u32(stages + s * stage);
-          mbar_arrive_expect_tx(bar, kStageA + (to - from) * box * 128);
+          mbar_arrive_expect_tx(bar, bytes);
           tma_load_2d(at, &maps.x, c * 64, (int)row0, bar);
-          for (int i = from; i < to; ++i)
-            tma_load_3d(at + kStageA + (i - from) * box * 128, &maps.down, c * 64, (p % blocks) * plan.columns,
-                        listed[i], bar);
+          tma_load_3d(at + kStageA, &maps.down, c * 64, j0, adapter, bar);
+          for (int i = from + 1; i < to; ++i)
+            tma_load_3d(at + kStageA + (i - from) * box_bytes, &maps.down, c * 64, j0, listed[i], bar);
           if (++s == S) s = 0, phase ^= 1u;
           ++issued;
         }
@@ -588,10 +595,12 @@ __global__ void __launch_bounds__(kLowThreads, 2)
     }
     __syncwarp();
   } else {
+    uint8_t* const own_low = low_row(a, row0 + r);
+    const float own_scale = scales[r];
     for (int p = 0; p < passes; ++p) {
       const int from = blocks > 1 ? p / blocks : p * together;
       const int to = blocks > 1 ? from + 1 : min(count, from + together);
-      const int j0 = (p % blocks) * plan.columns, width = min(plan.columns, a.rank - j0);
+      const int j0 = blocks > 1 ? p % blocks * plan.columns : 0, width = min(plan.columns, a.rank - j0);
       const bool ok = mbar_wait(smem_u32(acc_full), (uint32_t)p & 1, abort_flag, 58);
       if (!__all_sync(0xffffffffu, ok)) break;
       fence_after();
@@ -601,7 +610,19 @@ __global__ void __launch_bounds__(kLowThreads, 2)
         for (int j = 0; j < width; j += 16) {
           float v[16];
           tmem_ld16(tmem + ((uint32_t)(warp & 3) << 21) + (i - from) * box + j, v);
-          if (mine == adapter) {
+          if (mine == adapter && gridDim.y == 1) {  // nothing to add up
+#pragma unroll
+            for (int e = 0; e < 16; e += 8) {
+              uint4 hi, lo;
+              split2(v[e] * own_scale, v[e + 1] * own_scale, hi.x, lo.x);
+              split2(v[e + 2] * own_scale, v[e + 3] * own_scale, hi.y, lo.y);
+              split2(v[e + 4] * own_scale, v[e + 5] * own_scale, hi.z, lo.z);
+              split2(v[e + 6] * own_scale, v[e + 7] * own_scale, hi.w, lo.w);
+              uint8_t* out = own_low + (j0 + j) / kRankBlock * 128 + ((j0 + j) % kRankBlock + e) * 2;
+              *reinterpret_cast<uint4*>(out) = hi;
+              *reinterpret_cast<uint4*>(out + 64) = lo;
+            }
+          } else if (mine == adapter) {
 #pragma unroll
             for (int e = 0; e < 16; e += 4)
               *reinterpret_cast<float4*>(sums + r * pitch + j0 + j + e) =
@@ -614,38 +635,46 @@ __global__ void __launch_bounds__(kLowThreads, 2)
       if (lane == 0) mbar_arrive(smem_u32(acc_empty));
     }
   }
-  cluster_barrier();
-  if (warp >= 2 && *reinterpret_cast<volatile int*>(abort_flag) == 0) {
-    // this CTA's share of the rows: four ranks a thread and turn, summed over the cluster in order
-    const int parts = gridDim.y, share = (BM + parts - 1) / parts;
-    const int begin = blockIdx.y * share, end = min(BM, begin + share);
-    const int fours = a.rank / 4, low_blocks = (a.rank + kRankBlock - 1) / kRankBlock;
-    const uint32_t base = smem_u32(sums);
-    for (int i = r; i < (end - begin) * fours; i += 128) {
-      const int row = begin + i / fours, j = i % fours * 4;
-      const float scale = scales[row];
-      if (scale == -INFINITY) continue;
-      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-      for (int c = 0; c < parts; ++c) {
-        uint32_t peer;
-        asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(peer) : "r"(base + (row * pitch + j) * 4), "r"(c));
-        float4 w;
-        asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-                     : "=f"(w.x), "=f"(w.y), "=f"(w.z), "=f"(w.w)
-                     : "r"(peer)
-                     : "memory");
-        v.x += w.x, v.y += w.y, v.z += w.z, v.w += w.w;
+  if (gridDim.y == 1) {
+    __syncthreads();
+  } else {
+    cluster_barrier();
+    if (warp >= 2 && *reinterpret_cast<volatile int*>(abort_flag) == 0) {
+      // this CTA's share of the rows: four ranks a thread and turn, summed over the cluster in order
+      const int parts = gridDim.y, share = (BM + parts - 1) / parts;
+      const int begin = blockIdx.y * share, end = min(BM, begin + share), fours = a.rank / 4;
+      const uint32_t base = smem_u32(sums);
+      for (int i = r; i < (end - begin) * fours; i += 128) {
+        const int row = begin + i / fours, j = i % fours * 4;
+        const float scale = scales[row];
+        if (scale == -INFINITY) continue;
+        float4 w[8];
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+          uint32_t peer;
+          asm("mapa.shared::cluster.u32 %0, %1, %2;"
+              : "=r"(peer)
+              : "r"(base + (row * pitch + j) * 4), "r"(c < parts ? c : 0));
+          w[c] = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (c < parts)
+            asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                         : "=f"(w[c].x), "=f"(w[c].y), "=f"(w[c].z), "=f"(w[c].w)
+                         : "r"(peer)
+                         : "memory");
+        }
+        float4 v = w[0];
+#pragma unroll
+        for (int c = 1; c < 8; ++c) v.x += w[c].x, v.y += w[c].y, v.z += w[c].z, v.w += w[c].w;
+        uint2 hi, lo;
+        split2(v.x * scale, v.y * scale, hi.x, lo.x);
+        split2(v.z * scale, v.w * scale, hi.y, lo.y);
+        uint8_t* out = low_row(a, row0 + row) + j / kRankBlock * 128 + j % kRankBlock * 2;
+        *reinterpret_cast<uint2*>(out) = hi;
+        *reinterpret_cast<uint2*>(out + 64) = lo;
       }
-      uint2 hi, lo;
-      split2(v.x * scale, v.y * scale, hi.x, lo.x);
-      split2(v.z * scale, v.w * scale, hi.y, lo.y);
-      uint8_t* out = reinterpret_cast<uint8_t*>(a.low) + ((row0 + row) * low_blocks + j / kRankBlock) * 128 +
-                     j % kRankBlock * 2;
-      *reinterpret_cast<uint2*>(out) = hi;
-      *reinterpret_cast<uint2*>(out + 64) = lo;
     }
+    cluster_barrier();  // a CTA's sums stay until its peers have read them
   }
-  cluster_barrier();  // a CTA's sums stay until its peers have read them
   __syncwarp();
   if (warp == 1) {
     fence_after();
@@ -1196,16 +1225,9 @@ __global__ void __launch_bounds__(kFewThreads, 2)
   const int r = threadIdx.x - 64, col = n0 + r;
   const int begin = part * plan.share, end = min((int)a.rows, begin + plan.share);
   if (warp >= 2) {
-    // the share's adapters, and their up rows on the way to L2, before the low-rank rows are there
+    // the share's adapters, before the low-rank rows are there
     if (begin + r < end) adapters[r] = row_adapter(a, begin + r);
     adapter_barrier(true);
-    const int bytes = a.rank * (kF16 ? 4 : 2);
-    for (int t = begin; t < end; ++t) {
-      const int adapter = adapters[t - begin];
-      if (adapter < 0 || col >= a.n) continue;
-      const uint8_t* row = reinterpret_cast<const uint8_t*>(a.up) + ((int64_t)adapter * a.n + col) * bytes;
-      for (int b = 0; b < bytes; b += 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(row + b));
-    }
     // the low-rank rows are the previous kernel's, which may still run; every CTA waits for its end
     asm volatile("griddepcontrol.wait;" ::: "memory");
     for (int t = begin; t < end; t += 16) {

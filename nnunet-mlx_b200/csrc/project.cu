@@ -1074,17 +1074,48 @@ struct FewMaps {
   CUtensorMap x, weight;
 };
 
+constexpr int kFewLow = 1024;  // low-rank values of a CTA's share that it may compute itself
+
 struct FewPlan {
-  int parts;    // of the low-rank rows
+  int parts;    // of the low-rank rows; 0: the kernel computes its share's itself
   int columns;  // rows rounded up to 16
   int stages;
   int split;    // CTAs of a cluster
   int share;    // rows a CTA of the cluster writes
 };
 
-// The adapters' share of rows [t0, t0 + N) in one column, into sums[t - t0][128].
+// The low-rank rows [begin, end), a dot product per warp and turn, into low[t - begin][rank].
+template <typename T>
+__device__ __forceinline__ void few_low(const nnb_project_args& a, int begin, int end, int r,
+                                        const volatile int* adapters, float* low) {
+  const int lane = r & 31, whole = a.k & ~7;
+  for (int i = r >> 5; i < (end - begin) * a.rank; i += 4) {
+    const int t = i / a.rank, j = i - t * a.rank, adapter = adapters[t];
+    float sum = 0.f;
+    if (adapter >= 0) {
+      const T* x = reinterpret_cast<const T*>(a.x) + (begin + t) * a.x_stride;
+      const T* down = reinterpret_cast<const T*>(a.down) + ((int64_t)adapter * a.rank + j) * a.weight_stride;
+#pragma unroll 4
+      for (int k = lane * 8; k < whole; k += 256) {
+        float v[8], d[8];
+        widen<T>(v, *reinterpret_cast<const uint4*>(x + k));
+        widen<T>(d, __ldg(reinterpret_cast<const uint4*>(down + k)));
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sum = fmaf(v[e], d[e], sum);
+      }
+      if (whole + lane < a.k) sum = fmaf(value(x[whole + lane]), value(down[whole + lane]), sum);
+#pragma unroll
+      for (int h = 16; h >= 1; h >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, h);
+      sum *= __ldg(a.scales + adapter);
+    }
+    if (lane == 0) low[i] = sum;
+  }
+}
+
+// The adapters' share of rows [t0, t0 + N) in one column, into sums[t - t0][128].  `low`: those rows' low-rank
+// values, or null where the workspace has them.
 template <bool F16, int N>
-__device__ __forceinline__ void few_dots(const nnb_project_args& a, int parts, int t0, int end, int col, int r,
+__device__ __forceinline__ void few_dots(const nnb_project_args& a, const float* low, int parts, int t0, int end, int col, int r,
                                          float* values, const volatile int* adapters, float* sums) {
   constexpr int kPlanes = F16 ? 2 : 1;
   float acc[N] = {};
@@ -1095,7 +1126,9 @@ __device__ __forceinline__ void few_dots(const nnb_project_args& a, int parts, i
       const int t = i / fours, j = (i - t * fours) * 4;
       const bool some = t0 + t < end && adapters[t] >= 0;
       *reinterpret_cast<float4*>(values + t * kFewRanks + j) =
-          some ? low_values(a, parts, t0 + t, j0 + j) : make_float4(0.f, 0.f, 0.f, 0.f);
+          !some ? make_float4(0.f, 0.f, 0.f, 0.f)
+          : low != nullptr ? *reinterpret_cast<const float4*>(low + t * a.rank + j0 + j)
+                           : low_values(a, parts, t0 + t, j0 + j);
     }
     adapter_barrier(true);
     const __nv_bfloat16* up[N];
@@ -1144,7 +1177,8 @@ __global__ void __launch_bounds__(kFewThreads, 2)
   float* partial = reinterpret_cast<float*>(stages);  // [rows][128] after the MMAs, over the stages
   float* sums = reinterpret_cast<float*>(stages + S * stage);  // [share][128]
   float* values = sums + plan.share * BM;                      // [16][kFewRanks]
-  uint64_t* full = reinterpret_cast<uint64_t*>(values + 16 * kFewRanks);
+  float* own_low = values + 16 * kFewRanks;                    // [share][rank], up to kFewLow
+  uint64_t* full = reinterpret_cast<uint64_t*>(own_low + kFewLow);
   uint64_t* empty = full + S;
   uint64_t* acc_full = empty + S;
   uint64_t* drain = acc_full + 1;
@@ -1229,14 +1263,18 @@ __global__ void __launch_bounds__(kFewThreads, 2)
     if (begin + r < end) adapters[r] = row_adapter(a, begin + r);
     adapter_barrier(true);
     // the low-rank rows are the previous kernel's, which may still run; every CTA waits for its end
-    asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (plan.parts > 0)
+      asm volatile("griddepcontrol.wait;" ::: "memory");
+    else
+      few_low<T>(a, begin, end, r, adapters, own_low);
     for (int t = begin; t < end; t += 16) {
+      const float* low = plan.parts > 0 ? nullptr : own_low + (t - begin) * a.rank;
       float* to = sums + (t - begin) * BM;
       const volatile int* of = adapters + (t - begin);
       if (end - t <= 4)
-        few_dots<kF16, 4>(a, plan.parts, t, end, min(col, a.n - 1), r, values, of, to);
+        few_dots<kF16, 4>(a, low, plan.parts, t, end, min(col, a.n - 1), r, values, of, to);
       else
-        few_dots<kF16, 16>(a, plan.parts, t, end, min(col, a.n - 1), r, values, of, to);
+        few_dots<kF16, 16>(a, low, plan.parts, t, end, min(col, a.n - 1), r, values, of, to);
     }
     const bool ok = mbar_wait(smem_u32(acc_full), 0, abort_flag, 63);
     if (__all_sync(0xffffffffu, ok)) {
@@ -1323,6 +1361,17 @@ bool rows_in_place(const nnb_project_args& a) {
 
 bool narrow(const nnb_project_args& a) { return a.k <= 128 && a.n <= 128; }
 
+// Plans are made for a whole B200, so that the workspace's size needs no device.
+constexpr int kPlanSms = 148;
+
+// CTAs of a cluster: as many parts of the channels as leave two CTAs an SM.
+int few_split(const nnb_project_args& a) {
+  const int tiles = (a.n + BM - 1) / BM, chunks = (a.k + 63) / 64;
+  int split = 1;
+  while (split < 8 && split * 2 <= chunks && tiles * split * 2 <= 2 * kPlanSms) split *= 2;
+  return split;
+}
+
 // How the low-rank rows are computed: by tiles or by rows, in how many parts of the channels.
 struct LowPlan {
   bool few;   // up to one tile of rows
@@ -1335,6 +1384,15 @@ struct LowPlan {
 LowPlan low_plan(const nnb_project_args& a) {
   LowPlan p;
   p.few = a.rows <= BM;
+  if (p.few) {
+    // Every tile of columns would compute a share of the rows again; up to 128 products a thread that is less than a
+    // launch (one row of 320 -> 320 channels, rank 8).
+    const int64_t share = (a.rows + few_split(a) - 1) / few_split(a) * a.rank;
+    if (share <= kFewLow && share * a.k <= 128 * 256) {
+      p.parts = p.part = 0;
+      return p;
+    }
+  }
   const int64_t units = p.few ? a.rows * (a.rank / 16) : (a.rows + BM - 1) / BM;
   const int total = p.few ? a.k : (a.k + 63) / 64, least = p.few ? 512 : 4;
   p.parts = 1;
@@ -1354,13 +1412,14 @@ int64_t low_bytes(const nnb_project_args& a) {
                : a.rows * ((a.rank + kRankBlock - 1) / kRankBlock) * 128;
 }
 
-// A GEMM kernel's launch while the low-rank kernel before it still runs: only the warps that read its rows wait
-// for its end (griddepcontrol).
+// A GEMM kernel's launch; `early`: while the low-rank kernel before it still runs, and only the warps that read its
+// rows wait for its end (griddepcontrol).
 template <typename... P, typename... V>
-int launch_early(void (*kernel)(P...), int grid, int threads, int smem, int cluster, cudaStream_t stream, V... args) {
+int launch_gemm(void (*kernel)(P...), int grid, int threads, int smem, int cluster, bool early, cudaStream_t stream,
+                V... args) {
   cudaLaunchAttribute attributes[2];
   attributes[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attributes[0].val.programmaticStreamSerializationAllowed = 1;
+  attributes[0].val.programmaticStreamSerializationAllowed = early ? 1 : 0;
   attributes[1].id = cudaLaunchAttributeClusterDimension;
   attributes[1].val.clusterDim.x = cluster;
   attributes[1].val.clusterDim.y = attributes[1].val.clusterDim.z = 1;
@@ -1393,6 +1452,7 @@ template <typename T>
 int launch_low(const nnb_project_args& a, const LowPlan& plan, int dev, cudaStream_t stream) {
   constexpr bool kF16 = !std::is_same<T, __nv_bfloat16>::value;
   if (plan.few) {
+    if (plan.parts == 0) return NNB_OK;
     project_low_kernel<T><<<dim3((unsigned)a.rows, a.rank / 16, plan.parts), 128, 0, stream>>>(a, plan.part);
     NNB_LAUNCH_CHECK();
     return NNB_OK;
@@ -1428,17 +1488,16 @@ int launch_low(const nnb_project_args& a, const LowPlan& plan, int dev, cudaStre
 }
 
 template <typename T>
-int launch_few(const nnb_project_args& a, const LowPlan& low, int sms, int dev, cudaStream_t stream) {
+int launch_few(const nnb_project_args& a, const LowPlan& low, int dev, cudaStream_t stream) {
   constexpr bool kF16 = !std::is_same<T, __nv_bfloat16>::value;
   const int tiles = (a.n + BM - 1) / BM, chunks = (a.k + 63) / 64;
   FewPlan plan;
+  plan.split = few_split(a);
   plan.parts = low.parts;
   plan.columns = ((int)a.rows + 15) / 16 * 16;
-  plan.split = 1;  // as many parts of the channels as leave two CTAs an SM
-  while (plan.split < 8 && plan.split * 2 <= chunks && tiles * plan.split * 2 <= 2 * sms) plan.split *= 2;
   plan.share = ((int)a.rows + plan.split - 1) / plan.split;
   const int stage = BM * 128 + plan.columns * 128;
-  const int fixed = 1024 + plan.share * BM * 4 + 16 * kFewRanks * 4 + 1024;
+  const int fixed = 1024 + plan.share * BM * 4 + (16 * kFewRanks + kFewLow) * 4 + 1024;
   // stages for two CTAs an SM, but room for the partial sums ([rows][128] floats over the stages) and at least two
   plan.stages = std::max(2, std::min({8, (112 * 1024 - fixed) / stage, (chunks + plan.split - 1) / plan.split}));
   while (plan.stages * stage < (int)a.rows * BM * 4) ++plan.stages;
@@ -1452,7 +1511,8 @@ int launch_few(const nnb_project_args& a, const LowPlan& low, int sms, int dev, 
   FewMaps maps;
   if (const int rc = encode_rows(&maps.x, kF16, a, plan.columns)) return rc;
   if (const int rc = encode_weight(&maps.weight, kF16, a, BM)) return rc;
-  return launch_early(project_few_kernel<T>, tiles * plan.split, kFewThreads, smem, plan.split, stream, a, maps, plan);
+  return launch_gemm(project_few_kernel<T>, tiles * plan.split, kFewThreads, smem, plan.split, plan.parts > 0, stream, a,
+                     maps, plan);
 }
 
 template <typename T, int BN, bool PAIR>
@@ -1479,7 +1539,7 @@ int launch_tiles(const nnb_project_args& a, int sms, int dev, cudaStream_t strea
   const int64_t tiles = (a.rows + C::kRows - 1) / C::kRows * ((a.n + BN - 1) / BN);
   NNB_REQUIRE(tiles < (int64_t)1 << 30, "project: %lld tiles", (long long)tiles);
   const int grid = (int)std::min<int64_t>(tiles, (int64_t)sms / C::kPeers) * C::kPeers;
-  return launch_early(project_kernel<T, BN, PAIR>, grid, kThreads, C::kSmem, C::kPeers, stream, a, maps);
+  return launch_gemm(project_kernel<T, BN, PAIR>, grid, kThreads, C::kSmem, C::kPeers, true, stream, a, maps);
 }
 
 // Tile width: the one whose waves of tiles take least, by the time of a tile measured on B200 with every SM busy:
@@ -1935,7 +1995,7 @@ int launch_project(nnb_project_args a, cudaStream_t stream) {
   }
   const LowPlan plan = low_plan(a);
   if (const int rc = launch_low<T>(a, plan, dev, stream)) return rc;
-  if (plan.few) return launch_few<T>(a, plan, sms, dev, stream);
+  if (plan.few) return launch_few<T>(a, plan, dev, stream);
   switch (tile_columns(a, sms)) {
     case 64: return launch_tiles<T, 64, false>(a, sms, dev, stream);
     case 128: return launch_tiles<T, 128, false>(a, sms, dev, stream);

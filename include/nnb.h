@@ -708,7 +708,9 @@ int32_t nnb_gated_join(const nnb_join_args* args, void* stream);
  *   out_t = W x_t + bias + scale_a up_a (down_a x_t),  a = index[t / rows_per_index], -1 for none
  *
  * An index outside [-1, adapters) gives its rows the shared projection alone
- * and records NNB_E_DEVICE for nnb_device_status.
+ * and records NNB_E_DEVICE for nnb_device_status.  `down` and `up` must be
+ * finite: a tile of rows of several requests multiplies each adapter by the
+ * others' zeros.
  */
 #define NNB_PROJECT_MAX_RANK 256
 

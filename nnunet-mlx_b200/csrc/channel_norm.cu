@@ -329,7 +329,7 @@ __global__ void __launch_bounds__(block_threads(TPR)) gated_join_kernel(const nn
     for (int ch = 0; ch < NCH; ++ch) load_chunk<ALIGNED, TPR>(skip[ch], s, ch, lane, channels);
     if (wide_gate) {
       int64_t at_gate = at;
-      if (a.gate_mode == NNB_GATE_SAMPLE)
+      if (a.gate_mode == NNB_GATE_SAMPLE)  // (rows_per_sample is at most rows)
         at_gate = a.rows <= UINT32_MAX ? (uint32_t)at / (uint32_t)a.rows_per_sample : at / a.rows_per_sample;
       const TB* g = reinterpret_cast<const TB*>(a.gate) + at_gate * a.gate_stride;
 #pragma unroll
@@ -530,7 +530,8 @@ extern "C" int32_t nnb_channel_norm_rows(const nnb_norm_args* args, void* stream
 
 extern "C" int32_t nnb_gated_join(const nnb_join_args* args, void* stream) {
   NNB_REQUIRE(args != nullptr, "gated_join: null args");
-  const nnb_join_args& a = *args;
+  nnb_join_args a = *args;
+  a.rows_per_sample = std::min(a.rows_per_sample, a.rows);
   NNB_REQUIRE(a.branch != nullptr && a.skip != nullptr && a.stream != nullptr, "gated_join: null pointer");
   NNB_REQUIRE(a.rows >= 1 && a.channels >= 1 && a.channels <= NNB_NORM_MAX_CHANNELS,
               "gated_join: %lld rows of %d channels (1 to %d)", (long long)a.rows, a.channels, NNB_NORM_MAX_CHANNELS);

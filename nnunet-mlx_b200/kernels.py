@@ -1002,7 +1002,14 @@ def _channels_pointer(p: torch.Tensor | None, name: str, channels: int, device: 
     if p.shape != (channels,) or p.device != device:
         raise ContractError(f"{name} must hold {channels} values on {device}, "
                             f"got {tuple(p.shape)} on {p.device}")
+    _check_no_gradient(p, name)
     return p.data_ptr()
+
+
+def _check_no_gradient(t: torch.Tensor, name: str) -> None:
+    if t.requires_grad and torch.is_grad_enabled():
+        raise ContractError(f"{name} requires a gradient: this operator has no backward pass "
+                            "(call it under torch.no_grad())")
 
 
 def _check_rows(t: torch.Tensor, name: str) -> None:
@@ -1010,9 +1017,7 @@ def _check_rows(t: torch.Tensor, name: str) -> None:
         raise ContractError(f"{name} must be a float32, bfloat16 or float16 CUDA tensor")
     if t.dim() < 1 or t.shape[-1] < 1:
         raise ContractError(f"{name} must have channels in its last axis, got shape {tuple(t.shape)}")
-    if t.requires_grad and torch.is_grad_enabled():
-        raise ContractError(f"{name} requires a gradient: this operator has no backward pass "
-                            "(call it under torch.no_grad())")
+    _check_no_gradient(t, name)
 
 
 def _row_stride(t: torch.Tensor, name: str) -> int:
@@ -1254,7 +1259,7 @@ def pack_projection(weight: torch.Tensor, adapters: list[Adapter],
         raise ContractError("an adapted projection needs at least one adapter")
     n, k = (int(v) for v in weight.shape)
     device, dtype = weight.device, weight.dtype
-    _channels_pointer(bias, "projection bias", n, device)
+    _channels_pointer(None if bias is None else bias.detach(), "projection bias", n, device)
     for i, a in enumerate(adapters):
         if a.down.shape[1] != k or a.up.shape != (n, a.down.shape[0]):
             raise ContractError(f"adapter {i}: down {tuple(a.down.shape)} and up {tuple(a.up.shape)} do not fit a "
@@ -1290,7 +1295,7 @@ def adapted_projection(x: torch.Tensor, projection: AdaptedProjection, index: to
     """``x W^T + bias`` of every row, plus ``scale x down^T up^T`` of the adapter its request names.
 
     ``x`` is ``(..., K)`` rows of the projection's type (contiguous channels,
-    evenly spaced rows).  ``index`` is a contiguous int32 tensor over leading
+    evenly spaced rows, fewer than 2^31 of them).  ``index`` is a contiguous int32 tensor over leading
     axes of ``x``: one adapter, or -1 for none, per row (``x.shape[:-1]``) or
     per sample (``x.shape[:1]`` and so on).  An index out of range gives its
     rows the shared projection alone and is reported by
@@ -1322,7 +1327,8 @@ def adapted_projection(x: torch.Tensor, projection: AdaptedProjection, index: to
     else:
         out_stride = _check_out(out, "out", (*shape[:-1], n), x.dtype, device)
         for name, t in (("x", x), ("index", index), ("the projection", weight), ("the projection", down),
-                        ("the projection", projection.up), ("the projection", projection.bias)):
+                        ("the projection", projection.up), ("the projection", projection.scales),
+                        ("the projection", projection.bias)):
             if t is not None and _overlap(out, t):
                 raise ContractError(f"out overlaps {name}")
     rows = out.numel() // n

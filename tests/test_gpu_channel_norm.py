@@ -245,6 +245,19 @@ def test_gate_values_at_the_edges(cuda_device):
     assert empty.shape == normed.shape == (0, 8)
 
 
+def test_what_lies_behind_a_row_is_not_read(cuda_device):
+    rng = np.random.default_rng(11)
+    for channels in (24, 31, 320, 333, 2048, 5000):
+        for dtype in ("f32", "bf16"):
+            wide = [make(rng, (9, channels + 8), dtype, cuda_device) for _ in range(3)]
+            for t in wide:
+                t[:, channels:] = float("nan")
+            branch, skip, gate = (t[:, :channels] for t in wide)
+            p, n = (("layer", *params(rng, channels, cuda_device), 1e-5) for _ in range(2))
+            check_norm(branch, "layer", p[1], p[2], 1e-5, torch.float32)
+            check_join(branch, skip, p, gate, "sigmoid", p[1], 0.7, n, torch.float32)
+
+
 def test_other_stream_and_capture(cuda_device):
     from nnunet_mlx_b200 import kernels
 
@@ -297,6 +310,10 @@ def test_refusals(cuda_device):
     refused(lambda: kernels.channel_norm(x[:1], kernels.ChannelNorm("rms", w), out=w.view(1, 32)), "out overlaps weight")
     refused(lambda: kernels.channel_norm(x, n, out=x[:1].expand(4, 32)), "overlap")
     refused(lambda: kernels.channel_norm(x.requires_grad_(), n), "no backward pass")
+    refused(lambda: kernels.channel_norm(x.detach(), kernels.ChannelNorm("rms", torch.nn.Parameter(w))),
+            "no backward pass")
+    with torch.no_grad():
+        assert not kernels.channel_norm(x, kernels.ChannelNorm("rms", torch.nn.Parameter(w))).requires_grad
     x = x.detach()
     join = kernels.gated_residual_join
     refused(lambda: join(x, x[:3]), "residual shapes differ")

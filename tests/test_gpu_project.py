@@ -207,6 +207,49 @@ def test_values_do_not_reach_other_rows(cuda_device):
     check(make_rows(rng, (150, 64), "f16", cuda_device), parts, make_index(rng, 150, 3, "one", cuda_device) * 0)
 
 
+@pytest.mark.parametrize("rows,k,n", [(1, 330, 40), (5, 1001, 48), (100, 330, 200), (300, 1001, 333), (700, 100, 90)])
+def test_what_lies_behind_a_row_is_not_read(cuda_device, rows, k, n):
+    rng = np.random.default_rng(10)
+    for dtype in ("bf16", "f16"):
+        parts = problem(rng, k, n, [8, 20], dtype, cuda_device)
+        buffer = make_rows(rng, (rows + 2, (k + 15) // 8 * 8), dtype, cuda_device)  # rows that are read in place
+        buffer[:, k:] = float("nan")
+        buffer[rows:] = float("inf")
+        check(buffer[:rows, :k], parts, make_index(rng, rows, 2, "mixed", cuda_device))
+
+
+def test_first_call_inside_a_capture():
+    """A process whose first call of every operator is captured: nothing needs a call outside before it."""
+    import subprocess
+    import sys
+
+    program = """
+import torch
+from nnunet_mlx_b200 import kernels
+d = torch.device("cuda:0")
+def rows(r, k): return torch.ones((r, k), dtype=torch.bfloat16, device=d)
+cases = []
+for r, k, n in ((1, 256, 64), (64, 1024, 256), (300, 256, 512), (300, 255, 64), (4000, 32, 32)):
+    p = kernels.pack_projection(rows(n, k), [kernels.Adapter(rows(16, k), rows(n, 16))])
+    cases.append((rows(r, k), p, torch.zeros(r, dtype=torch.int32, device=d)))
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    out = [kernels.adapted_projection(*c) for c in cases]
+    normed = kernels.channel_norm(cases[0][0], kernels.ChannelNorm())
+    joined, _ = kernels.gated_residual_join(normed, cases[0][0], next_norm=kernels.ChannelNorm())
+for _ in range(2):
+    graph.replay()
+torch.cuda.synchronize()
+for (x, p, i), o in zip(cases, out):
+    k = x.shape[1]
+    assert (o == torch.tensor(17.0 * k).bfloat16()).all(), (o.min(), o.max(), k)
+assert (joined == 2).all()
+"""
+    done = subprocess.run([sys.executable, "-c", program], capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0, done.stderr[-2000:]
+
+
 def test_order_of_rows_does_not_matter(cuda_device):
     from nnunet_mlx_b200 import kernels
 

@@ -106,7 +106,7 @@ def _project_args(**over):
                                      "adapters", "rank", "rows_per_index")),
     dict(rows=2 ** 31), dict(used_rank=0), dict(used_rank=17), dict(rank=8), dict(rank=272), dict(rank=24), dict(type=_native.F32), dict(x_stride=-1),
     dict(out_stride=7), dict(weight_stride=0), dict(weight_stride=12), dict(weight=18), dict(down=8), dict(up=4),
-    dict(low=20), dict(low=0, k=256, weight_stride=256, x_stride=256)])
+    dict(low=20), dict(low=0, k=256, weight_stride=256, x_stride=256, rows=200)])
 def test_c_entry_refuses_projection(over):
     args = _project_args(**over)
     assert _native.load().nnb_project(ctypes.byref(args), None) == -1
@@ -115,7 +115,13 @@ def test_c_entry_refuses_projection(over):
 
 def test_projection_workspace():
     load = _native.load()
-    assert load.nnb_project_workspace_bytes(ctypes.byref(_project_args(rows=10, rank=32, k=256))) >= 10 * 32 * 4
+    assert load.nnb_project_workspace_bytes(ctypes.byref(_project_args(rows=100, rank=32, k=4096))) >= 100 * 32 * 4
+    assert load.nnb_project_workspace_bytes(ctypes.byref(_project_args(rows=300, rank=48, k=256,
+                                                                       x_stride=256))) == 300 * 2 * 128
+    # rows off 16 bytes are copied; a row or few, or few channels, need nothing else
+    assert load.nnb_project_workspace_bytes(ctypes.byref(_project_args(rows=2, x_stride=9))) == 2 * 8 * 2
+    assert load.nnb_project_workspace_bytes(ctypes.byref(_project_args(rows=1, k=256, x_stride=256))) == 0
+    assert load.nnb_project_workspace_bytes(ctypes.byref(_project_args(rows=1000))) == 0
     for bad in (dict(rows=0), dict(k=0), dict(rank=0)):
         assert load.nnb_project_workspace_bytes(ctypes.byref(_project_args(**bad))) == -1
     assert load.nnb_project_workspace_bytes(None) == -1

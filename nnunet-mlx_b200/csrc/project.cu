@@ -1379,8 +1379,8 @@ struct LowPlan {
   int part;   // channels (few) or chunks of 64 of a part
 };
 
-// Enough parts that some 300 CTAs run (two per SM), of at least 512 channels (four loads of a lane) or four
-// chunks, and no more than eight.
+// Enough parts that some 300 CTAs run (two per SM; of rows, whose CTAs are small, some 1000), of at least 512
+// channels (two loads of a lane) or four chunks, and no more than eight.
 LowPlan low_plan(const nnb_project_args& a) {
   LowPlan p;
   p.few = a.rows <= BM;
@@ -1396,7 +1396,7 @@ LowPlan low_plan(const nnb_project_args& a) {
   const int64_t units = p.few ? a.rows * (a.rank / 16) : (a.rows + BM - 1) / BM;
   const int total = p.few ? a.k : (a.k + 63) / 64, least = p.few ? 512 : 4;
   p.parts = 1;
-  while (p.parts < 8 && total / (p.parts * 2) >= least && units * p.parts * 2 <= 320) p.parts *= 2;
+  while (p.parts < 8 && total / (p.parts * 2) >= least && units * p.parts * 2 <= (p.few ? 1024 : 320)) p.parts *= 2;
   p.part = (total + p.parts - 1) / p.parts;
   if (p.few) {
     p.part = (p.part + 255) / 256 * 256;  // whole loads of a warp

@@ -960,7 +960,7 @@ def nearest_axis_resize(source: torch.Tensor, target) -> torch.Tensor:
 _ROW_TYPES = {torch.float32: _native.F32, torch.bfloat16: _native.BF16, torch.float16: _native.F16}
 _CHANNEL_NORMS = {"rms": 1, "layer": 2}
 _GATE_ACTS = {"none": 0, "sigmoid": 1, "silu": 2, "tanh": 3}
-_NO_NORM = _native.ChannelNorm()
+_NO_NORM = (0, 0.0, 0, 0)
 
 
 @dataclass(frozen=True)
@@ -988,10 +988,10 @@ class ChannelNorm:
             if p is not None:
                 _check_tensor(p, f"norm {name}")
 
-    def arguments(self, channels: int, device: torch.device) -> _native.ChannelNorm:
+    def arguments(self, channels: int, device: torch.device) -> tuple:
         w = _channels_pointer(self.weight, "norm weight", channels, device)
         b = _channels_pointer(self.bias, "norm bias", channels, device)
-        return _native.ChannelNorm(_CHANNEL_NORMS[self.kind], self.eps, w, b)
+        return _CHANNEL_NORMS[self.kind], self.eps, w, b
 
 
 def _channels_pointer(p: torch.Tensor | None, name: str, channels: int, device: torch.device) -> int:
@@ -1025,6 +1025,8 @@ def _row_stride(t: torch.Tensor, name: str) -> int:
     channels = t.shape[-1]
     if t.is_contiguous():
         return channels
+    if t.dim() == 2 and t.stride(1) == 1:
+        return t.stride(0)
     if channels == 1 or t.stride(-1) == 1:
         axes = [(n, st) for n, st in zip(t.shape[:-1], t.stride()[:-1]) if n != 1]
         if all(outer == n * inner for (_, outer), (n, inner) in zip(axes, axes[1:])):
@@ -1061,7 +1063,7 @@ def _check_out(out: torch.Tensor, name: str, shape, dtype: torch.dtype, device: 
     return stride
 
 
-def _call_rows(function, args, device: torch.device, what: str) -> None:
+def _call_rows(function, args: bytes, device: torch.device, what: str) -> None:
     """A row operator's launch, on ``device``'s current stream.
 
     The stream is asked for as a plain handle: the Stream object that
@@ -1069,10 +1071,10 @@ def _call_rows(function, args, device: torch.device, what: str) -> None:
     """
     index = device.index
     if index == torch.cuda.current_device():
-        status = function(ctypes.byref(args), torch._C._cuda_getCurrentRawStream(index))
+        status = function(args, torch._C._cuda_getCurrentRawStream(index))
     else:
         with torch.cuda.device(device):
-            status = function(ctypes.byref(args), torch._C._cuda_getCurrentRawStream(index))
+            status = function(args, torch._C._cuda_getCurrentRawStream(index))
     if status != 0:
         _native.check(status, what)
 
@@ -1105,8 +1107,8 @@ def channel_norm(x: torch.Tensor, norm: ChannelNorm, *, out_dtype: torch.dtype |
     rows = out.numel() // channels
     if rows == 0:
         return out
-    args = _native.NormArgs(x.data_ptr(), out.data_ptr(), rows, x_stride, out_stride, channels,
-                            _ROW_TYPES[x.dtype], _ROW_TYPES[dtype], 0, n)
+    args = _native.pack_norm(x.data_ptr(), out.data_ptr(), rows, x_stride, out_stride, channels,
+                             _ROW_TYPES[x.dtype], _ROW_TYPES[dtype], 0, *n)
     token = None
     if PROFILE.active:
         token = PROFILE.start("channel_norm", 0.0, float(rows * channels * (x.element_size() + out.element_size())))
@@ -1188,10 +1190,10 @@ def gated_residual_join(branch: torch.Tensor, skip: torch.Tensor, *, post: Chann
         normed, normed_type = _empty_rows(branch, dtype), _ROW_TYPES[dtype]
     if rows == 0:
         return out, normed
-    args = _native.JoinArgs(branch.data_ptr(), skip.data_ptr(), _ptr(gate), out.data_ptr(), _ptr(normed), rows,
-                            branch_stride, skip_stride, gate_stride, out_stride, channels, per_sample, channels,
-                            _ROW_TYPES[branch.dtype], _ROW_TYPES[skip.dtype], normed_type, mode,
-                            _GATE_ACTS[gate_act], residual_scale, 0, scale_pointer, post_args, next_args)
+    args = _native.pack_join(branch.data_ptr(), skip.data_ptr(), _ptr(gate), out.data_ptr(), _ptr(normed), rows,
+                             branch_stride, skip_stride, gate_stride, out_stride, channels, per_sample, channels,
+                             _ROW_TYPES[branch.dtype], _ROW_TYPES[skip.dtype], normed_type, mode,
+                             _GATE_ACTS[gate_act], residual_scale, 0, scale_pointer, *post_args, *next_args)
     token = None
     if PROFILE.active:
         nbytes = (branch.element_size() + 2 * skip.element_size() + (0 if normed is None else normed.element_size())
@@ -1335,16 +1337,17 @@ def adapted_projection(x: torch.Tensor, projection: AdaptedProjection, index: to
     if rows == 0:
         return out
     lib = _native.load()
-    args = _native.ProjectArgs(x.data_ptr(), weight.data_ptr(), down.data_ptr(), projection.up.data_ptr(),
-                               projection.scales.data_ptr(), _ptr(projection.bias), index.data_ptr(), out.data_ptr(),
-                               0, rows, x_stride, out_stride, rows // index.numel(), weight_stride, shape[-1], n,
-                               adapters, rank, _ROW_TYPES[x.dtype], projection.used_rank)
-    nbytes = lib.nnb_project_workspace_bytes(ctypes.byref(args))
+    pointers = (x.data_ptr(), weight.data_ptr(), down.data_ptr(), projection.up.data_ptr(),
+                projection.scales.data_ptr(), _ptr(projection.bias), index.data_ptr(), out.data_ptr())
+    sizes = (rows, x_stride, out_stride, rows // index.numel(), weight_stride, shape[-1], n, adapters, rank,
+             _ROW_TYPES[x.dtype], projection.used_rank)
+    args = _native.pack_project(*pointers, 0, *sizes)
+    nbytes = lib.nnb_project_workspace_bytes(args)
     if nbytes < 0:
         _native.check(nbytes, "adapted_projection")
     if nbytes > 0:
         workspace = x.new_empty(nbytes, dtype=torch.uint8)
-        args.low = workspace.data_ptr()
+        args = _native.pack_project(*pointers, workspace.data_ptr(), *sizes)
     token = None
     if PROFILE.active:
         k = shape[-1]

@@ -128,6 +128,17 @@ def test_projection_workspace():
     assert load.nnb_project(None, None) == -1
 
 
+def test_packed_arguments_are_the_structures():
+    values = list(range(1, 10))
+    norm = _native.ChannelNorm(2, 0.5, 21, 22)
+    assert _native.pack_norm(*values, 2, 0.5, 21, 22) == bytes(_native.NormArgs(*values, norm))
+    values = [*range(1, 19), 0.25, 0, 23]
+    join = _native.JoinArgs(*values, norm, _native.ChannelNorm(1, 2.0, 31, 0))
+    assert _native.pack_join(*values, 2, 0.5, 21, 22, 1, 2.0, 31, 0) == bytes(join)
+    values = list(range(1, 21))
+    assert _native.pack_project(*values) == bytes(_native.ProjectArgs(*values))
+
+
 def test_structures_match_the_header(tmp_path):
     names = {"nnb_channel_norm": _native.ChannelNorm, "nnb_norm_args": _native.NormArgs,
              "nnb_join_args": _native.JoinArgs, "nnb_project_args": _native.ProjectArgs}

@@ -6,10 +6,11 @@
 // down_a has the adapter's rank of rows, up_a that many columns; both are
 // padded with zeros to a common multiple of 16.
 //
-// Low-rank rows scale_a down_a x_t come first, then, by the number of rows alone
-// (so a row's value does not depend on the rows beside it):
+// Low-rank rows scale_a down_a x_t come first, then, by sizes alone (so a row's
+// value does not depend on the rows beside it):
 //
-//  * more than 128 rows: project_low_tile_kernel (tcgen05) and project_kernel, a
+//  * more than 128 rows: project_low_tile_kernel (tcgen05; project_low_kernel
+//    where a tile may have too many adapters for it) and project_kernel, a
 //    tcgen05 GEMM over tiles of 128 rows x 64 or 128 columns, or of 256 x 256 by
 //    pairs of CTAs, whose K axis goes on past W's channels.  For every adapter
 //    among a tile's rows it appends the adapter's ranks, with the rows of other
@@ -31,9 +32,14 @@
 //          bfloat16 parts hi + lo (2^-17 of the value at most is lost; a single
 //          bfloat16 would cost the output as much as its own rounding)
 //   6-13   epilogue: TMEM -> bias -> 16-bit rows; warps 6-9 one of the two accumulators, 10-13 the other
+//   14     TMA producer of the adapters' up columns
 // W's chunks and the adapters' have rings of their own, so each producer runs
 // ahead as far as its ring allows; warps 2-5 announce the number of adapters of
-// a tile, which only the MMA issuer needs.
+// a tile to the MMA issuer, and their list to warp 14.  Tiles of many adapters
+// are bound by the latency of a stage: so each of warps 2-5 arrives for itself,
+// a row is written only where it has the stage's adapter or has to become zero
+// again, and another warp issues the copies (256 rows, 1024 -> 1024, 64 adapters
+// of rank 16: 46.2 -> 42.5 us; 320 -> 320 of rank 8: 49.1 -> 45.6 us).
 #include <cuda.h>
 #include <cudaTypedefs.h>
 #include <cuda_bf16.h>
@@ -62,7 +68,7 @@ using namespace tc;
 
 constexpr int kBadIndex = 41;  // site number of an adapter index out of range; 42-63 are waits
 
-constexpr int kThreads = 448;
+constexpr int kThreads = 480;
 constexpr int kStageA = BM * 128;
 constexpr int kRankBlock = 32;  // ranks of an adapter stage: a 128-byte row of 32 hi and 32 lo parts
 
@@ -82,7 +88,7 @@ struct Tile {
   static constexpr int kStaging = 32 * 32 * 2;  // an epilogue warp's 32 rows of 32 columns
   static constexpr int kTmem = 2 * BN;
   static constexpr int kSmem =
-      1024 + kStages * kStage + kLowStages * kLowStage + 8 * kStaging + 4 * BN * 4 + 3072;
+      1024 + kStages * kStage + kLowStages * kLowStage + 8 * kStaging + 4 * BN * 4 + 4096;
 };
 
 constexpr int kCounts = 4;  // tiles whose number of adapters may be announced ahead
@@ -146,8 +152,23 @@ __global__ void __launch_bounds__(256) align_rows_kernel(const uint16_t* x, int6
   }
 }
 
+// Two low-rank values as two bfloat16 parts each, hi + lo.  What an infinity leaves would be no number: the larger
+// of it and a bound below every true remainder (half a step of the largest value is 2^119) is that bound.
+__device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t& lo) {
+  hi = pack2(a, b, __nv_bfloat16());
+  lo = pack2(a - __uint_as_float(hi << 16), b - __uint_as_float(hi & 0xffff0000u), __nv_bfloat16());
+  asm("max.bf16x2 %0, %0, %1;" : "+r"(lo) : "r"(0xfb80fb80u));  // -2^120
+}
+
+// A row's low-rank values in the workspace, as the GEMM's stages take them: per block of 32 ranks 128 bytes, 32 hi
+// parts and 32 lo parts.
+__device__ __forceinline__ uint8_t* low_row(const nnb_project_args& a, int64_t row) {
+  return reinterpret_cast<uint8_t*>(a.low) + row * ((a.rank + kRankBlock - 1) / kRankBlock) * 128;
+}
+
 // ---------------------------------------------------------------------------
-// low[p][t][j] = scale_a sum over part p of k of down_a[j][k] x[t][k]: a warp takes four ranks of one row.
+// low[p][t][j] = scale_a sum over part p of k of down_a[j][k] x[t][k]: a warp takes four ranks of one row.  PACKED:
+// of all of k, as hi and lo parts.
 // ---------------------------------------------------------------------------
 // 32 TMEM columns of this thread's lane, asked for and waited for apart.
 __device__ __forceinline__ void tmem_load32(uint32_t taddr, uint32_t (&r)[32]) {
@@ -180,7 +201,7 @@ __device__ __forceinline__ void widen(float (&v)[8], const uint4& raw) {
   for (int i = 0; i < 8; ++i) v[i] = value(t[i]);
 }
 
-template <typename T>
+template <typename T, bool PACKED>
 __global__ void __launch_bounds__(128) project_low_kernel(const nnb_project_args a, const int part) {
   asm volatile("griddepcontrol.launch_dependents;");
   const int64_t row = blockIdx.x;
@@ -212,8 +233,16 @@ __global__ void __launch_bounds__(128) project_low_kernel(const nnb_project_args
   for (int j = 0; j < 4; ++j) {
 #pragma unroll
     for (int h = 16; h >= 1; h >>= 1) sum[j] += __shfl_xor_sync(0xffffffffu, sum[j], h);
-    if (lane == j)
-      a.low[(blockIdx.z * a.rows + row) * a.rank + j0 + j] = sum[j] * __ldg(a.scales + adapter);
+    sum[j] *= __ldg(a.scales + adapter);
+    if (!PACKED && lane == j) a.low[(blockIdx.z * a.rows + row) * a.rank + j0 + j] = sum[j];
+  }
+  if (PACKED && lane == 0) {
+    uint2 hi, lo;
+    split2(sum[0], sum[1], hi.x, lo.x);
+    split2(sum[2], sum[3], hi.y, lo.y);
+    uint8_t* out = low_row(a, row) + j0 / kRankBlock * 128 + j0 % kRankBlock * 2;
+    *reinterpret_cast<uint2*>(out) = hi;
+    *reinterpret_cast<uint2*>(out + 64) = lo;
   }
 }
 
@@ -329,20 +358,20 @@ __device__ __forceinline__ void cluster_barrier() {
   asm volatile("barrier.cluster.arrive.release;\n barrier.cluster.wait.acquire;" ::: "memory");
 }
 
-// Barrier of four warps; true when every one of their threads passed `ok`.  Barrier 1: the adapter warps.
-template <int ID>
-__device__ __forceinline__ bool four_warps_barrier(bool ok) {
+// Barrier of THREADS threads; true when every one of them passed `ok`.
+template <int ID, int THREADS = 128>
+__device__ __forceinline__ bool warps_barrier(bool ok) {
   uint32_t all;
   asm volatile(
-      "{\n .reg .pred p, q;\n setp.ne.u32 p, %1, 0;\n barrier.cta.red.and.pred q, %2, 128, p;\n"
+      "{\n .reg .pred p, q;\n setp.ne.u32 p, %1, 0;\n barrier.cta.red.and.pred q, %2, %3, p;\n"
       " selp.u32 %0, 1, 0, q;\n}\n"
       : "=r"(all)
-      : "r"((uint32_t)ok), "n"(ID)
+      : "r"((uint32_t)ok), "n"(ID), "n"(THREADS)
       : "memory");
   return all != 0;
 }
 
-__device__ __forceinline__ bool adapter_barrier(bool ok) { return four_warps_barrier<1>(ok); }
+__device__ __forceinline__ bool adapter_barrier(bool ok) { return warps_barrier<1>(ok); }
 
 // One thread of a converged warp.  The warp walks a kernel's loops together and this thread issues: with loops of
 // a single lane the compiler takes every descriptor through a vector register, and an MMA takes 120 cycles to
@@ -421,17 +450,8 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, float (&v)[16]) {
   for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
 }
 
-// Two low-rank values as two bfloat16 parts each, hi + lo.  What an infinity leaves would be no number: the larger
-// of it and a bound below every true remainder (half a step of the largest value is 2^119) is that bound.
-__device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t& lo) {
-  hi = pack2(a, b, __nv_bfloat16());
-  lo = pack2(a - __uint_as_float(hi << 16), b - __uint_as_float(hi & 0xffff0000u), __nv_bfloat16());
-  asm("max.bf16x2 %0, %0, %1;" : "+r"(lo) : "r"(0xfb80fb80u));  // -2^120
-}
-
 // ---------------------------------------------------------------------------
-// Low-rank rows of more than 128 rows, as the GEMM's stages take them: per row
-// and block of 32 ranks 128 bytes, 32 hi parts and 32 lo parts.
+// Low-rank rows of many rows, as the GEMM's stages take them.
 //
 // A cluster takes 128 rows, a CTA of it a part of the channels: x's chunk
 // against the down rows of the tile's adapters, as many as fit the MMA's
@@ -440,11 +460,6 @@ __device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t&
 // coming while one starts or ends.
 // ---------------------------------------------------------------------------
 constexpr int kLowThreads = 192;
-
-// A row's low-rank values in the workspace.
-__device__ __forceinline__ uint8_t* low_row(const nnb_project_args& a, int64_t row) {
-  return reinterpret_cast<uint8_t*>(a.low) + row * ((a.rank + kRankBlock - 1) / kRankBlock) * 128;
-}
 
 struct LowMaps {
   CUtensorMap x, down;
@@ -723,8 +738,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* drain = count_empty + kCounts;
   volatile int* counts = reinterpret_cast<volatile int*>(drain + 1);  // adapters of the tiles announced
   volatile int* heads = counts + kCounts;                             // the adapter warps' lists
-  volatile int* listed = heads + 4 + C::kRows;                        // the tile's adapters, ascending
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(const_cast<int*>(listed + C::kRows));
+  volatile int* lists = heads + 4 + C::kRows;  // by the tile's parity: its number of adapters, and they ascending
+  constexpr int kList = 1 + C::kRows;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(const_cast<int*>(lists + 2 * kList));
   int* abort_flag = reinterpret_cast<int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -742,7 +758,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(smem_u32(&empty[s]), 1);
     }
     for (int s = 0; s < SL; ++s) {
-      mbar_init(smem_u32(&low_full[s]), C::kPeers);  // the adapter warps of both CTAs
+      mbar_init(smem_u32(&low_full[s]), 4 * C::kPeers + 1);  // the adapter warps of both CTAs, and the copies
       mbar_init(smem_u32(&low_empty[s]), 1);
     }
     for (int i = 0; i < 2; ++i) {
@@ -884,11 +900,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     // The low-rank rows are the previous kernel's, which may still run; every CTA waits for its end.
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int r = threadIdx.x - 64;
-    const bool leader = r == 0;
     Ring<SL> ring;
     Ring<kCounts> counted;
-    int issued = 0;
-    bool alive = true;  // this thread; `all`: the four warps, which go on together or stop together
+    uint32_t written = ~0u;  // stages whose row is not zero, a bit each
+    bool alive = true;       // this warp; `all`: every one that takes part in the lists, so that none waits for another
     bool all = true;
     // A tile's rows are asked for their adapters, and for the 128 bytes of their first block of ranks, while the
     // tile before is filled in (whether the row has an adapter or not, so that neither load waits for the other);
@@ -921,55 +936,83 @@ __global__ void __launch_bounds__(kThreads, 1)
       next_low = nullptr;
       ask(it + 1);
       if (mine < 0) fetch(next_low);
-      const int count = list_adapters<C::kRows>(mine, other, r, heads, listed);
-      if (leader && cta == 0) {
-        alive = mbar_wait(smem_u32(&count_empty[counted.s]), counted.phase ^ 1, abort_flag, 49);
-        counts[counted.s] = count;
-        mbar_arrive(smem_u32(&count_full[counted.s]));
+      volatile int* list = lists + (it & 1) * kList;
+      const int count = list_adapters<C::kRows>(mine, other, r, heads, list + 1);
+      if (r == 0) list[0] = count;
+      if (warp == 2 && cta == 0) {
+        const bool free = mbar_wait(smem_u32(&count_empty[counted.s]), counted.phase ^ 1, abort_flag, 49);
+        alive = __all_sync(0xffffffffu, alive && free);
+        if (lane == 0) {
+          counts[counted.s] = count;
+          mbar_arrive(smem_u32(&count_full[counted.s]));
+        }
       }
       counted.next();
-      all = adapter_barrier(alive);  // also makes the list visible
-      for (int i = 0; i < count && all; ++i) {
-        const int adapter = listed[i];
-        const bool own = mine == adapter;
-        for (int block = 0; block < blocks && all; ++block) {
-          alive = alive && mbar_wait(smem_u32(&low_empty[ring.s]), ring.phase ^ 1, abort_flag, 50);
-          uint8_t* at = low_stages + ring.s * C::kLowStage;
-          const uint32_t bar = smem_u32(&low_full[ring.s]);
-          if (leader && alive) {
-            const uint32_t dst = smem_u32(at) + kStageA;
-            const int j0 = block * kRankBlock;
-            if (cta == 0) mbar_expect_tx(bar, C::kPlane * (kF16 ? 2 : 1) * C::kPeers);
-            if constexpr (PAIR) {
-              const uint32_t first = in_first_cta(bar);
-              const int col = t.col0 + cta * (BN / 2);
-              tma_load_3d_pair(dst, &maps.up, j0, col, adapter, first);
-              if constexpr (kF16) tma_load_3d_pair(dst + C::kPlane, &maps.up, a.rank + j0, col, adapter, first);
-            } else {
-              tma_load_3d(dst, &maps.up, j0, t.col0, adapter, bar);
-              if constexpr (kF16) tma_load_3d(dst + C::kPlane, &maps.up, a.rank + j0, t.col0, adapter, bar);
-            }
-            ++issued;
-          }
-          if (alive) {
-            uint4* line = reinterpret_cast<uint4*>(at + r * 128);
+      all = warps_barrier<4, 160>(alive);  // also makes the list visible
+      if (!all) break;
+      for (int i = 0; i < count && alive; ++i) {
+        const bool own = mine == list[1 + i];
+        for (int block = 0; block < blocks; ++block) {
+          alive = __all_sync(0xffffffffu, mbar_wait(smem_u32(&low_empty[ring.s]), ring.phase ^ 1, abort_flag, 50));
+          if (!alive) break;
+          if (own || (written >> ring.s & 1)) {
+            uint4* line = reinterpret_cast<uint4*>(low_stages + ring.s * C::kLowStage + r * 128);
 #pragma unroll
             for (int c = 0; c < 8; ++c) line[c ^ (r & 7)] = own ? v[c] : make_uint4(0, 0, 0, 0);
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            written = own ? written | 1u << ring.s : written & ~(1u << ring.s);
+          }
+          __syncwarp();
+          if (lane == 0) {
+            if constexpr (PAIR)
+              mbar_arrive_first(smem_u32(&low_full[ring.s]));
+            else
+              mbar_arrive(smem_u32(&low_full[ring.s]));
           }
           if (own) fetch(block + 1 < blocks ? low + (block + 1) * 8 : next_low);
-          all = adapter_barrier(alive);
-          if (leader && alive) {  // also on the way out, so that the copy's phase completes
-            if constexpr (PAIR)
-              mbar_arrive_first(bar);
-            else
-              mbar_arrive(bar);
-          }
           ring.next();
         }
       }
     }
-    if (leader && *reinterpret_cast<volatile int*>(abort_flag))
+    __syncwarp();
+  } else if (warp == 14) {
+    // -------------------------- TMA producer of up columns --------------------
+    const bool issuer = elect_one();
+    Ring<SL> ring;
+    int issued = 0;
+    bool alive = true;
+    for (int it = 0; it < my_tiles; ++it) {
+      const TileAt t = tile_at<C>(first_tile + it * tile_step, row_tiles, col_tiles, BN);
+      const int col = t.col0 + cta * (BN / 2);
+      if (!warps_barrier<4, 160>(alive)) break;
+      const volatile int* list = lists + (it & 1) * kList;
+      const int count = list[0];
+      for (int i = 0; i < count && alive; ++i) {
+        const int adapter = list[1 + i];
+        for (int block = 0; block < blocks; ++block) {
+          alive = __all_sync(0xffffffffu, mbar_wait(smem_u32(&low_empty[ring.s]), ring.phase ^ 1, abort_flag, 50));
+          if (!alive) break;
+          const uint32_t bar = smem_u32(&low_full[ring.s]);
+          const uint32_t dst = smem_u32(low_stages + ring.s * C::kLowStage) + kStageA;
+          const int j0 = block * kRankBlock;
+          if (issuer) {
+            if (cta == 0) mbar_arrive_expect_tx(bar, C::kPlane * (kF16 ? 2 : 1) * C::kPeers);
+            if constexpr (PAIR) {
+              const uint32_t first = in_first_cta(bar);
+              tma_load_3d_pair(dst, &maps.up, j0, col, adapter, first);
+              if constexpr (kF16) tma_load_3d_pair(dst + C::kPlane, &maps.up, a.rank + j0, col, adapter, first);
+            } else {
+              tma_load_3d(dst, &maps.up, j0, col, adapter, bar);
+              if constexpr (kF16) tma_load_3d(dst + C::kPlane, &maps.up, a.rank + j0, col, adapter, bar);
+            }
+          }
+          __syncwarp();
+          ring.next();
+          ++issued;
+        }
+      }
+    }
+    if (issuer && *reinterpret_cast<volatile int*>(abort_flag))  // wait (bounded) for the copies still in flight
       for (int g = max(0, issued - SL); g < issued; ++g)
         mbar_wait(smem_u32(&low_full[g % SL]), (uint32_t)(g / SL) & 1, abort_flag, 51, false);
     __syncwarp();
@@ -989,7 +1032,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int c = quarter * 32 + lane; c < BN; c += 128)
         bias[c] = a.bias != nullptr && t.col0 + c < a.n ? a.bias[t.col0 + c] : 0.f;
       const bool ok = mbar_wait(smem_u32(&acc_full[acc]), (uint32_t)(it >> 1) & 1, abort_flag, 52);
-      if (!(acc == 0 ? four_warps_barrier<2>(ok) : four_warps_barrier<3>(ok))) break;
+      if (!(acc == 0 ? warps_barrier<2>(ok) : warps_barrier<3>(ok))) break;
       fence_after();
       const uint32_t src = tmem + acc * BN + ((uint32_t)quarter << 21);
       const int64_t row0 = t.row0 + cta * BM + quarter * 32;
@@ -1359,6 +1402,8 @@ bool rows_in_place(const nnb_project_args& a) {
          (a.rows == 1 || (a.x_stride % 8 == 0 && a.x_stride >= a.k));
 }
 
+// (Two million rows, by this kernel and by tiles: 32 -> 32 channels of rank 8 54 and 533 us, 64 -> 64 of rank 16 146
+// and 564, 128 -> 128 of rank 16 455 and 616.)
 bool narrow(const nnb_project_args& a) { return a.k <= 128 && a.n <= 128; }
 
 // Plans are made for a whole B200, so that the workspace's size needs no device.
@@ -1374,16 +1419,33 @@ int few_split(const nnb_project_args& a) {
 
 // How the low-rank rows are computed: by tiles or by rows, in how many parts of the channels.
 struct LowPlan {
-  bool few;   // up to one tile of rows
-  int parts;  // partial sums (few), or CTAs of a cluster
-  int part;   // channels (few) or chunks of 64 of a part
+  bool few;   // up to one tile of rows: partial sums for project_few_kernel (128 rows, 4096 -> 4096 of rank 16, by it
+              // and by tiles: 1 adapter 20.1 and 21.3 us, 64 adapters 21.7 and 82.1; 256 rows: 50 to 64 and 24 to 55)
+  bool dots;  // by rows, packed
+  int parts;  // partial sums (few), or CTAs of a cluster (tiles)
+  int part;   // channels (few, dots) or chunks of 64 (tiles) of a part
 };
+
+// By rows beyond a tile too, where a tile may hold so many adapters that its passes over them take longer: some 0.8 us
+// for 64 ranks against 250 ns for a million products.  Whole calls by tiles and by rows: 256 rows, 1024 -> 1024, rank
+// 16, 64 adapters 42.2 and 22.0 us, 8 adapters 13.4 and 11.1; 160 rows, 4096 -> 4096, 64 adapters 72.5 and 48.3 us; 1024
+// rows of them, near the bound, 56.8 and 56.9.
+bool low_by_rows(const nnb_project_args& a) {
+  const int64_t ranks = std::min<int64_t>(a.adapters, BM) * a.rank;
+  return a.rows <= 8 * BM && a.rows * a.rank * a.k / 4000 < ranks * 800 / 64;
+}
 
 // Enough parts that some 300 CTAs run (two per SM; of rows, whose CTAs are small, some 1000), of at least 512
 // channels (two loads of a lane) or four chunks, and no more than eight.
 LowPlan low_plan(const nnb_project_args& a) {
   LowPlan p;
   p.few = a.rows <= BM;
+  p.dots = !p.few && low_by_rows(a);
+  if (p.dots) {
+    p.parts = 1;
+    p.part = a.k;
+    return p;
+  }
   if (p.few) {
     // Every tile of columns would compute a share of the rows again; up to 128 products a thread that is less than a
     // launch (one row of 320 -> 320 channels, rank 8).
@@ -1453,7 +1515,12 @@ int launch_low(const nnb_project_args& a, const LowPlan& plan, int dev, cudaStre
   constexpr bool kF16 = !std::is_same<T, __nv_bfloat16>::value;
   if (plan.few) {
     if (plan.parts == 0) return NNB_OK;
-    project_low_kernel<T><<<dim3((unsigned)a.rows, a.rank / 16, plan.parts), 128, 0, stream>>>(a, plan.part);
+    project_low_kernel<T, false><<<dim3((unsigned)a.rows, a.rank / 16, plan.parts), 128, 0, stream>>>(a, plan.part);
+    NNB_LAUNCH_CHECK();
+    return NNB_OK;
+  }
+  if (plan.dots) {
+    project_low_kernel<T, true><<<dim3((unsigned)a.rows, a.rank / 16), 128, 0, stream>>>(a, plan.part);
     NNB_LAUNCH_CHECK();
     return NNB_OK;
   }
@@ -1560,8 +1627,8 @@ int tile_columns(const nnb_project_args& a, int sms) {
 }
 
 // ---------------------------------------------------------------------------
-// Narrow projections (up to 128 channels on either side), bound by HBM: a warp
-// carries 16 M rows from x to out in registers, low-rank values included.
+// Narrow projections (up to 128 channels on either side): a warp carries 16 M
+// rows from x to out in registers, low-rank values included.
 //
 // mma.sync fragments, with the axes permuted so that every thread's share is
 // contiguous: of 32 channels thread q of a row's four holds 8q..8q+7 (one
@@ -1569,8 +1636,10 @@ int tile_columns(const nnb_project_args& a, int sms) {
 // columns 8q..8q+7 (one 16-byte store), of 16 ranks 4q..4q+3.  The low-rank
 // accumulators are the A fragments of the product with up_a, as two bfloat16
 // parts; rows of other requests are zeroed there, once per adapter among the
-// warp's rows.  The tensor rate is no bound here (some 20 operations per byte),
-// so the plain warp MMAs serve, and no stage or barrier stands between x and out.
+// warp's rows.  No stage or barrier stands between x and out.  32 channels are
+// bound by HBM (82% of a copy's rate); from 64 on the rate of these MMAs and the
+// registers bound it (64 channels 57%, 128 channels 37%), still ahead of tiles,
+// whose K axis is padded to whole chunks and whose epilogue goes through TMEM.
 // ---------------------------------------------------------------------------
 // d = a b + c of 16 rows, 8 columns and 16 channels.
 __device__ __forceinline__ void warp_mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, float c0,

@@ -109,6 +109,9 @@ SHAPES = [  # rows, k, n, ranks, index
     (3000, 40, 24, [5], "none"),
     (700, 4096, 16, [16, 16], "runs"),
     (260, 16, 2000, [16, 16, 2], "mixed"),
+    (256, 320, 700, [16, 9] * 40, "mixed"),    # many adapters in tiles of every width
+    (1500, 256, 2000, [40, 9] * 20, "mixed"),
+    (1100, 192, 8000, [20] * 50, "mixed"),
     (100, 4096, 320, [16] * 20, "mixed"),      # up to 128 rows: clusters of every size, shares of few and many rows
     (128, 640, 129, [144, 80], "mixed"),
     (3, 192, 4000, [24, 256], "mixed"),

@@ -526,7 +526,7 @@ int norm_by_channels(const nnb_norm_args& a, bool aligned, cudaStream_t stream) 
 
 // A join, with registers for three operands and their successors, does better with one chunk and more threads where
 // both fit (512 channels: 64 x 1 119 us, 32 x 2 140 us; 2560: 320 x 1 92%, 160 x 2 79%), but for lengths at which an SM
-// would hold one block of them alone (3072: 192 x 2 80%, 384 x 1 71%; 4096: 256 x 2 146 us, 512 x 1 161 us; 6144:
+// would hold one block of them alone (2816: 192 x 2 80%, 384 x 1 71%; 4096: 256 x 2 146 us, 512 x 1 161 us; 6144:
 // 384 x 2 75%, 768 x 1 74%).
 template <typename TS, typename TB>
 int join_by_channels(const nnb_join_args& a, bool aligned, cudaStream_t stream) {

@@ -2,8 +2,8 @@
 
 Tolerances are sums of roundings, derived before the first run.  ``U`` is half
 a float32 step.  A row's sums run over at most 32 values in a thread, then 5
-shuffles and 16 warps, so a sum of C terms is off by at most 53 U times the
-sum of their magnitudes; products, the root and the quotient add a few U.
+shuffles and 16 warps (or 16 values and 32 warps, summed by fours), so a sum of
+C terms is off by at most 53 U times the sum of their magnitudes; products, the root and the quotient add a few U.
 """
 
 from __future__ import annotations
@@ -207,6 +207,31 @@ def test_join(cuda_device, channels, join):
         p = None if post is None else (post, *params(rng, channels, cuda_device, post == "layer"), 1e-5)
         n = None if following is None else (following, *params(rng, channels, cuda_device), 1e-6)
         check_join(branch, skip, p, g, act, scale, 0.7, n, None if ntype is None else TYPES[ntype])
+
+
+# One length for every number of threads a row and elements a thread, aligned and not, with more rows than the GPU
+# holds at once.
+@pytest.mark.parametrize("channels", [
+    40, 72, 136, 264, 400, 640, 776, 1280, 1536, 1544, 2304, 2816, 3096, 4560, 5128, 6152, 8200, 10248, 12296,
+    13, 21, 37, 45, 61, 75, 91, 121, 150, 189, 251, 301, 381, 501, 701, 1001, 1201, 1501, 2001, 2501, 3001, 4001, 4501,
+    5001, 6001, 8001, 10001, 12001])
+def test_every_number_of_threads(cuda_device, channels):
+    rows = max(450, min(5000, 1_200_000 // channels))
+    gen = torch.Generator(device=cuda_device).manual_seed(channels)
+
+    def values(shape, dtype):
+        return torch.randn(shape, device=cuda_device, generator=gen).add_(0.3).to(TYPES[dtype])
+
+    def norm(kind):
+        return kind, values(channels, "f32"), values(channels, "f32"), 1e-5
+
+    for dtype, kind, out in (("f32", "rms", "bf16"), ("f16", "layer", "f32")):
+        _, weight, bias, eps = norm(kind)
+        check_norm(values((rows, channels), dtype), kind, weight, bias, eps, TYPES[out])
+    for dtype, btype, gate in (("f32", "bf16", (rows, channels)), ("bf16", "bf16", (rows, 1)), ("f32", "f32", None)):
+        check_join(values((rows, channels), btype), values((rows, channels), dtype), norm("layer"),
+                   None if gate is None else values(gate, btype), "none" if gate is None else "sigmoid",
+                   values(channels, "f32"), 0.7, norm("rms"), None)
 
 
 @pytest.mark.parametrize("channels", [24, 333, 1024])

@@ -1351,8 +1351,11 @@ def adapted_projection(x: torch.Tensor, projection: AdaptedProjection, index: to
     token = None
     if PROFILE.active:
         k = shape[-1]
+        # rows that are not aligned are copied first; what else the workspace holds are low-rank rows
+        copied = x.data_ptr() % 16 != 0 or (rows > 1 and (x_stride % 8 != 0 or x_stride < k))
         token = PROFILE.start("adapted_projection", 2.0 * rows * (n * k + rank * (n + k)),
-                              2.0 * (rows * (n + k) + n * k), launches=2 if nbytes > 0 else 1)
+                              2.0 * (rows * (n + k) + n * k),
+                              launches=1 + copied + (nbytes > copied * rows * weight_stride * 2))
     _call_rows(lib.nnb_project, args, device, "adapted_projection")
     PROFILE.stop(token)
     return out

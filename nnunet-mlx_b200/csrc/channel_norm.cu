@@ -58,7 +58,7 @@ struct Map {
   static constexpr int kThreads = TPR <= 32 ? 128 : TPR;
   static constexpr int kRows = kThreads / TPR;       // of a block
   static constexpr int kWarps = (TPR + 31) / 32;     // of a row
-  static constexpr int kSlots = TPR * NCH * E;       // channels
+  [[maybe_unused]] static constexpr int kSlots = TPR * NCH * E;  // channels
   static constexpr bool kHeld = NCH == 1;            // per-channel parameters stay in registers
   static constexpr bool kAhead = NCH <= 3;           // the next row's loads before the present one's sums
 

@@ -32,7 +32,7 @@
 //          bfloat16 parts hi + lo (2^-17 of the value at most is lost; a single
 //          bfloat16 would cost the output as much as its own rounding)
 //   6-13   epilogue: TMEM -> bias -> 16-bit rows; warps 6-9 one of the two accumulators, 10-13 the other
-//   14     TMA producer of the adapters' up columns
+//   14     TMA producer of the adapters' up columns, and of the low-rank rows where a tile has one adapter
 // W's chunks and the adapters' have rings of their own, so each producer runs
 // ahead as far as its ring allows; warps 2-5 announce the number of adapters of
 // a tile to the MMA issuer, and their list to warp 14.  Tiles of many adapters
@@ -106,7 +106,7 @@ struct Ring {
 };
 
 struct Maps {
-  CUtensorMap x, weight, up;
+  CUtensorMap x, weight, up, low;
 };
 
 __device__ __forceinline__ float value(__nv_bfloat16 v) { return __bfloat162float(v); }
@@ -406,9 +406,11 @@ __device__ __forceinline__ void chunk_mmas(uint32_t d, uint64_t x, uint64_t w, u
 
 // The adapters among a tile's rows in ascending order, by the four adapter warps (thread r holds row r's in
 // `mine` and a pair's other row's in `other`, -1 for none); returns their number.  Each warp lists its own, and
-// every thread merges the four lists.  `heads`: 4 counts, then 4 lists of ROWS / 4.
+// every thread merges the four lists.  `any_idle`: whether one of the threads passed `idle`.  `heads`: 4 counts (and
+// idle << 16), then 4 lists of ROWS / 4.
 template <int ROWS>
-__device__ __forceinline__ int list_adapters(int mine, int other, int r, volatile int* heads, volatile int* listed) {
+__device__ __forceinline__ int list_adapters(int mine, int other, int r, volatile int* heads, volatile int* listed,
+                                             bool idle, bool& any_idle) {
   constexpr int kList = ROWS / 4;
   const int warp = r >> 5;
   volatile int* own = heads + 4 + warp * kList;
@@ -419,10 +421,13 @@ __device__ __forceinline__ int list_adapters(int mine, int other, int r, volatil
     if ((r & 31) == 0) own[count] = low;
     ++count;
   }
-  if ((r & 31) == 0) heads[warp] = count;
+  idle = __any_sync(0xffffffffu, idle);
+  if ((r & 31) == 0) heads[warp] = count | (int)idle << 16;
   adapter_barrier(true);
   int at[4] = {0, 0, 0, 0}, total = 0;
-  const int counts[4] = {heads[0], heads[1], heads[2], heads[3]};
+  const int words[4] = {heads[0], heads[1], heads[2], heads[3]};
+  const int counts[4] = {words[0] & 0xffff, words[1] & 0xffff, words[2] & 0xffff, words[3] & 0xffff};
+  any_idle = (words[0] | words[1] | words[2] | words[3]) >> 16;
   int next[4];
 #pragma unroll
   for (int w = 0; w < 4; ++w) next[w] = counts[w] > 0 ? heads[4 + w * kList] : INT_MAX;
@@ -529,7 +534,8 @@ __global__ void __launch_bounds__(kLowThreads, 2)
   if (warp >= 2) {
     if (row0 + r < a.rows) mine = row_adapter(a, row0 + r);
     scales[r] = mine < 0 ? -INFINITY : __ldg(a.scales + mine);
-    const int count = list_adapters<BM>(mine, -1, r, heads, listed);
+    bool any_idle;
+    const int count = list_adapters<BM>(mine, -1, r, heads, listed, false, any_idle);
     if (r == 0) *list_count = count;
   }
   fence_before();
@@ -905,9 +911,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint32_t written = ~0u;  // stages whose row is not zero, a bit each
     bool alive = true;       // this warp; `all`: every one that takes part in the lists, so that none waits for another
     bool all = true;
-    // A tile's rows are asked for their adapters, and for the 128 bytes of their first block of ranks, while the
-    // tile before is filled in (whether the row has an adapter or not, so that neither load waits for the other);
-    // each next block is asked for when the one before has been written.
+    // A tile whose rows all have one adapter takes their low-rank rows as they lie, by a copy of warp 14 (32768 rows,
+    // 160 -> 640, four requests: 33.1 -> 28.5 us; 12427 rows, 32 -> 3200 of rank 58: 55.4 -> 47.5 us).  Otherwise
+    // rows are asked for the 128 bytes of their first block of ranks while the tile before is filled in (whether the
+    // row has an adapter or not, so that this load and the index's do not wait for one another), and for each next
+    // block when the one before has been written.
     int next_mine, next_other;
     const uint4 *low = nullptr, *next_low;
     uint4 v[8];
@@ -929,16 +937,21 @@ __global__ void __launch_bounds__(kThreads, 1)
     next_low = nullptr;
     ask(0);
     fetch(next_low);
+    const uint4* held = next_low;  // what v holds
     for (int it = 0; it < my_tiles && all; ++it) {
       const TileAt t = tile_at<C>(first_tile + it * tile_step, row_tiles, col_tiles, BN);
       const int mine = checked_adapter(a, next_mine), other = checked_adapter(a, next_other);
       low = next_low;
       next_low = nullptr;
       ask(it + 1);
-      if (mine < 0) fetch(next_low);
       volatile int* list = lists + (it & 1) * kList;
-      const int count = list_adapters<C::kRows>(mine, other, r, heads, list + 1);
-      if (r == 0) list[0] = count;
+      const int64_t row = t.row0 + cta * BM + r, peer_row = t.row0 + (cta ^ 1) * BM + r;
+      const bool idle = (mine < 0 && row < a.rows) || (PAIR && other < 0 && peer_row < a.rows);
+      bool any_idle;
+      const int count = list_adapters<C::kRows>(mine, other, r, heads, list + 1, idle, any_idle);
+      const bool one = count == 1 && !any_idle;
+      if (r == 0) list[0] = count | (int)one << 16;
+      if (!one && mine < 0) fetch(held = next_low);
       if (warp == 2 && cta == 0) {
         const bool free = mbar_wait(smem_u32(&count_empty[counted.s]), counted.phase ^ 1, abort_flag, 49);
         alive = __all_sync(0xffffffffu, alive && free);
@@ -955,7 +968,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int block = 0; block < blocks; ++block) {
           alive = __all_sync(0xffffffffu, mbar_wait(smem_u32(&low_empty[ring.s]), ring.phase ^ 1, abort_flag, 50));
           if (!alive) break;
-          if (own || (written >> ring.s & 1)) {
+          if (one) {
+            written |= 1u << ring.s;
+          } else if (own || (written >> ring.s & 1)) {
+            if (own && held != low + block * 8) fetch(held = low + block * 8);
             uint4* line = reinterpret_cast<uint4*>(low_stages + ring.s * C::kLowStage + r * 128);
 #pragma unroll
             for (int c = 0; c < 8; ++c) line[c ^ (r & 7)] = own ? v[c] : make_uint4(0, 0, 0, 0);
@@ -969,14 +985,15 @@ __global__ void __launch_bounds__(kThreads, 1)
             else
               mbar_arrive(smem_u32(&low_full[ring.s]));
           }
-          if (own) fetch(block + 1 < blocks ? low + (block + 1) * 8 : next_low);
+          if (own && !one) fetch(held = block + 1 < blocks ? low + (block + 1) * 8 : next_low);
           ring.next();
         }
       }
     }
     __syncwarp();
   } else if (warp == 14) {
-    // -------------------------- TMA producer of up columns --------------------
+    // ------------- TMA producer of up columns, and of low-rank rows -----------
+    asm volatile("griddepcontrol.wait;\n fence.proxy.async;" ::: "memory");
     const bool issuer = elect_one();
     Ring<SL> ring;
     int issued = 0;
@@ -986,22 +1003,26 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int col = t.col0 + cta * (BN / 2);
       if (!warps_barrier<4, 160>(alive)) break;
       const volatile int* list = lists + (it & 1) * kList;
-      const int count = list[0];
+      const int count = list[0] & 0xffff;
+      const bool one = list[0] >> 16;
       for (int i = 0; i < count && alive; ++i) {
         const int adapter = list[1 + i];
         for (int block = 0; block < blocks; ++block) {
           alive = __all_sync(0xffffffffu, mbar_wait(smem_u32(&low_empty[ring.s]), ring.phase ^ 1, abort_flag, 50));
           if (!alive) break;
           const uint32_t bar = smem_u32(&low_full[ring.s]);
-          const uint32_t dst = smem_u32(low_stages + ring.s * C::kLowStage) + kStageA;
+          const uint32_t rows_at = smem_u32(low_stages + ring.s * C::kLowStage), dst = rows_at + kStageA;
           const int j0 = block * kRankBlock;
           if (issuer) {
-            if (cta == 0) mbar_arrive_expect_tx(bar, C::kPlane * (kF16 ? 2 : 1) * C::kPeers);
+            if (cta == 0)
+              mbar_arrive_expect_tx(bar, (C::kPlane * (kF16 ? 2 : 1) + (one ? kStageA : 0)) * C::kPeers);
             if constexpr (PAIR) {
               const uint32_t first = in_first_cta(bar);
+              if (one) tma_load_2d_pair(rows_at, &maps.low, j0 * 2, (int)t.row0 + cta * BM, first);
               tma_load_3d_pair(dst, &maps.up, j0, col, adapter, first);
               if constexpr (kF16) tma_load_3d_pair(dst + C::kPlane, &maps.up, a.rank + j0, col, adapter, first);
             } else {
+              if (one) tma_load_2d(rows_at, &maps.low, j0 * 2, (int)t.row0, bar);
               tma_load_3d(dst, &maps.up, j0, col, adapter, bar);
               if constexpr (kF16) tma_load_3d(dst + C::kPlane, &maps.up, a.rank + j0, col, adapter, bar);
             }
@@ -1602,6 +1623,13 @@ int launch_tiles(const nnb_project_args& a, int sms, int dev, cudaStream_t strea
     const cuuint64_t strides[2] = {width * 2, width * 2 * (cuuint64_t)a.n};
     const cuuint32_t box[3] = {kRankBlock, BN / C::kPeers, 1};
     if (const int rc = encode(&maps.up, false, 3, a.up, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_64B)) return rc;
+  }
+  {
+    const cuuint64_t width = (a.rank + kRankBlock - 1) / kRankBlock * 64;
+    const cuuint64_t dims[2] = {width, (cuuint64_t)a.rows};
+    const cuuint64_t strides[1] = {width * 2};
+    const cuuint32_t box[2] = {64, BM};
+    if (const int rc = encode(&maps.low, false, 2, a.low, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B)) return rc;
   }
   const int64_t tiles = (a.rows + C::kRows - 1) / C::kRows * ((a.n + BN - 1) / BN);
   NNB_REQUIRE(tiles < (int64_t)1 << 30, "project: %lld tiles", (long long)tiles);

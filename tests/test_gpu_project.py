@@ -140,6 +140,19 @@ def test_projection(cuda_device, shape, dtype):
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("n,ranks", [(48, [16, 3]), (264, [40, 9, 64]), (1400, [24] * 5)])
+def test_tiles_of_one_adapter_beside_tiles_of_several(cuda_device, dtype, n, ranks):
+    rng = np.random.default_rng(n)
+    rows, k = 40_001, 136
+    runs = [np.full(rng.choice([1, 64, 128, 256, 300, 1024]), rng.integers(-1, len(ranks))) for _ in range(400)]
+    index = torch.from_numpy(np.concatenate(runs)[:rows].astype(np.int32)).to(cuda_device)
+    assert index.numel() == rows
+    check(make_rows(rng, (rows, k), dtype, cuda_device), problem(rng, k, n, ranks, dtype, cuda_device), index)
+    one = torch.full((rows,), len(ranks) - 1, dtype=torch.int32, device=cuda_device)
+    check(make_rows(rng, (rows, k), dtype, cuda_device), problem(rng, k, n, ranks, dtype, cuda_device), one)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
 def test_index_per_sample(cuda_device, dtype):
     rng = np.random.default_rng(1)
     for shape, k, n in (((3, 5, 6, 7), 32, 32), ((2, 40, 50), 64, 200), ((2, 3, 4), 40, 8), ((5, 100), 32, 320)):

@@ -58,10 +58,11 @@ struct Map {
   static constexpr int kThreads = TPR <= 32 ? 128 : TPR;
   static constexpr int kRows = kThreads / TPR;       // of a block
   static constexpr int kWarps = (TPR + 31) / 32;     // of a row
-  [[maybe_unused]] static constexpr int kSlots = TPR * NCH * E;  // channels
   static constexpr bool kHeld = NCH == 1;            // per-channel parameters stay in registers
   static constexpr bool kAhead = NCH <= 3;           // the next row's loads before the present one's sums
 
+  // Channels that a row may have.
+  static constexpr int slots() { return TPR * NCH * E; }
   // Channel of element j of chunk ch.
   static __device__ __forceinline__ int channel(int ch, int j, int lane) {
     return ALIGNED ? (ch * TPR + lane) * 8 + j : (ch * E + j) * TPR + lane;
@@ -471,7 +472,7 @@ int first_that_holds(const L& launch) {
   if constexpr (sizeof...(Rest) == 0) {
     return launch.template run<M>();
   } else {
-    if (launch.a.channels <= M::kSlots) return launch.template run<M>();
+    if (launch.a.channels <= M::slots()) return launch.template run<M>();
     return first_that_holds<Rest...>(launch);
   }
 }

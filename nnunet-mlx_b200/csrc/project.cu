@@ -83,10 +83,10 @@ struct Tile {
   static constexpr int kStage = kStageA + kStageB;
   static constexpr int kPlane = BN / kPeers * 64;  // one part of up: 64-byte rows of 32 ranks
   static constexpr int kLowStage = kStageA + kPlane * (kF16 ? 2 : 1);
-  static constexpr int kStages = 4;  // as shared memory allows
-  // Narrow tiles are those of few rows, whose adapters may be many: 4 of their stages and 4 of W's rather than 2 and 6
-  // (256 rows of 64 adapters of rank 64, 1024 -> 1024: 70 -> 65 us; one adapter a tile: the same).
-  static constexpr int kLowStages = BN == 64 ? 4 : 2;
+  // As shared memory allows.  (Narrow tiles with 4 of W's and 4 of adapters' stages: 256 rows of 64 adapters of rank 64,
+  // 1024 -> 1024, 65 us instead of 70, but of one adapter, 4096 -> 4096, 26.7 instead of 22.0.)
+  static constexpr int kStages = BN == 64 ? 6 : 4;
+  static constexpr int kLowStages = 2;
   static constexpr int kStaging = 32 * 32 * 2;  // an epilogue warp's 32 rows of 32 columns
   static constexpr int kTmem = 2 * BN;
   static constexpr int kSmem =

@@ -496,7 +496,7 @@ LowTilePlan low_tile_plan(int rank) {
   p.part = 0;
   p.columns = rank <= 64 ? 64 : 128;
   p.stages = rank <= 128 ? 3 : 2;
-  p.smem = 1024 + p.stages * (kStageA + p.columns * 128) + BM * (rank + 4) * 4 + 2048;
+  p.smem = 1024 + p.stages * (kStageA + p.columns * 128) + BM * (rank + 4) * 4 + 2560;
   return p;
 }
 
@@ -509,8 +509,8 @@ __global__ void __launch_bounds__(kLowThreads, 2)
   const int S = plan.stages, stage = kStageA + plan.columns * 128;
   const int pitch = a.rank + 4;  // floats of a row of sums: neighbouring rows 16 bytes apart modulo the banks
   float* sums = reinterpret_cast<float*>(stages + S * stage);
-  float* scales = sums + BM * pitch;  // of each row's adapter; negative infinity for none
-  uint64_t* full = reinterpret_cast<uint64_t*>(scales + BM);
+  float2* factors = reinterpret_cast<float2*>(sums + BM * pitch);  // of each row's adapter its scale, and 1; 0 for none
+  uint64_t* full = reinterpret_cast<uint64_t*>(factors + BM);
   uint64_t* empty = full + S;
   uint64_t* acc_full = empty + S;
   uint64_t* acc_empty = acc_full + 1;
@@ -547,7 +547,7 @@ __global__ void __launch_bounds__(kLowThreads, 2)
   int mine = -1;
   if (warp >= 2) {
     if (row0 + r < a.rows) mine = row_adapter(a, row0 + r);
-    scales[r] = mine < 0 ? -INFINITY : __ldg(a.scales + mine);
+    factors[r] = mine < 0 ? make_float2(0.f, 0.f) : make_float2(__ldg(a.scales + mine), 1.f);
     bool any_idle;
     const int count = list_adapters<BM>(mine, -1, r, heads, listed, false, any_idle);
     if (r == 0) *list_count = count;
@@ -631,7 +631,7 @@ __global__ void __launch_bounds__(kLowThreads, 2)
     __syncwarp();
   } else {
     uint8_t* const own_low = low_row(a, row0 + r);
-    const float own_scale = scales[r];
+    const float own_scale = factors[r].x;
     for (int p = 0; p < passes; ++p) {
       const int from = blocks > 1 ? p / blocks : p * together;
       const int to = blocks > 1 ? from + 1 : min(count, from + together);
@@ -681,8 +681,8 @@ __global__ void __launch_bounds__(kLowThreads, 2)
       const uint32_t base = smem_u32(sums);
       for (int i = r; i < (end - begin) * fours; i += 128) {
         const int row = begin + i / fours, j = i % fours * 4;
-        const float scale = scales[row];
-        if (scale == -INFINITY) continue;
+        const float scale = factors[row].x;
+        if (factors[row].y == 0.f) continue;
         float4 w[8];
 #pragma unroll
         for (int c = 0; c < 8; ++c) {
@@ -1940,6 +1940,13 @@ __global__ void __launch_bounds__(kNarrowThreads, 2) project_narrow_kernel(const
             }
           }
         }
+        // scaled first: a scale that is not finite must not meet the zeros of other requests' rows
+#pragma unroll
+        for (int m = 0; m < M; ++m)
+#pragma unroll
+          for (int t = 0; t < (HALF ? 1 : 2); ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) low[m][t][e] *= scale;
         if (mixed) {
 #pragma unroll
           for (int m = 0; m < M; ++m)
@@ -1964,7 +1971,7 @@ __global__ void __launch_bounds__(kNarrowThreads, 2) project_narrow_kernel(const
                 hi[m][2 + h] = lo[m][h];
                 lo[m][2 + h] = 0;
               } else {
-                split2(low[m][t][h * 2] * scale, low[m][t][h * 2 + 1] * scale, hi[m][t * 2 + h], lo[m][t * 2 + h]);
+                split2(low[m][t][h * 2], low[m][t][h * 2 + 1], hi[m][t * 2 + h], lo[m][t * 2 + h]);
               }
             }
 #pragma unroll

@@ -961,6 +961,7 @@ _ROW_TYPES = {torch.float32: _native.F32, torch.bfloat16: _native.BF16, torch.fl
 _CHANNEL_NORMS = {"rms": 1, "layer": 2}
 _GATE_ACTS = {"none": 0, "sigmoid": 1, "silu": 2, "tanh": 3}
 _NO_NORM = (0, 0.0, 0, 0)
+_FLOAT32_MAX = torch.finfo(torch.float32).max
 
 
 @dataclass(frozen=True)
@@ -1248,7 +1249,7 @@ def pack_projection(weight: torch.Tensor, adapters: list[Adapter],
     tensors are copies: later changes of the originals do not reach them.
     Adapters may differ in rank (1 to 256) and must be finite, since a tile of
     rows of several requests multiplies each adapter by the others' zeros
-    (read once here, which synchronises).
+    (read once here, which synchronises); so must their scales, in float32.
     """
     for name, t in (("weight", weight), *((f"adapter {part}", getattr(a, part)) for a in adapters
                                           for part in ("down", "up"))):
@@ -1268,8 +1269,8 @@ def pack_projection(weight: torch.Tensor, adapters: list[Adapter],
                                 f"{n} x {k} projection")
         if a.down.shape[0] > _native.PROJECT_MAX_RANK:
             raise ContractError(f"adapter {i}: rank {a.down.shape[0]} above {_native.PROJECT_MAX_RANK}")
-        if not math.isfinite(a.scale):
-            raise ContractError(f"adapter {i}: scale must be finite, got {a.scale}")
+        if not abs(float(a.scale)) <= _FLOAT32_MAX:  # (no number fails too)
+            raise ContractError(f"adapter {i}: scale must be finite in float32, got {a.scale}")
     with torch.no_grad():
         rank = max(-(-int(a.down.shape[0]) // 16) * 16 for a in adapters)
         stride = -(-k // 8) * 8

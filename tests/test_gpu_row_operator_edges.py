@@ -1,0 +1,72 @@
+"""Row operators on B200 at the edges of their values, on every kernel that a projection may take.
+
+``PATHS`` names, for each kernel or combination of them, a projection that
+takes it.  Ranks of one and two are among the adapters, since an infinite
+low-rank value leaves infinities only where the signs of all its products
+agree; the other ranks make those be padded.
+"""
+
+from __future__ import annotations
+
+import dataclasses
+
+import numpy as np
+import pytest
+import torch
+
+from tests.test_gpu_project import TYPES, check, make_index, make_rows, problem
+
+pytestmark = pytest.mark.gpu
+
+PATHS = {  # rows, k, n, ranks
+    "narrow, 8 ranks": (200, 32, 32, [1, 5, 8]),
+    "narrow, one group": (200, 30, 32, [1, 2, 13]),
+    "narrow, several groups": (300, 72, 100, [2, 1, 20]),
+    "few rows, low-rank rows in the kernel": (4, 320, 320, [1, 2, 8]),
+    "few rows, partial sums": (100, 1024, 640, [2, 1, 40]),
+    "low-rank rows by rows, tiles of 64": (256, 1024, 512, [1, 2, 16] * 20),
+    "low-rank tiles by clusters, tiles of 64": (300, 1024, 333, [2, 13, 1]),
+    "low-rank tiles, tiles of 128": (1500, 136, 1500, [1, 20, 2]),
+    "low-rank tiles, pairs": (2100, 136, 1100, [1, 2, 20]),
+}
+BAD_INDEX = 64  # the site that an adapter index out of range is reported at
+
+
+def adapted_problem(rng, path, dtype, device, bias=True):
+    rows, k, n, ranks = PATHS[path]
+    parts = problem(rng, k, n, ranks, dtype, device, bias)
+    for a in parts[1]:
+        a.up[::2] = a.up[::2].bfloat16().to(a.up.dtype)  # (float16) values that leave no remainder beside those that do
+    return rows, k, n, ranks, parts
+
+
+@pytest.mark.parametrize("factor", [float("inf"), -float("inf"), float("nan")])
+@pytest.mark.parametrize("path", PATHS)
+def test_an_infinite_factor_reaches_its_own_rows_alone(cuda_device, path, factor):
+    """``pack_projection`` refuses it; laid out by other means it spoils no other request."""
+    from nnunet_mlx_b200 import kernels
+
+    rng = np.random.default_rng(25)
+    rows, k, n, ranks, parts = adapted_problem(rng, path, "bf16", cuda_device)
+    projection = kernels.pack_projection(parts[0], parts[1], bias=parts[2])
+    scales = projection.scales.clone()
+    scales.view(len(ranks), -1)[0, 0] = factor
+    spoilt = dataclasses.replace(projection, scales=scales)
+    x = make_rows(rng, (rows, k), "bf16", cuda_device)
+    index = make_index(rng, rows, len(ranks), "mixed", cuda_device)
+    index[0] = 0
+    want, got = (kernels.adapted_projection(x, p, index) for p in (projection, spoilt))
+    others = index != 0
+    assert torch.equal(got[others], want[others])
+    assert not got[~others].isfinite().any()
+
+
+def test_factors_outside_float32_are_refused(cuda_device):
+    from nnunet_mlx_b200 import kernels
+    from nnunet_mlx_b200.errors import ContractError
+
+    rng = np.random.default_rng(26)
+    weight, adapters, bias = problem(rng, 64, 48, [8, 4], "bf16", cuda_device)
+    for scale in (1e39, -1e39, 3.5e38, float("inf")):
+        with pytest.raises(ContractError, match="finite"):
+            kernels.pack_projection(weight, [adapters[0], kernels.Adapter(adapters[1].down, adapters[1].up, scale)])

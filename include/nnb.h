@@ -30,7 +30,7 @@
 extern "C" {
 #endif
 
-#define NNB_ABI_VERSION 15
+#define NNB_ABI_VERSION 16
 
 enum nnb_status {
   NNB_OK = 0,
@@ -710,7 +710,8 @@ int32_t nnb_gated_join(const nnb_join_args* args, void* stream);
  * An index outside [-1, adapters) gives its rows the shared projection alone
  * and records NNB_E_DEVICE for nnb_device_status.  `down` and `up` must be
  * finite: a tile of rows of several requests multiplies each adapter by the
- * others' zeros.
+ * others' zeros.  Low-rank values from an adapter's rank on count as zero, so an
+ * infinity in a row gives it what the formula gives.
  */
 #define NNB_PROJECT_MAX_RANK 256
 
@@ -720,7 +721,7 @@ typedef struct nnb_project_args {
   const void* down;     /* (adapters, rank, weight_stride), x's type; zero from each adapter's rank and from k on */
   const void* up;       /* (adapters, n, rank) bfloat16 for bfloat16 rows; (adapters, n, 2, rank) bfloat16 for
                            float16 rows: the values rounded to bfloat16, then what the rounding left */
-  const float* scales;  /* (adapters) */
+  const float* scales;  /* (adapters, 2): each adapter's scale and its rank, 8-byte aligned */
   const float* bias;    /* (n) or NULL */
   const int32_t* index; /* an adapter, or -1, for each rows_per_index rows */
   void* out;            /* rows out_stride elements apart, x's type */

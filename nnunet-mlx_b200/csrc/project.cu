@@ -123,6 +123,12 @@ __device__ __forceinline__ uint32_t pack2(float a, float b, __half) {
   return *reinterpret_cast<const uint32_t*>(&v);
 }
 
+// An adapter's scale (x) and rank (y).  Values of the ranks that it is padded with are set to zero, not computed: an
+// infinity in x times their zeros would be no number.
+__device__ __forceinline__ float2 factor(const nnb_project_args& a, int adapter) {
+  return __ldg(reinterpret_cast<const float2*>(a.scales) + adapter);
+}
+
 // What the index holds for a row.
 __device__ __forceinline__ int row_index(const nnb_project_args& a, int64_t row) {
   return __ldg(a.index + (a.rows_per_index == 1 ? row : (uint32_t)row / (uint32_t)a.rows_per_index));
@@ -166,12 +172,15 @@ __global__ void __launch_bounds__(256) align_rows_kernel(const uint16_t* __restr
   }
 }
 
-// Two low-rank values as two bfloat16 parts each, hi + lo.  What an infinity leaves would be no number: the larger
-// of it and a bound below every true remainder (half a step of the largest value is 2^119) is that bound.
+// Two low-rank values as two bfloat16 parts each, hi + lo.  hi is bounded, so that an infinity is lo's alone: hi's
+// remainder would be no number, and neither would hi times the zeros of a float16 adapter's second plane.  For bfloat16
+// the bound is the largest finite value; for float16 2^110, whose products with that plane's remainders (up to 2^5) add
+// up to no infinity (such a value overflows any float16 result, whatever its bits below the first eight).
+template <bool F16>
 __device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t& lo) {
   hi = pack2(a, b, __nv_bfloat16());
+  asm("min.NaN.xorsign.abs.bf16x2 %0, %0, %1;" : "+r"(hi) : "r"(F16 ? 0x76807680u : 0x7f7f7f7fu));  // a's sign
   lo = pack2(a - __uint_as_float(hi << 16), b - __uint_as_float(hi & 0xffff0000u), __nv_bfloat16());
-  asm("max.bf16x2 %0, %0, %1;" : "+r"(lo) : "r"(0xfb80fb80u));  // -2^120
 }
 
 // A row's low-rank values in the workspace, as the GEMM's stages take them: per block of 32 ranks 128 bytes, 32 hi
@@ -221,6 +230,7 @@ __global__ void __launch_bounds__(128) project_low_kernel(const nnb_project_args
   const int64_t row = blockIdx.x;
   const int adapter = row_adapter(a, row);
   if (adapter < 0) return;
+  const float2 own = factor(a, adapter);
   const int lane = threadIdx.x & 31, j0 = blockIdx.y * 16 + (threadIdx.x >> 5) * 4;
   const T* x = reinterpret_cast<const T*>(a.x) + row * a.x_stride;
   const T* down = reinterpret_cast<const T*>(a.down) + ((int64_t)adapter * a.rank + j0) * a.weight_stride;
@@ -247,13 +257,14 @@ __global__ void __launch_bounds__(128) project_low_kernel(const nnb_project_args
   for (int j = 0; j < 4; ++j) {
 #pragma unroll
     for (int h = 16; h >= 1; h >>= 1) sum[j] += __shfl_xor_sync(0xffffffffu, sum[j], h);
-    sum[j] *= __ldg(a.scales + adapter);
+    sum[j] = j0 + j < (int)own.y ? sum[j] * own.x : 0.f;
     if (!PACKED && lane == j) a.low[(blockIdx.z * a.rows + row) * a.rank + j0 + j] = sum[j];
   }
   if (PACKED && lane == 0) {
     uint2 hi, lo;
-    split2(sum[0], sum[1], hi.x, lo.x);
-    split2(sum[2], sum[3], hi.y, lo.y);
+    constexpr bool kF16 = !std::is_same<T, __nv_bfloat16>::value;
+    split2<kF16>(sum[0], sum[1], hi.x, lo.x);
+    split2<kF16>(sum[2], sum[3], hi.y, lo.y);
     uint8_t* out = low_row(a, row) + j0 / kRankBlock * 128 + j0 % kRankBlock * 2;
     *reinterpret_cast<uint2*>(out) = hi;
     *reinterpret_cast<uint2*>(out + 64) = lo;
@@ -509,7 +520,7 @@ __global__ void __launch_bounds__(kLowThreads, 2)
   const int S = plan.stages, stage = kStageA + plan.columns * 128;
   const int pitch = a.rank + 4;  // floats of a row of sums: neighbouring rows 16 bytes apart modulo the banks
   float* sums = reinterpret_cast<float*>(stages + S * stage);
-  float2* factors = reinterpret_cast<float2*>(sums + BM * pitch);  // of each row's adapter its scale, and 1; 0 for none
+  float2* factors = reinterpret_cast<float2*>(sums + BM * pitch);  // of each row's adapter its scale and rank; rank 0 for none
   uint64_t* full = reinterpret_cast<uint64_t*>(factors + BM);
   uint64_t* empty = full + S;
   uint64_t* acc_full = empty + S;
@@ -547,7 +558,7 @@ __global__ void __launch_bounds__(kLowThreads, 2)
   int mine = -1;
   if (warp >= 2) {
     if (row0 + r < a.rows) mine = row_adapter(a, row0 + r);
-    factors[r] = mine < 0 ? make_float2(0.f, 0.f) : make_float2(__ldg(a.scales + mine), 1.f);
+    factors[r] = mine < 0 ? make_float2(0.f, 0.f) : factor(a, mine);
     bool any_idle;
     const int count = list_adapters<BM>(mine, -1, r, heads, listed, false, any_idle);
     if (r == 0) *list_count = count;
@@ -631,7 +642,7 @@ __global__ void __launch_bounds__(kLowThreads, 2)
     __syncwarp();
   } else {
     uint8_t* const own_low = low_row(a, row0 + r);
-    const float own_scale = factors[r].x;
+    const float2 own = factors[r];
     for (int p = 0; p < passes; ++p) {
       const int from = blocks > 1 ? p / blocks : p * together;
       const int to = blocks > 1 ? from + 1 : min(count, from + together);
@@ -647,12 +658,14 @@ __global__ void __launch_bounds__(kLowThreads, 2)
           tmem_ld16(tmem + ((uint32_t)(warp & 3) << 21) + (i - from) * box + j, v);
           if (mine == adapter && gridDim.y == 1) {  // nothing to add up
 #pragma unroll
+            for (int e = 0; e < 16; ++e) v[e] = j0 + j + e < (int)own.y ? v[e] * own.x : 0.f;
+#pragma unroll
             for (int e = 0; e < 16; e += 8) {
               uint4 hi, lo;
-              split2(v[e] * own_scale, v[e + 1] * own_scale, hi.x, lo.x);
-              split2(v[e + 2] * own_scale, v[e + 3] * own_scale, hi.y, lo.y);
-              split2(v[e + 4] * own_scale, v[e + 5] * own_scale, hi.z, lo.z);
-              split2(v[e + 6] * own_scale, v[e + 7] * own_scale, hi.w, lo.w);
+              split2<kF16>(v[e], v[e + 1], hi.x, lo.x);
+              split2<kF16>(v[e + 2], v[e + 3], hi.y, lo.y);
+              split2<kF16>(v[e + 4], v[e + 5], hi.z, lo.z);
+              split2<kF16>(v[e + 6], v[e + 7], hi.w, lo.w);
               uint8_t* out = own_low + (j0 + j) / kRankBlock * 128 + ((j0 + j) % kRankBlock + e) * 2;
               *reinterpret_cast<uint4*>(out) = hi;
               *reinterpret_cast<uint4*>(out + 64) = lo;
@@ -681,8 +694,8 @@ __global__ void __launch_bounds__(kLowThreads, 2)
       const uint32_t base = smem_u32(sums);
       for (int i = r; i < (end - begin) * fours; i += 128) {
         const int row = begin + i / fours, j = i % fours * 4;
-        const float scale = factors[row].x;
-        if (factors[row].y == 0.f) continue;
+        const float2 own = factors[row];
+        if (own.y == 0.f) continue;
         float4 w[8];
 #pragma unroll
         for (int c = 0; c < 8; ++c) {
@@ -701,8 +714,9 @@ __global__ void __launch_bounds__(kLowThreads, 2)
 #pragma unroll
         for (int c = 1; c < 8; ++c) v.x += w[c].x, v.y += w[c].y, v.z += w[c].z, v.w += w[c].w;
         uint2 hi, lo;
-        split2(v.x * scale, v.y * scale, hi.x, lo.x);
-        split2(v.z * scale, v.w * scale, hi.y, lo.y);
+        const int left = (int)own.y - j;  // ranks of the adapter from j on
+        split2<kF16>(left > 0 ? v.x * own.x : 0.f, left > 1 ? v.y * own.x : 0.f, hi.x, lo.x);
+        split2<kF16>(left > 2 ? v.z * own.x : 0.f, left > 3 ? v.w * own.x : 0.f, hi.y, lo.y);
         uint8_t* out = low_row(a, row0 + row) + j / kRankBlock * 128 + j % kRankBlock * 2;
         *reinterpret_cast<uint2*>(out) = hi;
         *reinterpret_cast<uint2*>(out + 64) = lo;
@@ -1184,7 +1198,8 @@ __device__ __forceinline__ void few_low(const nnb_project_args& a, int begin, in
       if (whole + lane < a.k) sum = fmaf(value(x[whole + lane]), value(down[whole + lane]), sum);
 #pragma unroll
       for (int h = 16; h >= 1; h >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, h);
-      sum *= __ldg(a.scales + adapter);
+      const float2 own = factor(a, adapter);
+      sum = j < (int)own.y ? sum * own.x : 0.f;
     }
     if (lane == 0) low[i] = sum;
   }
@@ -1813,6 +1828,7 @@ __global__ void __launch_bounds__(kNarrowThreads, 2) project_narrow_kernel(const
   uint4 held_down[kHold ? 2 : 1];
   uint2 held_up[kHold ? 4 : 1], held_rest[kHold && kF16 ? 4 : 1];
   int held = -1;
+  bool padded = false;  // whether that adapter has fewer ranks than are computed
 
   int64_t row0 = ((int64_t)blockIdx.x * (kNarrowThreads / 32) + (threadIdx.x >> 5)) * kRows;
   if (row0 >= rows) return;
@@ -1885,7 +1901,11 @@ __global__ void __launch_bounds__(kNarrowThreads, 2) project_narrow_kernel(const
         if (listed == INT_MAX) break;
       }
       const bool mixed = !RUNS || border < kRows;  // else every row is the adapter's
-      const float scale = __ldg(a.scales + listed);
+      const float2 own_factor = factor(a, listed);
+      const float scale = own_factor.x;
+      const int own_rank = (int)own_factor.y;
+      // (Where rows are loaded ahead with the adapter, not with every tile: two volumes of 32 -> 32 100.7 and 103.5 us.)
+      if (!kAhead || held != listed) padded = own_rank != (HALF ? 8 : a.rank);
 #pragma unroll 1
       for (int j0 = 0; j0 < a.rank; j0 += 16) {
         int down_stride = (int)a.weight_stride, up_width = a.rank * (kF16 ? 2 : 1);
@@ -1940,26 +1960,6 @@ __global__ void __launch_bounds__(kNarrowThreads, 2) project_narrow_kernel(const
             }
           }
         }
-        // scaled first: a scale that is not finite must not meet the zeros of other requests' rows
-#pragma unroll
-        for (int m = 0; m < M; ++m)
-#pragma unroll
-          for (int t = 0; t < (HALF ? 1 : 2); ++t)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) low[m][t][e] *= scale;
-        if (mixed) {
-#pragma unroll
-          for (int m = 0; m < M; ++m)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const bool own = RUNS ? (m * 16 + h * 8 + g < border) == (turn == 0) : mine[m][h] == listed;
-#pragma unroll
-              for (int t = 0; t < 2; ++t) {
-                low[m][t][h * 2] = own ? low[m][t][h * 2] : 0.f;
-                low[m][t][h * 2 + 1] = own ? low[m][t][h * 2 + 1] : 0.f;
-              }
-            }
-        }
         uint32_t hi[M][4], lo[M][4];
 #pragma unroll
         for (int m = 0; m < M; ++m)
@@ -1971,9 +1971,35 @@ __global__ void __launch_bounds__(kNarrowThreads, 2) project_narrow_kernel(const
                 hi[m][2 + h] = lo[m][h];
                 lo[m][2 + h] = 0;
               } else {
-                split2(low[m][t][h * 2], low[m][t][h * 2 + 1], hi[m][t * 2 + h], lo[m][t * 2 + h]);
+                split2<kF16>(low[m][t][h * 2] * scale, low[m][t][h * 2 + 1] * scale, hi[m][t * 2 + h], lo[m][t * 2 + h]);
               }
             }
+        // Zeros for rows of others and for ranks that the adapter is padded with.  As words of the parts: a scale or an x
+        // that is not finite leaves nothing there that a product with zero could make no number of.
+        auto keep = [&](int m, int h, int t, bool own, bool all_ranks) {
+          const int left = all_ranks ? 2 : own_rank - j0 - (HALF ? q * 2 : q * 4 + t * 2);  // ranks from the word's first on
+          const uint32_t bits = !own || left <= 0 ? 0 : left == 1 ? 0xffffu : 0xffffffffu;
+          hi[m][t * 2 + h] &= bits;
+          lo[m][t * 2 + h] &= bits;
+        };
+        if (!RUNS || mixed || padded) {
+#pragma unroll
+          for (int m = 0; m < M; ++m)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const bool own = !mixed || (RUNS ? (m * 16 + h * 8 + g < border) == (turn == 0) : mine[m][h] == listed);
+#pragma unroll
+              for (int t = 0; t < 2; ++t) keep(m, h, t, own, !RUNS);
+            }
+        }
+        if (!RUNS && padded) {
+#pragma unroll
+          for (int m = 0; m < M; ++m)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+              for (int t = 0; t < 2; ++t) keep(m, h, t, true, false);
+        }
 #pragma unroll
         for (int p = 0; p < NN; ++p) {
           uint2 w[4], rest[kF16 ? 4 : 1];
@@ -1997,12 +2023,14 @@ __global__ void __launch_bounds__(kNarrowThreads, 2) project_narrow_kernel(const
 #pragma unroll
               for (int m = 0; m < M; ++m) warp_mma(acc[m][p * 4 + t], lo[m], w[t].x, w[t].y, __nv_bfloat16());
           }
-          if constexpr (kF16) {  // (HALF: the lo parts meet zeros)
+          if constexpr (kF16) {  // (without the lo parts that HALF has beside the hi parts)
 #pragma unroll
             for (int t = 0; t < 4; ++t)
 #pragma unroll
-              for (int m = 0; m < M; ++m)
-                warp_mma(acc[m][p * 4 + t], hi[m], rest[t].x, HALF ? 0u : rest[t].y, __nv_bfloat16());
+              for (int m = 0; m < M; ++m) {
+                const uint32_t only_hi[4] = {hi[m][0], hi[m][1], HALF ? 0u : hi[m][2], HALF ? 0u : hi[m][3]};
+                warp_mma(acc[m][p * 4 + t], only_hi, rest[t].x, rest[t].y, __nv_bfloat16());
+              }
           }
         }
       }
@@ -2165,6 +2193,7 @@ extern "C" int32_t nnb_project(const nnb_project_args* args, void* stream) {
                   (reinterpret_cast<uintptr_t>(a.weight) | reinterpret_cast<uintptr_t>(a.down) |
                    reinterpret_cast<uintptr_t>(a.up) | reinterpret_cast<uintptr_t>(a.low)) % 16 == 0,
               "project: packed weights and workspace must be 16-byte aligned");
+  NNB_REQUIRE(reinterpret_cast<uintptr_t>(a.scales) % 8 == 0, "project: scales must be 8-byte aligned");
   NNB_REQUIRE(a.low != nullptr || nnb_project_workspace_bytes(args) == 0, "project: missing workspace");
   return a.type == NNB_BF16 ? launch_project<__nv_bfloat16>(a, (cudaStream_t)stream)
                             : launch_project<__half>(a, (cudaStream_t)stream);

@@ -1227,7 +1227,7 @@ class AdaptedProjection:
     weight: torch.Tensor       # (N, K rounded up to 8)
     down: torch.Tensor         # (adapters, R, K rounded up to 8), R the largest rank rounded up to 16
     up: torch.Tensor           # (adapters, N, planes, R) bfloat16
-    scales: torch.Tensor       # (adapters,) float32
+    scales: torch.Tensor       # (adapters, 2) float32: each adapter's scale and its rank
     bias: torch.Tensor | None  # (N,) float32
     in_channels: int
     used_rank: int             # the largest rank
@@ -1288,7 +1288,7 @@ def pack_projection(weight: torch.Tensor, adapters: list[Adapter],
                 up[i, :, 1, :r] = a.up.float() - up[i, :, 0, :r].float()
         if not bool(torch.isfinite(down).all() & torch.isfinite(up).all()):
             raise ContractError("adapters must be finite")
-        scales = torch.tensor([float(a.scale) for a in adapters], dtype=torch.float32, device=device)
+        scales = torch.tensor([[float(a.scale), a.down.shape[0]] for a in adapters], dtype=torch.float32, device=device)
         return AdaptedProjection(packed, down, up, scales, None if bias is None else bias.detach().clone(), k,
                                  max(int(a.down.shape[0]) for a in adapters))
 
@@ -1304,8 +1304,9 @@ def adapted_projection(x: torch.Tensor, projection: AdaptedProjection, index: to
     rows the shared projection alone and is reported by
     ``_native.device_status``.  Products are accumulated in float32, the
     low-rank rows are kept to 16 bits of mantissa or more, and the result is
-    rounded once to the projection's type.  ``out`` receives the result and
-    shares no memory with the inputs.
+    rounded once to the projection's type.  An infinity or no number in a row
+    gives that row what the formula gives, and reaches no other.  ``out``
+    receives the result and shares no memory with the inputs.
 
     Rows of one request that follow one another share the reading of its
     adapter; any order gives the same values.

@@ -40,6 +40,56 @@ def adapted_problem(rng, path, dtype, device, bias=True):
     return rows, k, n, ranks, parts
 
 
+def by_definition(x, parts, index):
+    """Float64 rows, each product taken apart, so that nothing but the formula meets an infinity."""
+    weight, adapters, bias = parts
+    out = []
+    for row, a in zip(x.double(), index.tolist()):
+        y = (weight.double() * row).sum(-1)
+        if bias is not None:
+            y = y + bias.double()
+        if a >= 0:
+            low = (adapters[a].down.double() * row).sum(-1)
+            y = y + adapters[a].scale * (adapters[a].up.double() * low).sum(-1)
+        out.append(y)
+    return torch.stack(out)
+
+
+@pytest.mark.parametrize("mode", ["mixed", "one"])
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("path", PATHS)
+def test_infinities_follow_the_definition(cuda_device, path, dtype, mode):
+    from nnunet_mlx_b200 import kernels
+
+    rng = np.random.default_rng(21)
+    rows, k, n, ranks, parts = adapted_problem(rng, path, dtype, cuda_device)
+    projection = kernels.pack_projection(parts[0], parts[1], bias=parts[2])
+    x = make_rows(rng, (rows, k), dtype, cuda_device)
+    index = make_index(rng, rows, len(ranks), "mixed", cuda_device)
+    if mode == "one":
+        index.fill_(ranks.index(1))
+    index[:4] = torch.tensor([ranks.index(1), ranks.index(2) if 2 in ranks else 0, -1, len(ranks) - 1])
+    if mode == "one":
+        index[:4] = ranks.index(1)
+    want = kernels.adapted_projection(x, projection, index)
+    assert want.isfinite().all()
+    hit = torch.tensor([0, 1, 2, 3] + ([rows // 2, rows - 1] if rows > 8 else []), device=cuda_device)
+    for i, row in enumerate(hit.tolist()):
+        x[row, (7 * i) % k] = float("inf") if i % 2 == 0 else -float("inf")
+    got = kernels.adapted_projection(x, projection, index)
+    ref = by_definition(x[hit], parts, index[hit])
+    mine = got[hit].double()
+    assert ref.isinf().any()
+    assert torch.equal(mine.isnan(), ref.isnan())
+    assert torch.equal(mine.isposinf(), ref.isposinf()) and torch.equal(mine.isneginf(), ref.isneginf())
+    rest = torch.ones(rows, dtype=torch.bool, device=cuda_device)
+    rest[hit] = False
+    assert torch.equal(got[rest], want[rest])
+    x[hit[0]] = float("nan")
+    got = kernels.adapted_projection(x, projection, index)
+    assert got[hit[0]].isnan().all() and torch.equal(got[rest], want[rest])
+
+
 @pytest.mark.parametrize("factor", [float("inf"), -float("inf"), float("nan")])
 @pytest.mark.parametrize("path", PATHS)
 def test_an_infinite_factor_reaches_its_own_rows_alone(cuda_device, path, factor):

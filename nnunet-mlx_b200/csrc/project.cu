@@ -66,7 +66,7 @@ namespace {
 
 using namespace tc;
 
-constexpr int kBadIndex = 41;  // site number of an adapter index out of range; 42-63 are waits
+constexpr int kBadIndex = 64;  // site number of an adapter index out of range; all below are waits, here or in tc_conv.cu
 
 constexpr int kThreads = 480;
 constexpr int kStageA = BM * 128;

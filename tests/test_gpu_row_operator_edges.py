@@ -90,6 +90,29 @@ def test_infinities_follow_the_definition(cuda_device, path, dtype, mode):
     assert got[hit[0]].isnan().all() and torch.equal(got[rest], want[rest])
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("path", PATHS)
+def test_bad_index_on_every_path(cuda_device, path, dtype):
+    from nnunet_mlx_b200 import _native, kernels
+
+    rng = np.random.default_rng(22)
+    rows, k, n, ranks, parts = adapted_problem(rng, path, dtype, cuda_device)
+    projection = kernels.pack_projection(parts[0], parts[1], bias=parts[2])
+    x = make_rows(rng, (rows, k), dtype, cuda_device)
+    for mode in ("mixed", "one"):
+        index = make_index(rng, rows, len(ranks), mode, cuda_device)
+        for bad_rows in ([0, rows - 1], list(range(rows // 2, rows))):  # (the second leaves whole tiles without any)
+            bad = index.clone()
+            bad[bad_rows] = torch.tensor([len(ranks), -2, 2 ** 31 - 1, -2 ** 31], dtype=torch.int32,
+                                         device=cuda_device).repeat(len(bad_rows))[:len(bad_rows)]
+            got = kernels.adapted_projection(x, projection, bad)
+            assert _native.device_status(reset=True) == (-4, BAD_INDEX)
+            good = index.clone()
+            good[bad_rows] = -1
+            assert torch.equal(got, kernels.adapted_projection(x, projection, good))
+            assert _native.device_status(reset=True)[0] == 0
+
+
 @pytest.mark.parametrize("factor", [float("inf"), -float("inf"), float("nan")])
 @pytest.mark.parametrize("path", PATHS)
 def test_an_infinite_factor_reaches_its_own_rows_alone(cuda_device, path, factor):

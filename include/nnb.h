@@ -101,7 +101,8 @@ const char* nnb_last_error(void);
 /*
  * First device-side error recorded by a kernel since the last reset (0 when
  * none), e.g. a bounded mbarrier wait that expired; `where` receives the wait
- * site.  Synchronises with the device.  No reference counterpart: the
+ * site.  A reset clears the error that is returned: call until 0 for the others
+ * (convolutions and adapted projections keep one each).  Synchronises with the device.  No reference counterpart: the
  * reference's Metal kernels have no device-side waits.
  */
 int32_t nnb_device_status(int32_t* where, int32_t reset);

@@ -1988,17 +1988,13 @@ extern "C" int32_t nnb_device_status(int32_t* where, int32_t reset) {
   if (cudaDeviceSynchronize() != cudaSuccess) return NNB_E_CUDA;
   if (cudaMemcpyFromSymbol(&status, nnb::g_device_status, sizeof(int)) != cudaSuccess) return NNB_E_CUDA;
   cudaMemcpyFromSymbol(&loc, nnb::g_device_status_where, sizeof(int));
-  if (reset) {
+  if (reset && status != 0) {
     const int zero = 0;
     cudaMemcpyToSymbol(nnb::g_device_status, &zero, sizeof(int));
     cudaMemcpyToSymbol(nnb::g_device_status_where, &zero, sizeof(int));
   }
-  int project_loc = 0;
-  const int project_status = nnb::project_device_status(&project_loc, reset != 0);
-  if (status == 0) {
-    status = project_status;
-    loc = project_loc;
-  }
+  // one error at a time: the projection's stays for the next call where the convolutions have one
+  if (status == 0) status = nnb::project_device_status(&loc, reset != 0);
   if (where) *where = loc;
   return status;
 }

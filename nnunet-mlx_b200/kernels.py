@@ -1250,6 +1250,8 @@ def pack_projection(weight: torch.Tensor, adapters: list[Adapter],
     Adapters may differ in rank (1 to 256) and must be finite, since a tile of
     rows of several requests multiplies each adapter by the others' zeros
     (read once here, which synchronises); so must their scales, in float32.
+    Tensors that require a gradient are packed under ``torch.no_grad()`` only:
+    none would come back to them.
     """
     for name, t in (("weight", weight), *((f"adapter {part}", getattr(a, part)) for a in adapters
                                           for part in ("down", "up"))):
@@ -1258,11 +1260,12 @@ def pack_projection(weight: torch.Tensor, adapters: list[Adapter],
         if t.dim() != 2 or min(t.shape) < 1 or t.dtype != weight.dtype or t.device != weight.device:
             raise ContractError(f"{name} must be a matrix of the weight's type and device, got "
                                 f"{tuple(t.shape)} {t.dtype} on {t.device}")
+        _check_no_gradient(t, name)
     if not adapters:
         raise ContractError("an adapted projection needs at least one adapter")
     n, k = (int(v) for v in weight.shape)
     device, dtype = weight.device, weight.dtype
-    _channels_pointer(None if bias is None else bias.detach(), "projection bias", n, device)
+    _channels_pointer(bias, "projection bias", n, device)
     for i, a in enumerate(adapters):
         if a.down.shape[1] != k or a.up.shape != (n, a.down.shape[0]):
             raise ContractError(f"adapter {i}: down {tuple(a.down.shape)} and up {tuple(a.up.shape)} do not fit a "

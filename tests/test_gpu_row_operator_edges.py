@@ -143,3 +143,24 @@ def test_factors_outside_float32_are_refused(cuda_device):
     for scale in (1e39, -1e39, 3.5e38, float("inf")):
         with pytest.raises(ContractError, match="finite"):
             kernels.pack_projection(weight, [adapters[0], kernels.Adapter(adapters[1].down, adapters[1].up, scale)])
+
+
+def test_packing_refuses_what_requires_a_gradient(cuda_device):
+    from nnunet_mlx_b200 import kernels
+    from nnunet_mlx_b200.errors import ContractError
+
+    rng = np.random.default_rng(27)
+    weight, adapters, bias = problem(rng, 64, 48, [8, 4], "bf16", cuda_device)
+    tracked = [torch.nn.Parameter(t) for t in (weight, adapters[0].down, adapters[0].up, bias)]
+    calls = [
+        lambda: kernels.pack_projection(tracked[0], adapters, bias=bias),
+        lambda: kernels.pack_projection(weight, [kernels.Adapter(tracked[1], adapters[0].up), adapters[1]], bias=bias),
+        lambda: kernels.pack_projection(weight, [adapters[1], kernels.Adapter(adapters[0].down, tracked[2])], bias=bias),
+        lambda: kernels.pack_projection(weight, adapters, bias=tracked[3]),
+    ]
+    for call in calls:
+        with pytest.raises(ContractError, match="no backward pass"):
+            call()
+        with torch.no_grad():
+            p = call()
+        assert not any(t.requires_grad for t in (p.weight, p.down, p.up, p.scales))

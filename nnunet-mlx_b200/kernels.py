@@ -20,6 +20,7 @@ from dataclasses import dataclass, field
 
 import numpy as np
 import torch
+from torch.autograd import forward_ad
 
 from nnunet_mlx_b200 import _native
 from nnunet_mlx_b200.errors import ContractError
@@ -1011,6 +1012,10 @@ def _check_no_gradient(t: torch.Tensor, name: str) -> None:
     if t.requires_grad and torch.is_grad_enabled():
         raise ContractError(f"{name} requires a gradient: this operator has no backward pass "
                             "(call it under torch.no_grad())")
+    # (the level first: unpack_dual takes as long as a tenth of a small call)
+    if forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None:
+        raise ContractError(f"{name} carries a forward-mode tangent, which this operator would drop "
+                            "(give it the primal of torch.autograd.forward_ad.unpack_dual)")
 
 
 def _check_rows(t: torch.Tensor, name: str) -> None:

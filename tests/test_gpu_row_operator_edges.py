@@ -164,3 +164,33 @@ def test_packing_refuses_what_requires_a_gradient(cuda_device):
         with torch.no_grad():
             p = call()
         assert not any(t.requires_grad for t in (p.weight, p.down, p.up, p.scales))
+
+
+def test_forward_mode_tangents_are_refused(cuda_device):
+    from torch.autograd import forward_ad
+
+    from nnunet_mlx_b200 import kernels
+    from nnunet_mlx_b200.errors import ContractError
+
+    rng = np.random.default_rng(28)
+    weight, adapters, bias = problem(rng, 32, 32, [8], "bf16", cuda_device)
+    p = kernels.pack_projection(weight, adapters, bias=bias)
+    x, index = make_rows(rng, (6, 32), "bf16", cuda_device), torch.zeros(6, dtype=torch.int32, device=cuda_device)
+    plain, w = x.float(), torch.ones(32, device=cuda_device)
+    norm = kernels.ChannelNorm("rms", w)
+    with forward_ad.dual_level():
+        kernels.channel_norm(plain, norm)  # no tangent, no refusal
+        kernels.adapted_projection(x, p, index)
+        dual, dual_x, dual_w = (forward_ad.make_dual(t, torch.ones_like(t)) for t in (plain, x, w))
+        for call in (
+            lambda: kernels.channel_norm(dual, norm),
+            lambda: kernels.channel_norm(plain, kernels.ChannelNorm("rms", dual_w)),
+            lambda: kernels.gated_residual_join(dual, plain),
+            lambda: kernels.gated_residual_join(plain, dual),
+            lambda: kernels.gated_residual_join(plain, plain, gate=dual),
+            lambda: kernels.gated_residual_join(plain, plain, scale=dual_w),
+            lambda: kernels.adapted_projection(dual_x, p, index),
+            lambda: kernels.pack_projection(forward_ad.make_dual(weight, weight), adapters),
+        ):
+            with pytest.raises(ContractError, match="tangent"):
+                call()

@@ -1069,8 +1069,8 @@ def _check_out(out: torch.Tensor, name: str, shape, dtype: torch.dtype, device: 
     return stride
 
 
-def _call_rows(function, args: bytes, device: torch.device, what: str) -> None:
-    """A row operator's launch, on ``device``'s current stream.
+def _call_rows(function, args: bytes, device: torch.device, what: str, written: torch.Tensor | None = None) -> None:
+    """A row operator's launch, on ``device``'s current stream; ``written`` is a caller's tensor that it writes to.
 
     The stream is asked for as a plain handle: the Stream object that
     ``torch.cuda.current_stream`` builds costs as much host time as a launch.
@@ -1083,6 +1083,8 @@ def _call_rows(function, args: bytes, device: torch.device, what: str) -> None:
             status = function(args, torch._C._cuda_getCurrentRawStream(index))
     if status != 0:
         _native.check(status, what)
+    if written is not None and not written.is_inference():
+        torch.autograd.graph.increment_version(written)  # what autograd has saved of it is no longer there
 
 
 def channel_norm(x: torch.Tensor, norm: ChannelNorm, *, out_dtype: torch.dtype | None = None,
@@ -1102,6 +1104,7 @@ def channel_norm(x: torch.Tensor, norm: ChannelNorm, *, out_dtype: torch.dtype |
         raise ContractError(f"out_dtype must be float32, bfloat16 or float16, got {dtype}")
     x_stride = _row_stride(x, "x")
     n = norm.arguments(channels, device)
+    given = out
     if out is None:
         out, out_stride = _empty_rows(x, dtype), channels
     else:
@@ -1118,7 +1121,7 @@ def channel_norm(x: torch.Tensor, norm: ChannelNorm, *, out_dtype: torch.dtype |
     token = None
     if PROFILE.active:
         token = PROFILE.start("channel_norm", 0.0, float(rows * channels * (x.element_size() + out.element_size())))
-    _call_rows(_native.load().nnb_channel_norm_rows, args, device, "channel_norm")
+    _call_rows(_native.load().nnb_channel_norm_rows, args, device, "channel_norm", given)
     PROFILE.stop(token)
     return out
 
@@ -1177,6 +1180,7 @@ def gated_residual_join(branch: torch.Tensor, skip: torch.Tensor, *, post: Chann
     branch_stride, skip_stride = _row_stride(branch, "branch"), _row_stride(skip, "skip")
     post_args = _NO_NORM if post is None else post.arguments(channels, device)
     next_args = _NO_NORM if next_norm is None else next_norm.arguments(channels, device)
+    given = out
     if out is None:
         out, out_stride = _empty_rows(skip, skip.dtype), channels
     else:
@@ -1205,7 +1209,7 @@ def gated_residual_join(branch: torch.Tensor, skip: torch.Tensor, *, post: Chann
         nbytes = (branch.element_size() + 2 * skip.element_size() + (0 if normed is None else normed.element_size())
                   + (gate.element_size() if mode == 1 else 0))
         token = PROFILE.start("gated_residual_join", 0.0, float(nbytes) * rows * channels)
-    _call_rows(_native.load().nnb_gated_join, args, device, "gated_residual_join")
+    _call_rows(_native.load().nnb_gated_join, args, device, "gated_residual_join", given)
     PROFILE.stop(token)
     return out, normed
 
@@ -1334,6 +1338,7 @@ def adapted_projection(x: torch.Tensor, projection: AdaptedProjection, index: to
     down = projection.down
     (n, weight_stride), (adapters, rank, _) = weight.shape, down.shape
     x_stride = _row_stride(x, "x")
+    given = out
     if out is None:
         out, out_stride = x.new_empty((*shape[:-1], n)), n
     else:
@@ -1366,6 +1371,6 @@ def adapted_projection(x: torch.Tensor, projection: AdaptedProjection, index: to
         token = PROFILE.start("adapted_projection", 2.0 * rows * (n * k + rank * (n + k)),
                               2.0 * (rows * (n + k) + n * k),
                               launches=1 + copied + (nbytes > copied * rows * weight_stride * 2))
-    _call_rows(lib.nnb_project, args, device, "adapted_projection")
+    _call_rows(lib.nnb_project, args, device, "adapted_projection", given)
     PROFILE.stop(token)
     return out

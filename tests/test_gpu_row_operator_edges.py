@@ -194,3 +194,27 @@ def test_forward_mode_tangents_are_refused(cuda_device):
         ):
             with pytest.raises(ContractError, match="tangent"):
                 call()
+
+
+def test_results_written_in_place_are_seen_by_autograd(cuda_device):
+    from nnunet_mlx_b200 import kernels
+
+    rng = np.random.default_rng(29)
+    weight, adapters, bias = problem(rng, 32, 32, [8], "bf16", cuda_device)
+    p = kernels.pack_projection(weight, adapters, bias=bias)
+    x, index = make_rows(rng, (6, 32), "bf16", cuda_device), torch.zeros(6, dtype=torch.int32, device=cuda_device)
+    norm = kernels.ChannelNorm()
+    for call in (lambda out: kernels.channel_norm(x, norm, out=out),
+                 lambda out: kernels.gated_residual_join(x, x, out=out),
+                 lambda out: kernels.adapted_projection(x, p, index, out=out)):
+        out = torch.zeros((6, 32), dtype=torch.bfloat16, device=cuda_device)
+        factor = torch.ones_like(out, requires_grad=True)
+        y = factor * out  # keeps `out` for its backward pass
+        call(out)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.sum().backward()
+    with torch.inference_mode():
+        inner = torch.zeros((6, 32), dtype=torch.bfloat16, device=cuda_device)
+        kernels.channel_norm(x, norm, out=inner)
+    kernels.channel_norm(x, norm, out=inner)  # an inference tensor has no versions
+    assert torch.equal(inner, kernels.channel_norm(x, norm))

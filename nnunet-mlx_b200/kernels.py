@@ -984,8 +984,8 @@ class ChannelNorm:
     def __post_init__(self) -> None:
         if self.kind not in _CHANNEL_NORMS:
             raise ContractError(f"unknown channel norm {self.kind!r}: one of {', '.join(_CHANNEL_NORMS)}")
-        if not 0.0 < float(self.eps) < math.inf:
-            raise ContractError(f"a channel norm's eps must be positive, got {self.eps}")
+        if not 0.0 < ctypes.c_float(self.eps).value < math.inf:
+            raise ContractError(f"a channel norm's eps must be positive and finite in float32, got {self.eps}")
         for name, p in (("weight", self.weight), ("bias", self.bias)):
             if p is not None:
                 _check_tensor(p, f"norm {name}")
@@ -1159,6 +1159,8 @@ def gated_residual_join(branch: torch.Tensor, skip: torch.Tensor, *, post: Chann
                             f"got {skip.dtype}")
     if gate_act not in _GATE_ACTS:
         raise ContractError(f"unknown gate activation {gate_act!r}: one of {', '.join(_GATE_ACTS)}")
+    if _FLOAT32_MAX < abs(residual_scale) < math.inf:
+        raise ContractError(f"residual_scale {residual_scale} leaves float32's range")
     channels = shape[-1]
     scale_pointer = _channels_pointer(scale, "scale", channels, device)
     rows = branch.numel() // channels
@@ -1330,7 +1332,9 @@ def adapted_projection(x: torch.Tensor, projection: AdaptedProjection, index: to
     if x.dtype != weight.dtype or device != weight.device or shape[-1] != projection.in_channels:
         raise ContractError(f"x must hold {projection.in_channels} {weight.dtype} channels on {weight.device}, got "
                             f"{tuple(shape)} {x.dtype} on {device}")
-    axes = index.dim()
+    axes = index.dim() if isinstance(index, torch.Tensor) else 0
+    if not axes:
+        raise ContractError(f"index must be a contiguous int32 tensor over leading axes of {tuple(shape)} on {device}")
     if index.dtype != torch.int32 or not index.is_contiguous() or index.device != device \
             or not 1 <= axes < len(shape) or index.shape != shape[:axes]:
         raise ContractError(f"index must be a contiguous int32 tensor over leading axes of {tuple(shape)} on {device}, "

@@ -145,6 +145,18 @@ def test_factors_outside_float32_are_refused(cuda_device):
             kernels.pack_projection(weight, [adapters[0], kernels.Adapter(adapters[1].down, adapters[1].up, scale)])
 
 
+def test_residual_scales_outside_float32_are_refused(cuda_device):
+    from nnunet_mlx_b200 import kernels
+    from nnunet_mlx_b200.errors import ContractError
+
+    x = torch.ones((4, 32), device=cuda_device)
+    for scale in (1e39, -1e39):
+        with pytest.raises(ContractError, match="residual_scale"):
+            kernels.gated_residual_join(x, x, residual_scale=scale)
+    got, _ = kernels.gated_residual_join(x, x, residual_scale=float("inf"))
+    assert got.isposinf().all()
+
+
 def test_packing_refuses_what_requires_a_gradient(cuda_device):
     from nnunet_mlx_b200 import kernels
     from nnunet_mlx_b200.errors import ContractError

@@ -157,3 +157,9 @@ def test_structures_match_the_header(tmp_path):
         assert int(found[c_name]) == ctypes.sizeof(struct)
         for field in struct._fields_:
             assert int(found[f"{c_name}.{field[0]}"]) == getattr(struct, field[0]).offset
+
+
+@pytest.mark.parametrize("eps", [1e39, 1e-60])  # an infinity and a zero there
+def test_channel_norm_eps_in_float32(eps):
+    with pytest.raises(ContractError, match="eps"):
+        kernels.ChannelNorm(eps=eps)

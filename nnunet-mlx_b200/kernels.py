@@ -1142,8 +1142,9 @@ def gated_residual_join(branch: torch.Tensor, skip: torch.Tensor, *, post: Chann
     multiplies each element (``branch``'s shape), each row (``(..., 1)``) or
     each channel of a sample (``(B, C)`` beside a ``(B, ..., C)`` branch, or
     ``(1, C)``), through ``gate_act`` (``"none"``, ``"sigmoid"``, ``"silu"``,
-    ``"tanh"``).  ``scale`` is a float32 ``(C,)`` factor.  Everything is
-    computed in float32; the stream is rounded to ``skip``'s type where it is
+    ``"tanh"``).  ``scale`` is a finite float32 ``(C,)`` factor.  Everything is
+    computed in float32 (a 16-bit gate's sigmoid within 4 + 2.4 abs(gate)
+    roundings, far below what the gate's own rounding does to it); the stream is rounded to ``skip``'s type where it is
     stored, the normed rows (``next_dtype``, by default ``branch``'s type) are
     taken from the unrounded stream.  ``out`` receives the stream: it may be
     ``skip`` itself, and shares no memory with the other inputs.

@@ -230,3 +230,33 @@ def test_results_written_in_place_are_seen_by_autograd(cuda_device):
         kernels.channel_norm(x, norm, out=inner)
     kernels.channel_norm(x, norm, out=inner)  # an inference tensor has no versions
     assert torch.equal(inner, kernels.channel_norm(x, norm))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_gates_of_every_size(cuda_device, dtype):
+    """A float32 gate's sigmoid within 16 float32 roundings whatever its size: the base-2 exponential is within 2^-22.5
+    (3 U), what its argument leaves out is made up for (2 U), the reciprocal within 2^-23 (2 U), and the sum's and the
+    products' roundings follow.  A bfloat16 gate's by the fast exponential, within 2 + 1.16 |g| units of the last place.
+    Either is zero where it is below float32's normal range."""
+    from nnunet_mlx_b200 import kernels
+
+    U = 2.0 ** -24
+    g = torch.cat([torch.linspace(-110.0, 110.0, 200_001, dtype=torch.float64),
+                   torch.tensor([-200.0, -3e38, 3e38, 0.0, -0.0, 1e-30, -1e-30])]).to(cuda_device)
+    gate = g[:g.numel() // 8 * 8].to(TYPES.get(dtype, torch.float32)).view(-1, 8)
+    branch, skip = torch.ones_like(gate), torch.zeros(gate.shape, device=cuda_device)
+    v = gate.double()
+    for act in ("sigmoid", "silu"):
+        got, _ = kernels.gated_residual_join(branch, skip, gate=gate, gate_act=act)
+        ref = torch.sigmoid(v) * (v if act == "silu" else 1.0)
+        times = v.abs().clamp(1.0, 128.0) if act == "silu" else 1.0
+        if dtype == "f32":
+            off = 16 * U * ref.abs() + 2.0 ** -126 * times
+        else:
+            off = (2 * (2 + 1.16 * v.abs().clamp(max=200.0)) + 8) * U * ref.abs() + 2.0 ** -126 * times
+        assert ((got.double() - ref).abs() <= off).all()
+    edge = torch.tensor([[float("nan"), float("inf"), -float("inf")]], device=cuda_device, dtype=gate.dtype)
+    for act, want in (("sigmoid", (1.0, 0.0)), ("silu", (float("inf"), None))):
+        got, _ = kernels.gated_residual_join(torch.ones_like(edge), torch.zeros_like(edge), gate=edge, gate_act=act)
+        assert got[0, 0].isnan() and got[0, 1] == want[0]
+        assert got[0, 2].isnan() if want[1] is None else got[0, 2] == want[1]

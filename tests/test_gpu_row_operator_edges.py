@@ -113,6 +113,34 @@ def test_bad_index_on_every_path(cuda_device, path, dtype):
             assert _native.device_status(reset=True)[0] == 0
 
 
+@pytest.mark.parametrize("path", PATHS)
+def test_low_rank_values_beyond_float16(cuda_device, path):
+    rng = np.random.default_rng(23)
+    rows, k, n, ranks, parts = adapted_problem(rng, path, "f16", cuda_device)
+    for a in parts[1]:
+        a.down.mul_(3e4)
+        a.up.mul_(1e-4)
+    for mode in ("mixed", "one"):
+        check(make_rows(rng, (rows, k), "f16", cuda_device), parts,
+              make_index(rng, rows, len(ranks), mode, cuda_device))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("path", PATHS)
+def test_calls_repeat_bit_by_bit(cuda_device, path, dtype):
+    from nnunet_mlx_b200 import kernels
+
+    rng = np.random.default_rng(24)
+    rows, k, n, ranks, parts = adapted_problem(rng, path, dtype, cuda_device)
+    projection = kernels.pack_projection(parts[0], parts[1], bias=parts[2])
+    xs = [make_rows(rng, (rows, k), dtype, cuda_device) for _ in range(2)]
+    index = make_index(rng, rows, len(ranks), "mixed", cuda_device)
+    want = [kernels.adapted_projection(x, projection, index) for x in xs]
+    for _ in range(10):
+        for x, w in zip(xs, want):
+            assert torch.equal(kernels.adapted_projection(x, projection, index), w)
+
+
 @pytest.mark.parametrize("factor", [float("inf"), -float("inf"), float("nan")])
 @pytest.mark.parametrize("path", PATHS)
 def test_an_infinite_factor_reaches_its_own_rows_alone(cuda_device, path, factor):
@@ -260,3 +288,45 @@ def test_gates_of_every_size(cuda_device, dtype):
         got, _ = kernels.gated_residual_join(torch.ones_like(edge), torch.zeros_like(edge), gate=edge, gate_act=act)
         assert got[0, 0].isnan() and got[0, 1] == want[0]
         assert got[0, 2].isnan() if want[1] is None else got[0, 2] == want[1]
+
+
+def test_norm_and_join_past_32_bits(cuda_device):
+    """More than 2^31 elements of every operand; rows from the end are compared with the same rows by themselves."""
+    from nnunet_mlx_b200 import kernels
+
+    for channels in (16384, 40):
+        rows = (2 ** 31) // channels + 77
+        x = torch.empty((rows, channels), dtype=torch.bfloat16, device=cuda_device).normal_()
+        skip = torch.empty_like(x).normal_()
+        norm = kernels.ChannelNorm("layer", torch.linspace(0.5, 1.5, channels, device=cuda_device))
+        got = kernels.channel_norm(x, norm)
+        stream, normed = kernels.gated_residual_join(x, skip, post=norm, gate=x, gate_act="tanh", next_norm=norm)
+        for part in (slice(0, 50), slice(rows - 100, rows)):
+            assert torch.equal(got[part], kernels.channel_norm(x[part].clone(), norm))
+            a, b = kernels.gated_residual_join(x[part].clone(), skip[part].clone(), post=norm, gate=x[part].clone(),
+                                               gate_act="tanh", next_norm=norm)
+            assert torch.equal(stream[part], a) and torch.equal(normed[part], b)
+        del x, skip, got, stream, normed
+
+
+def test_narrow_projection_past_32_bits(cuda_device):
+    from nnunet_mlx_b200 import kernels
+
+    rng = np.random.default_rng(30)
+    for ranks, per_row in (([4, 7], True), ([16, 9], False)):
+        rows = 2 ** 26 + 6 * 77
+        parts = problem(rng, 32, 40, ranks, "bf16", cuda_device)
+        projection = kernels.pack_projection(parts[0], parts[1], bias=parts[2])
+        x = torch.empty((rows, 32), dtype=torch.bfloat16, device=cuda_device).normal_()
+        if per_row:
+            index = torch.arange(rows, device=cuda_device).remainder_(3).sub_(1).int()
+            got = kernels.adapted_projection(x, projection, index)
+        else:
+            index = torch.tensor([1, 0], dtype=torch.int32, device=cuda_device)
+            got = kernels.adapted_projection(x.view(2, -1, 32), projection, index).view(rows, 40)
+            index = index.repeat_interleave(rows // 2)
+        for part in (slice(0, 500), slice(rows // 2 - 300, rows // 2 + 300), slice(rows - 500, rows)):
+            want = kernels.adapted_projection(x[part].clone(), projection, index[part].clone())
+            assert torch.equal(got[part], want)
+        check(x[-500:], parts, index[-500:].clone(), projection)
+        del x, got

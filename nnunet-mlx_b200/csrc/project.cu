@@ -230,7 +230,6 @@ __global__ void __launch_bounds__(128) project_low_kernel(const nnb_project_args
   const int64_t row = blockIdx.x;
   const int adapter = row_adapter(a, row);
   if (adapter < 0) return;
-  const float2 own = factor(a, adapter);
   const int lane = threadIdx.x & 31, j0 = blockIdx.y * 16 + (threadIdx.x >> 5) * 4;
   const T* x = reinterpret_cast<const T*>(a.x) + row * a.x_stride;
   const T* down = reinterpret_cast<const T*>(a.down) + ((int64_t)adapter * a.rank + j0) * a.weight_stride;
@@ -253,6 +252,7 @@ __global__ void __launch_bounds__(128) project_low_kernel(const nnb_project_args
 #pragma unroll
     for (int j = 0; j < 4; ++j) sum[j] = fmaf(v, value(down[j * a.weight_stride + whole + lane]), sum[j]);
   }
+  const float2 own = factor(a, adapter);
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
 #pragma unroll

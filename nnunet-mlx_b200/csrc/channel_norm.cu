@@ -1,5 +1,5 @@
 // Norms over the channels of channels-last rows (voxels or tokens), before a
-// block and after it: nnb_channel_norm and nnb_gated_join.
+// block and after it: nnb_channel_norm_rows and nnb_gated_join.
 //
 //   norm(v)  rms:   v * rsqrt(mean v^2 + eps) * w + b
 //            layer: (v - mean) * rsqrt(mean (v - mean)^2 + eps) * w + b
@@ -17,7 +17,7 @@
 //
 // Two things keep the loads coming while a row's sums and products are taken:
 // the next row's operands are on their way before the present one's are used
-// (up to two chunks a thread), and rows of one chunk a thread keep their
+// (up to three chunks a thread), and rows of one chunk a thread keep their
 // per-channel parameters in registers (from L1 they were more bytes than the
 // row itself, and the instructions to fetch them what bound the short rows).
 #include <cuda_bf16.h>
@@ -451,7 +451,8 @@ int launch_rows(K kernel, int (&resident)[64], const A& a, cudaStream_t stream) 
 
 // Threads that an SM should hold, by which the compiler bounds a kernel's registers (it is what bounds rows of a few
 // warps: joins of 1280 channels 85% of a copy's rate at 512 threads, 94% at 640; float32 norms of 8192 channels 85% at
-// 512, 98% at 1024).  Where that would spill a row's values, fewer.
+// 512, 98% at 1024).  Where that would spill a row's values, fewer; rows of more than 4096 channels that are not aligned
+// spill all the same (joins 24 to 404 bytes a thread, beyond 8192 channels up to 766).
 template <class M>
 constexpr int norm_threads() {
   if (M::kAligned) return M::kChunks == 3 ? 640 : M::kChunks == 2 && M::kTpr <= 32 ? 896 : 1024;

@@ -83,8 +83,8 @@ struct Tile {
   static constexpr int kStage = kStageA + kStageB;
   static constexpr int kPlane = BN / kPeers * 64;  // one part of up: 64-byte rows of 32 ranks
   static constexpr int kLowStage = kStageA + kPlane * (kF16 ? 2 : 1);
-  // As shared memory allows.  (Narrow tiles with 4 of W's and 4 of adapters' stages: 256 rows of 64 adapters of rank 64,
-  // 1024 -> 1024, 65 us instead of 70, but of one adapter, 4096 -> 4096, 26.7 instead of 22.0.)
+  // As shared memory allows.  (Narrow tiles with 4 of W's and 4 of adapters' stages: 256 rows, each of another request,
+  // 64 adapters of rank 64, 1024 -> 1024, 65 us instead of 70, but of one adapter, 4096 -> 4096, 26.7 instead of 22.0.)
   static constexpr int kStages = BN == 64 ? 6 : 4;
   static constexpr int kLowStages = 2;
   static constexpr int kStaging = 32 * 32 * 2;  // an epilogue warp's 32 rows of 32 columns
@@ -189,10 +189,6 @@ __device__ __forceinline__ uint8_t* low_row(const nnb_project_args& a, int64_t r
   return reinterpret_cast<uint8_t*>(a.low) + row * ((a.rank + kRankBlock - 1) / kRankBlock) * 128;
 }
 
-// ---------------------------------------------------------------------------
-// low[p][t][j] = scale_a sum over part p of k of down_a[j][k] x[t][k]: a warp takes four ranks of one row.  PACKED:
-// of all of k, as hi and lo parts.
-// ---------------------------------------------------------------------------
 // 32 TMEM columns of this thread's lane, asked for and waited for apart.
 __device__ __forceinline__ void tmem_load32(uint32_t taddr, uint32_t (&r)[32]) {
   asm volatile(
@@ -224,6 +220,10 @@ __device__ __forceinline__ void widen(float (&v)[8], const uint4& raw) {
   for (int i = 0; i < 8; ++i) v[i] = value(t[i]);
 }
 
+// ---------------------------------------------------------------------------
+// low[p][t][j] = scale_a sum over part p of k of down_a[j][k] x[t][k]: a warp takes four ranks of one row.  PACKED:
+// of all of k, as hi and lo parts.
+// ---------------------------------------------------------------------------
 template <typename T, bool PACKED>
 __global__ void __launch_bounds__(128) project_low_kernel(const nnb_project_args a, const int part) {
   asm volatile("griddepcontrol.launch_dependents;");
@@ -327,10 +327,6 @@ __device__ __forceinline__ uint32_t in_first_cta(uint32_t at) {
   uint32_t remote;
   asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(remote) : "r"(at));
   return remote;
-}
-
-__device__ __forceinline__ void mbar_expect_tx(uint32_t bar, uint32_t bytes) {
-  asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
 
 __device__ __forceinline__ void mma_f16(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
@@ -1452,8 +1448,8 @@ bool rows_in_place(const nnb_project_args& a) {
          (a.rows == 1 || (a.x_stride % 8 == 0 && a.x_stride >= a.k));
 }
 
-// (Two million rows, by this kernel and by tiles: 32 -> 32 channels of rank 8 54 and 533 us, 64 -> 64 of rank 16 146
-// and 564, 128 -> 128 of rank 16 455 and 616.)
+// (Two million rows of two samples, by this kernel and by tiles: 32 -> 32 channels of rank 8 51 and 396 us, 64 -> 64 of
+// rank 16 146 and 454, 128 -> 128 of rank 16 422 and 495.)
 bool narrow(const nnb_project_args& a) { return a.k <= 128 && a.n <= 128; }
 
 // Plans are made for a whole B200, so that the workspace's size needs no device.
@@ -1477,9 +1473,10 @@ struct LowPlan {
 };
 
 // By rows beyond a tile too, where a tile may hold so many adapters that its passes over them take longer: some 0.8 us
-// for 64 ranks against 250 ns for a million products.  Whole calls by tiles and by rows: 256 rows, 1024 -> 1024, rank
-// 16, 64 adapters 42.2 and 22.0 us, 8 adapters 13.4 and 11.1; 160 rows, 4096 -> 4096, 64 adapters 72.5 and 48.3 us; 1024
-// rows of them, near the bound, 56.8 and 56.9.
+// for 64 ranks against 250 ns for a million products.  Calls by tiles and by rows, adapters of rank 16: 256 rows of 64
+// requests, 1024 -> 1024, 64 adapters 43.6 and 22.8 us, and where each row is another request's 80.4 and 40.1; of 8
+// requests and adapters 13.8 and 11.1; 160 rows of as many requests, 4096 -> 4096, 64 adapters 107 and 55; 1024 rows of 64
+// requests, 1024 -> 1024, 24.4 and 17.2.
 bool low_by_rows(const nnb_project_args& a) {
   const int64_t ranks = std::min<int64_t>(a.adapters, BM) * a.rank;
   return a.rows <= 8 * BM && a.rows * a.rank * a.k / 4000 < ranks * 800 / 64;
@@ -1694,9 +1691,10 @@ int tile_columns(const nnb_project_args& a, int sms) {
 // accumulators are the A fragments of the product with up_a, as two bfloat16
 // parts; rows of other requests are zeroed there, once per adapter among the
 // warp's rows.  No stage or barrier stands between x and out.  32 channels are
-// bound by HBM (82% of a copy's rate); from 64 on the rate of these MMAs and the
-// registers bound it (64 channels 57%, 128 channels 37%), still ahead of tiles,
-// whose K axis is padded to whole chunks and whose epilogue goes through TMEM.
+// bound by HBM (83% of a copy's rate); from 64 on the rate of these MMAs and the
+// registers bound it (64 channels 57%, 128 channels 39%; 3 and 4 groups spill),
+// still ahead of project_kernel, whose K axis is padded to whole chunks and whose
+// epilogue goes through TMEM.
 // ---------------------------------------------------------------------------
 // d = a b + c of 16 rows, 8 columns and 16 channels.
 __device__ __forceinline__ void warp_mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, float c0,

@@ -1160,7 +1160,7 @@ def gated_residual_join(branch: torch.Tensor, skip: torch.Tensor, *, post: Chann
                             f"got {skip.dtype}")
     if gate_act not in _GATE_ACTS:
         raise ContractError(f"unknown gate activation {gate_act!r}: one of {', '.join(_GATE_ACTS)}")
-    if _FLOAT32_MAX < abs(residual_scale) < math.inf:
+    if abs(residual_scale) > _FLOAT32_MAX and abs(residual_scale) != math.inf:
         raise ContractError(f"residual_scale {residual_scale} leaves float32's range")
     channels = shape[-1]
     scale_pointer = _channels_pointer(scale, "scale", channels, device)
@@ -1259,7 +1259,8 @@ def pack_projection(weight: torch.Tensor, adapters: list[Adapter],
 
     ``weight`` is bfloat16 or float16, ``bias`` float32 ``(N,)``.  The packed
     tensors are copies: later changes of the originals do not reach them.
-    Adapters may differ in rank (1 to 256) and must be finite, since a tile of
+    Adapters may differ in rank (1 to 256), but each takes the memory, and a call
+    the time, of the largest rank among them.  They must be finite, since a tile of
     rows of several requests multiplies each adapter by the others' zeros
     (read once here, which synchronises); so must their scales, in float32.
     Tensors that require a gradient are packed under ``torch.no_grad()`` only:
@@ -1333,9 +1334,9 @@ def adapted_projection(x: torch.Tensor, projection: AdaptedProjection, index: to
     if x.dtype != weight.dtype or device != weight.device or shape[-1] != projection.in_channels:
         raise ContractError(f"x must hold {projection.in_channels} {weight.dtype} channels on {weight.device}, got "
                             f"{tuple(shape)} {x.dtype} on {device}")
-    axes = index.dim() if isinstance(index, torch.Tensor) else 0
-    if not axes:
+    if not isinstance(index, torch.Tensor):
         raise ContractError(f"index must be a contiguous int32 tensor over leading axes of {tuple(shape)} on {device}")
+    axes = index.dim()
     if index.dtype != torch.int32 or not index.is_contiguous() or index.device != device \
             or not 1 <= axes < len(shape) or index.shape != shape[:axes]:
         raise ContractError(f"index must be a contiguous int32 tensor over leading axes of {tuple(shape)} on {device}, "

@@ -330,3 +330,15 @@ def test_narrow_projection_past_32_bits(cuda_device):
             assert torch.equal(got[part], want)
         check(x[-500:], parts, index[-500:].clone(), projection)
         del x, got
+
+
+@pytest.mark.parametrize("index", [None, [0, 0, 0, 0], 0])
+def test_an_index_that_is_no_tensor_is_refused(cuda_device, index):
+    from nnunet_mlx_b200 import kernels
+    from nnunet_mlx_b200.errors import ContractError
+
+    rng = np.random.default_rng(31)
+    weight, adapters, _ = problem(rng, 32, 32, [8], "bf16", cuda_device)
+    projection = kernels.pack_projection(weight, adapters)
+    with pytest.raises(ContractError, match="index must be"):
+        kernels.adapted_projection(make_rows(rng, (4, 32), "bf16", cuda_device), projection, index)

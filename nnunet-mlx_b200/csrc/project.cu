@@ -2151,16 +2151,17 @@ int launch_project(nnb_project_args a, cudaStream_t stream) {
 }  // namespace
 
 // The projection's device status (see nnb_device_status); the device is idle.
-int project_device_status(int32_t* where, bool reset) {
+int project_device_status(int32_t* where) {
   int status = 0;
   NNB_CUDA_CHECK(cudaMemcpyFromSymbol(&status, g_device_status, sizeof(int)));
   NNB_CUDA_CHECK(cudaMemcpyFromSymbol(where, g_device_status_where, sizeof(int)));
-  if (reset && status != 0) {
-    const int zero = 0;
-    NNB_CUDA_CHECK(cudaMemcpyToSymbol(g_device_status, &zero, sizeof(int)));
-    NNB_CUDA_CHECK(cudaMemcpyToSymbol(g_device_status_where, &zero, sizeof(int)));
-  }
   return status;
+}
+
+void clear_project_device_status() {
+  const int zero = 0;
+  cudaMemcpyToSymbol(g_device_status, &zero, sizeof(int));
+  cudaMemcpyToSymbol(g_device_status_where, &zero, sizeof(int));
 }
 
 }  // namespace nnb

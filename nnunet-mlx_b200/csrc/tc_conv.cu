@@ -72,6 +72,7 @@
 #include <stdint.h>
 
 #include "common.cuh"
+#include "device_status.cuh"
 
 namespace nnb {
 __device__ int g_device_status = 0;
@@ -1980,21 +1981,35 @@ int launch_conv_transpose_tc(const nnb_segment& in, int batch, const int32_t in_
 }  // namespace nnb
 
 namespace nnb {
-int project_device_status(int32_t* where, bool reset);  // project.cu
+// project.cu's
+int project_device_status(int32_t* where);
+void clear_project_device_status();
+
+namespace {
+
+int conv_device_status(int32_t* where) {
+  int status = 0;
+  NNB_CUDA_CHECK(cudaMemcpyFromSymbol(&status, g_device_status, sizeof(int)));
+  NNB_CUDA_CHECK(cudaMemcpyFromSymbol(where, g_device_status_where, sizeof(int)));
+  return status;
 }
 
+void clear_conv_device_status() {
+  const int zero = 0;
+  cudaMemcpyToSymbol(g_device_status, &zero, sizeof(int));
+  cudaMemcpyToSymbol(g_device_status_where, &zero, sizeof(int));
+}
+
+}  // namespace
+}  // namespace nnb
+
 extern "C" int32_t nnb_device_status(int32_t* where, int32_t reset) {
-  int status = 0, loc = 0;
   if (cudaDeviceSynchronize() != cudaSuccess) return NNB_E_CUDA;
-  if (cudaMemcpyFromSymbol(&status, nnb::g_device_status, sizeof(int)) != cudaSuccess) return NNB_E_CUDA;
-  cudaMemcpyFromSymbol(&loc, nnb::g_device_status_where, sizeof(int));
-  if (reset && status != 0) {
-    const int zero = 0;
-    cudaMemcpyToSymbol(nnb::g_device_status, &zero, sizeof(int));
-    cudaMemcpyToSymbol(nnb::g_device_status_where, &zero, sizeof(int));
-  }
-  // one error at a time: the projection's stays for the next call where the convolutions have one
-  if (status == 0) status = nnb::project_device_status(&loc, reset != 0);
+  int loc = 0;
+  const int status = nnb::first_error(
+      2, reset != 0, &loc,
+      [](int i, int* at) { return i == 0 ? nnb::conv_device_status(at) : nnb::project_device_status(at); },
+      [](int i) { i == 0 ? nnb::clear_conv_device_status() : nnb::clear_project_device_status(); });
   if (where) *where = loc;
   return status;
 }
